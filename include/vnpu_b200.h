@@ -284,6 +284,147 @@ typedef struct vnpu_b200_matmul_i8_swiglu_args_t {
 } vnpu_b200_matmul_i8_swiglu_args_t;
 
 /*
+ * A paged key/value cache in 8 bits for many sequences (no reference
+ * counterpart: the reference has no KV cache).  K and V hold int8 codes,
+ * [num_pages][heads][page_size][head_dim]; K_scale and V_scale one f32 for
+ * each page and head, [num_pages][heads]; a cached value is code * scale.
+ * All four are device memory, owned by the caller, the codes 16-byte aligned;
+ * nothing needs to be cleared before a page's first use.  page_size is a power
+ * of two from 16 to 256, head_dim a multiple of 16 up to 256.
+ */
+typedef struct vnpu_b200_paged_cache_t {
+    int8_t *K;
+    int8_t *V;
+    float *K_scale;
+    float *V_scale;
+    uint32_t num_pages;
+    uint32_t heads;        /* key/value heads */
+    uint32_t page_size;    /* tokens */
+    uint32_t head_dim;
+} vnpu_b200_paged_cache_t;
+
+/*
+ * The sequences a paged command works on, and their rows.  Sequence b has rows
+ * cu_tokens[b] .. cu_tokens[b+1]-1 of the command's row arrays (none, one or
+ * many; cu_tokens[0] = 0, not falling, at most `tokens`), which are its LAST
+ * tokens: with n_b rows, row i has position seq_lens[b] - n_b + i.  The token
+ * at position p lies in slot p % page_size of page
+ * block_table[b][p / page_size].  Table entries past a sequence's length are
+ * not read.  The three arrays are read when the command runs, so a captured
+ * graph follows them.  max_tokens, when not 0, is a bound on every n_b; with 1
+ * the command takes its single-token form.
+ *
+ * What the arrays say is checked on the device: a sequence whose rows exceed
+ * max_tokens, `tokens` or its length, or a page outside the cache or the
+ * table, is not touched (its cached tokens and outputs that would depend on
+ * them are left out or zero) and sets the stream's device error.  tokens = 0
+ * or batch = 0 is no work.
+ */
+typedef struct vnpu_b200_paged_batch_t {
+    const int32_t *block_table;   /* [batch][table_stride] */
+    const int32_t *cu_tokens;     /* [batch + 1] */
+    const int32_t *seq_lens;      /* [batch], with the command's rows counted in */
+    uint32_t batch;
+    uint32_t table_stride;        /* entries between block_table rows */
+    uint32_t tokens;              /* rows of the command's row arrays */
+    uint32_t max_tokens;          /* bound on a sequence's rows; 0 = tokens */
+} vnpu_b200_paged_batch_t;
+
+/*
+ * Appends the rows' keys and values to a paged cache, rotating queries and
+ * keys on the way.  Q, K and V are rows of [heads][head_dim] elements of
+ * `dtype` (VNPU_DTYPE_F32, F16 or BF16) with row strides ldq, ldk, ldv in
+ * elements (0 = dense), so the parts of one projection's [Q | K | V] rows are
+ * read in place.  Q_out (row stride ldqo) receives the rotated queries in the
+ * same type; it may be Q.  Q and Q_out may both be NULL.
+ *
+ * Rotation: pair j of the first rotary_dim elements (0 = head_dim; a multiple
+ * of 16) turns by position * scaling * theta_base^(-2j/rotary_dim); pairs are
+ * (j, j + rotary_dim/2), or (2j, 2j+1) with VNPU_B200_PAGED_INTERLEAVED; none
+ * turn with VNPU_B200_PAGED_NO_ROPE.  The angle is position times a 64-bit
+ * count of 2^-64 turns, modulo one turn, so it is as exact at a position of
+ * millions as at 1 (ROPE_F32 multiplies in 32 bits, as the reference does; at
+ * short positions the two agree to that rounding).
+ *
+ * Quantization: for each page that receives tokens, and each head, the scale
+ * becomes max(scale so far, max |new values| / 127), where a page whose slot 0
+ * is written now has no scale so far; new codes are value / scale to nearest
+ * (ties to even), and where the scale grew the page's older codes are rounded
+ * to it once.  A NaN is stored as 0 and an infinity as the largest code, and
+ * neither counts toward the scale.  Two sequences must not append to one page
+ * in one command.
+ */
+#define VNPU_B200_OP_PAGED_KV_APPEND  0x109u
+#define VNPU_B200_PAGED_INTERLEAVED   (1u << 0)
+#define VNPU_B200_PAGED_NO_ROPE       (1u << 1)
+
+typedef struct vnpu_b200_paged_kv_append_args_t {
+    vnpu_b200_paged_cache_t cache;
+    vnpu_b200_paged_batch_t batch;
+    const void *Q;
+    const void *K;
+    const void *V;
+    void *Q_out;
+    uint32_t ldq, ldk, ldv, ldqo;
+    uint32_t q_heads;
+    uint32_t dtype;
+    uint32_t flags;        /* VNPU_B200_PAGED_* */
+    uint32_t rotary_dim;
+    float theta_base;      /* <= 0: 10000 */
+    float scaling;         /* <= 0: 1 */
+} vnpu_b200_paged_kv_append_args_t;
+
+/*
+ * Cached tokens back as values: row r of K_out and V_out ([tokens][heads]
+ * [head_dim] elements of `dtype`, element (r, h, d) at r * ld_row + h * ld_head
+ * + d; 0 and 0 = dense) receives code * scale of the row's token, rounded once.
+ * Either output may be NULL.  With ld_row = head_dim and ld_head = tokens *
+ * head_dim the result is the head-major layout of ATTENTION_F32.
+ */
+#define VNPU_B200_OP_PAGED_KV_READ  0x10au
+
+typedef struct vnpu_b200_paged_kv_read_args_t {
+    vnpu_b200_paged_cache_t cache;
+    vnpu_b200_paged_batch_t batch;
+    void *K_out;
+    void *V_out;
+    uint64_t ld_row;
+    uint64_t ld_head;
+    uint32_t dtype;
+    uint32_t reserved0;
+} vnpu_b200_paged_kv_read_args_t;
+
+/*
+ * Attention of the rows' queries to their sequence's cached tokens (the rows'
+ * own, appended before, among them).  Q and O are rows of [q_heads][head_dim]
+ * elements of `dtype` (row strides ldq, ldo in elements, 0 = dense; O may be
+ * Q); query head h reads key/value head h / (q_heads / heads), q_heads being a
+ * multiple of heads.  A query at position p attends to the positions j <
+ * seq_lens[b], with `causal` j <= p, with window w > 0 also j > p - w:
+ * O = sum_j softmax_j(scale * q.k_j) v_j (scale 0 = 1/sqrt(head_dim)).  A query
+ * that attends to nothing has the output 0.  Scores, softmax sums and
+ * accumulators are 32 bits wide; the softmax weights enter the value product
+ * as 16-bit floats for 16-bit outputs, and as two of them (22 bits) for f32.
+ * max_length, when not 0, is the longest seq_lens[b] to expect; it only
+ * chooses how the work is split.
+ */
+#define VNPU_B200_OP_PAGED_ATTENTION  0x10bu
+
+typedef struct vnpu_b200_paged_attention_args_t {
+    vnpu_b200_paged_cache_t cache;
+    vnpu_b200_paged_batch_t batch;
+    const void *Q;
+    void *O;
+    uint32_t ldq, ldo;
+    uint32_t q_heads;
+    uint32_t dtype;
+    uint32_t causal;
+    uint32_t window;
+    uint32_t max_length;
+    float scale;
+} vnpu_b200_paged_attention_args_t;
+
+/*
  * MATMUL_I8 of one column shard of a wider product (no reference
  * counterpart; the reference has no int8 multi-device split).  B holds the
  * shard's N columns, which are columns col_base .. col_base + N - 1 of an

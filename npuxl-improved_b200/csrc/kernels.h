@@ -18,6 +18,7 @@ enum DeviceError : uint32_t {
     kErrWaitTimeout = 1u << 0,   // an mbarrier / flag wait ran out of time
     kErrBadConfig = 1u << 1,     // a kernel saw a launch shape it cannot run
     kErrTmemAlloc = 1u << 2,     // tensor memory allocation returned nonsense
+    kErrBadIndex = 1u << 3,      // a device-side index (row, page, length) outside its array
 };
 
 // Dequant epilogue forms (vnpu_b200.h: block / stream / scalar); kFormMixed
@@ -240,6 +241,56 @@ cudaError_t attention(const LaunchCtx &ctx, const float *Q, const float *K, cons
                       const float *mask, float *O, uint32_t batch, uint32_t heads,
                       uint32_t seq_q, uint32_t seq_k, uint32_t head_dim, uint32_t causal,
                       float scale, bool o_token_major = false);
+
+// ---- paged 8-bit key/value cache (vnpu_b200.h) ----------------------------------
+enum class RowType : uint32_t { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+struct PagedCache {
+    int8_t *K = nullptr, *V = nullptr;             // [num_pages][heads][page_size][head_dim]
+    float *K_scale = nullptr, *V_scale = nullptr;  // [num_pages][heads]
+    uint32_t num_pages = 0, heads = 0, page_shift = 0, head_dim = 0;
+};
+struct PagedBatch {
+    const int32_t *table = nullptr;  // [batch][table_stride]
+    const int32_t *cu = nullptr;     // [batch + 1]
+    const int32_t *lens = nullptr;   // [batch]
+    uint32_t batch = 0, table_stride = 0, tokens = 0, max_tokens = 0;
+};
+struct PagedAppend {
+    PagedCache cache;
+    PagedBatch batch;
+    const void *Q = nullptr, *K = nullptr, *V = nullptr;
+    void *Q_out = nullptr;
+    uint32_t ldq = 0, ldk = 0, ldv = 0, ldqo = 0, q_heads = 0;
+    RowType type = RowType::kF32;
+    bool interleaved = false;
+    uint32_t rotary = 0;             // rotated elements of a head; 0 = none
+    const uint64_t *turns = nullptr; // host, rotary / 2 entries: 2^-64 turns per position
+};
+cudaError_t paged_kv_append(const LaunchCtx &ctx, const PagedAppend &p);
+
+struct PagedRead {
+    PagedCache cache;
+    PagedBatch batch;
+    void *K_out = nullptr, *V_out = nullptr;
+    uint64_t ld_row = 0, ld_head = 0;
+    RowType type = RowType::kF32;
+};
+cudaError_t paged_kv_read(const LaunchCtx &ctx, const PagedRead &p);
+
+struct PagedAttention {
+    PagedCache cache;
+    PagedBatch batch;
+    const void *Q = nullptr;
+    void *O = nullptr;
+    uint32_t ldq = 0, ldo = 0, q_heads = 0;
+    RowType type = RowType::kF32;
+    bool causal = true;
+    uint32_t window = 0;             // 0 = none
+    uint32_t max_length = 0;         // expected longest sequence; 0 = the table's reach
+    float scale = 1.0f;
+};
+cudaError_t paged_attention(const LaunchCtx &ctx, const PagedAttention &p);
 
 // ---- device-wait self test -------------------------------------------------------
 cudaError_t wait_timeout_probe(const LaunchCtx &ctx, const uint32_t *flag, uint64_t limit_ns);

@@ -1,0 +1,751 @@
+// paged_attention.cu - attention over the paged 8-bit key/value cache
+// (VNPU_B200_OP_PAGED_ATTENTION): the kernel for few query rows, which is
+// right for every shape, and the dispatch.
+//
+// The mathematics.  Scores are s_j = (q . c_j) * K_scale * scale with the int8
+// codes c_j.  A value scale is folded into the softmax weight: with
+//   t_j = s_j log2(e) + log2(V_scale of j),  m >= max t_j - 6,
+//   p_j = 2^(t_j - m + 8),  l = sum p_j / V_scale of j,  o = sum p_j code_j / l,
+// which is sum softmax(s)_j V_scale_j code_j: one addition a key and one
+// product a page instead of a product a value, and every p_j fits a 16-bit
+// float whatever the scales.  Codes are whole numbers below 128, exact in 16
+// bits, so both products run on f16 tensor instructions with nothing lost on
+// the cache's side.  A query row is scaled by a power of two to a largest
+// element in [2^13, 2^14): f16 and bf16 queries are then exact too (down to
+// 2^-27 of the row's largest), and f32 ones become hi + lo, 22 bits, as two
+// rows of the 16-row tile whose products are added; their weights p are split
+// the same way.  Sums, maxima and accumulators are f32.
+//
+// m follows the running maximum only when that has grown by more than 2^6, so
+// the accumulators are rescaled a few times a row instead of at every step.
+#include <algorithm>
+
+#include "paged_common.cuh"
+
+namespace vnpu_b200 {
+namespace {
+
+constexpr uint32_t kWarps = 4, kThreadsA = kWarps * 32;
+constexpr uint32_t kTile = 128;      // keys of a work unit, 32 for each warp
+constexpr uint32_t kWarpKeys = kTile / kWarps;
+constexpr float kSlack = 6.0f;       // growth of the maximum before a rescale (log2)
+constexpr float kLift = 8.0f;        // weights are scaled by 2^8: small ones stay normal numbers
+
+struct AttnParams {
+    PagedCache c;
+    PagedBatch pb;
+    const void *Q;
+    void *O;
+    uint32_t ldq, ldo, group;
+    uint32_t causal, window;
+    float scale_log2;
+    uint32_t vec;          // bit 0: Q 16-byte accesses, bit 1: O 4-element accesses
+    float *ws_o;           // [2 * grid][MR][DP] partial sums
+    float2 *ws_ml;         // [2 * grid][MR] their m and l
+    uint4 *ws_meta;        // [2 * grid]: who joins what
+    uint32_t *err;
+};
+
+template <uint32_t DP>
+struct AttnShape {
+    static constexpr uint32_t kStages = DP == 64 ? 6 : 3;
+    static constexpr uint32_t kSlot = kWarpKeys * DP * 2;   // a warp's K and V codes of a unit
+    static constexpr uint32_t kSmem = kWarps * kStages * kSlot;
+    static constexpr uint32_t kCtasPerSm = DP == 256 ? 1 : 2;
+};
+// A slot also takes a warp's 16 x DP f32 accumulators when warps are joined.
+static_assert(AttnShape<128>::kSlot == 16 * 128 * 4, "a slot holds a warp's accumulators");
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ float quad_max(float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+
+// The units (sequence, head, row tile, key tile) in that order, the last
+// fastest: where a CTA stands in them.
+struct Cursor {
+    uint32_t b, h, rt;      // sequence, key/value head, row tile
+    int32_t tile;           // key tile, lo <= tile < lo + nt
+    int32_t lo, nt;
+    uint32_t rts;           // row tiles of the sequence
+    PagedSeq s;
+};
+
+// Row tiles and key tiles of a sequence; 0 row tiles when it has no rows (or
+// bad numbers, which *bad reports).  An empty range of keys counts one tile, in
+// which everything is masked, so that its rows are written.
+template <uint32_t MR>
+__device__ __forceinline__ void seq_units(const AttnParams &p, uint32_t b, Cursor &k, bool *bad) {
+    k.b = b;
+    k.rts = 0;
+    k.lo = 0;
+    k.nt = 1;
+    const bool ok = load_seq(p.pb, p.c.page_shift, b, k.s);
+    *bad = !ok;
+    if (!ok || k.s.n == 0) return;
+    k.rts = (static_cast<uint32_t>(k.s.n) * p.group + MR - 1) / MR;
+    if (p.window && static_cast<uint32_t>(k.s.start) + 1u > p.window)
+        k.lo = (k.s.start + 1 - static_cast<int32_t>(p.window)) / static_cast<int32_t>(kTile);
+    const int32_t hi = (k.s.len + static_cast<int32_t>(kTile) - 1) / static_cast<int32_t>(kTile);
+    k.nt = max(1, hi - k.lo);
+}
+
+// The next unit; loads the next sequence that has rows where one ends (the
+// caller stops before the last unit's successor is asked for).
+template <uint32_t MR>
+__device__ __forceinline__ void next_unit(const AttnParams &p, Cursor &k) {
+    if (++k.tile < k.lo + k.nt) return;
+    if (++k.rt < k.rts) {
+        k.tile = k.lo;
+        return;
+    }
+    k.rt = 0;
+    if (++k.h < p.c.heads) {
+        k.tile = k.lo;
+        return;
+    }
+    k.h = 0;
+    bool bad;
+    uint32_t b = k.b;
+    do {
+        if (++b >= p.pb.batch) break;
+        seq_units<MR>(p, b, k, &bad);
+    } while (k.rts == 0);
+    k.tile = k.lo;
+}
+
+// Persistent CTAs, each with an equal run of units: sequences of any lengths
+// give every CTA the same work, and a (sequence, head, row tile) is split over
+// CTAs only where runs meet.  A warp keeps kStages - 1 units in flight through
+// its own ring of cp.async copies (no CTA-wide waits within a run), across
+// the ends of sequences too.
+template <RowType T, uint32_t DP>
+__global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
+    paged_attention_kernel(const AttnParams p, const uint32_t min_units) {
+    using E = typename RowOf<T>::type;
+    using Shape = AttnShape<DP>;
+    constexpr bool kSplit = T == RowType::kF32;
+    constexpr uint32_t MR = kSplit ? 8 : 16;       // query rows of a tile
+    constexpr uint32_t S = Shape::kStages, NC = DP / 16, NG = DP / 64, NJ = DP / 8;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float sh_scale[kWarps][S][4];       // K_scale and V_scale of a unit's 16-key groups
+    __shared__ float2 sh_ml[kWarps][16];
+    __shared__ unsigned long long sh_sum[kWarps];
+    __shared__ uint32_t sh_b;
+    __shared__ unsigned long long sh_off;
+    pdl_enter();
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, n = lane >> 2, kq = lane & 3u;
+    const uint32_t D = p.c.head_dim, cta = blockIdx.x;
+
+    // ---- this CTA's run of units
+    const uint32_t per_thread = (p.pb.batch + kThreadsA - 1) / kThreadsA;
+    const uint32_t b_lo = min(tid * per_thread, p.pb.batch), b_hi = min(b_lo + per_thread, p.pb.batch);
+    unsigned long long mine = 0;
+    Cursor cur;
+    for (uint32_t b = b_lo; b < b_hi; ++b) {
+        bool bad;
+        seq_units<MR>(p, b, cur, &bad);
+        if (bad) record_error(p.err, kErrBadIndex);
+        mine += static_cast<unsigned long long>(cur.rts) * p.c.heads * cur.nt;
+    }
+    unsigned long long upto = mine;
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) sh_sum[warp] = upto;
+    __syncthreads();
+    unsigned long long total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+        if (w < warp) upto += sh_sum[w];
+        total += sh_sum[w];
+    }
+    unsigned long long run = (total + gridDim.x - 1) / gridDim.x;
+    if (run < min_units) run = min_units;
+    const unsigned long long t0 = run * cta;
+    if (t0 >= total) {
+        if (tid == 0 && p.ws_meta) p.ws_meta[2 * cta].x = 0;
+        return;
+    }
+    uint32_t left = static_cast<uint32_t>(min(run, total - t0));  // units of this CTA
+    unsigned long long before = upto - mine;
+    if (before <= t0 && t0 < upto) {
+        for (uint32_t b = b_lo; b < b_hi; ++b) {
+            bool bad;
+            seq_units<MR>(p, b, cur, &bad);
+            const unsigned long long w = static_cast<unsigned long long>(cur.rts) * p.c.heads * cur.nt;
+            if (t0 < before + w) {
+                sh_b = b;
+                sh_off = t0 - before;
+                break;
+            }
+            before += w;
+        }
+    }
+    __syncthreads();
+    {
+        bool bad;
+        seq_units<MR>(p, sh_b, cur, &bad);
+        const unsigned long long off = sh_off;
+        const unsigned long long nt = static_cast<uint32_t>(cur.nt), row_tile = off / nt;
+        cur.h = static_cast<uint32_t>(row_tile / cur.rts);
+        cur.rt = static_cast<uint32_t>(row_tile - static_cast<unsigned long long>(cur.h) * cur.rts);
+        cur.tile = cur.lo + static_cast<int32_t>(off - row_tile * nt);
+    }
+    Cursor ahead = cur;         // the unit to copy next
+    uint32_t ahead_left = left;
+    uint32_t slot_in = 0;
+
+    uint8_t *const ring = smem + warp * (S * Shape::kSlot);
+
+    // Positions the row tile's first and last row see (the last row's limits
+    // are the widest above, the first row's the widest below).
+    const auto row_limits = [&](const Cursor &k, uint32_t r, int32_t &kmin, int32_t &kmax) {
+        const uint32_t rows = static_cast<uint32_t>(k.s.n) * p.group;
+        const int32_t pos = k.s.start + static_cast<int32_t>(min(r, rows - 1) / p.group);
+        kmax = p.causal ? pos : k.s.len - 1;
+        kmin = p.window && static_cast<uint32_t>(pos) + 1u > p.window ? pos + 1 - static_cast<int32_t>(p.window) : 0;
+    };
+    // Pages of the two 16-key groups of `ahead`'s part of this warp.
+    int32_t page_next[2];
+    const auto fetch_pages = [&]() {
+        if (ahead_left == 0) return;
+        const int32_t k0 = ahead.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int32_t key = k0 + 16 * i;
+            page_next[i] = key < ahead.s.len
+                               ? __ldg(p.pb.table + static_cast<uint64_t>(ahead.b) * p.pb.table_stride +
+                                       (static_cast<uint32_t>(key) >> p.c.page_shift))
+                               : -1;
+        }
+    };
+    const auto issue = [&]() {
+        if (ahead_left) {
+            const int32_t k0 = ahead.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
+            uint8_t *const dst = ring + slot_in * Shape::kSlot;
+            int32_t kmin0, kmax1, unused;
+            row_limits(ahead, ahead.rt * MR, kmin0, unused);
+            row_limits(ahead, ahead.rt * MR + MR - 1, unused, kmax1);
+            uint64_t base[2];
+            bool ok[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int32_t key = k0 + 16 * i;
+                // a group with nothing to see is left as it is
+                const bool live = key < ahead.s.len && key <= kmax1 && key + 16 > kmin0;
+                ok[i] = live && page_next[i] >= 0 && static_cast<uint32_t>(page_next[i]) < p.c.num_pages;
+                if (live && !ok[i] && lane == 0) record_error(p.err, kErrBadIndex);
+                const uint64_t at = ok[i] ? static_cast<uint64_t>(page_next[i]) * p.c.heads + ahead.h : 0;
+                base[i] = ((at << p.c.page_shift) + (static_cast<uint32_t>(key) & ((1u << p.c.page_shift) - 1u))) * D;
+                if (lane == i)
+                    cp_async_4_zfill(&sh_scale[warp][slot_in][i], p.c.K_scale + at, ok[i]);
+                if (lane == 2 + i)
+                    cp_async_4_zfill(&sh_scale[warp][slot_in][2 + i], p.c.V_scale + at, ok[i]);
+            }
+#pragma unroll
+            for (uint32_t q = 0; q < kWarpKeys * NC / 32; ++q) {
+                const uint32_t idx = lane + 32 * q, row = idx / NC, ch = idx % NC;
+                const uint32_t i = q / (16 * NC / 32);       // the row's 16-key group
+                const uint32_t sw = DP == 64 ? ch ^ ((row >> 1) & 3u) : ch ^ (row & 7u);
+                const bool in = ok[i] && k0 + static_cast<int32_t>(row) < ahead.s.len;
+                if (ch * 16u < D) {
+                    const uint64_t src = base[i] + (row & 15u) * D + ch * 16u;
+                    cp_async_16_zfill(dst + row * DP + sw * 16u, p.c.K + (in ? src : 0), in);
+                    cp_async_16_zfill(dst + kWarpKeys * DP + row * DP + sw * 16u, p.c.V + (in ? src : 0), in);
+                }
+            }
+            if (--ahead_left) next_unit<MR>(p, ahead);
+        }
+        cp_async_commit();
+        slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
+    };
+
+    fetch_pages();
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < S; ++i) {
+        issue();
+        fetch_pages();
+    }
+
+    // ---- state of the current (sequence, head, row tile)
+    uint32_t aq[NG][4][4];       // query fragments
+    float acc[NJ][4];
+    float m[2], l[2], qf[2];     // running maximum, sum, and score factor of rows n, n + 8
+    int32_t kmin[2], kmax[2], kmin_last = 0, kmax_first = 0, kmin_first = 0, kmax_last = 0;
+    int32_t first_tile = 0;
+    const auto begin_rows = [&]() {
+        first_tile = cur.tile;
+        const uint32_t rows = static_cast<uint32_t>(cur.s.n) * p.group;
+        row_limits(cur, cur.rt * MR, kmin_first, kmax_first);
+        row_limits(cur, cur.rt * MR + MR - 1, kmin_last, kmax_last);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            if (kSplit && i == 1) break;
+            const uint32_t r = cur.rt * MR + n + 8 * i;
+            row_limits(cur, r, kmin[i], kmax[i]);
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+            float v[NG][16];
+            float most = 0.0f;
+            const uint32_t token = r / p.group;
+            const E *q = static_cast<const E *>(p.Q) +
+                         static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldq +
+                         (cur.h * p.group + (r - token * p.group)) * D;
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g) {
+                const uint32_t d = 16u * (kq + 4u * g);
+#pragma unroll
+                for (uint32_t e = 0; e < 16; ++e) v[g][e] = 0.0f;
+                if (r < rows && d < D) {
+                    float x[8];
+                    load8(q + d, p.vec & 1u, x);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) v[g][e] = x[e];
+                    load8(q + d + 8, p.vec & 1u, x);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) v[g][8 + e] = x[e];
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 16; ++e) most = fmaxf(most, fabsf(v[g][e]));
+            }
+            most = quad_max(most);
+            // 2^k with most * 2^k in [2^13, 2^14); rows of zeros, and of infinities, stay
+            int ex = static_cast<int>((__float_as_uint(most) >> 23) & 255u) - 127;
+            ex = most > 0.0f && most <= 3.402823466e38f ? max(-114, min(100, 13 - ex)) : 0;
+            const float up = __int_as_float((127 + ex) << 23);
+            qf[i] = p.scale_log2 * __int_as_float((127 - ex) << 23);
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g)
+#pragma unroll
+                for (uint32_t s = 0; s < 4; ++s) {
+                    const float x0 = v[g][4 * s] * up, x1 = v[g][4 * s + 1] * up;
+                    const float x2 = v[g][4 * s + 2] * up, x3 = v[g][4 * s + 3] * up;
+                    aq[g][s][i] = pack_half2(x0, x1);
+                    aq[g][s][2 + i] = pack_half2(x2, x3);
+                    if constexpr (kSplit) {
+                        const float2 h0 = unpack_half2(aq[g][s][0]), h1 = unpack_half2(aq[g][s][2]);
+                        aq[g][s][1] = pack_half2(x0 - h0.x, x1 - h0.y);
+                        aq[g][s][3] = pack_half2(x2 - h1.x, x3 - h1.y);
+                    }
+                }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+    };
+
+    constexpr uint32_t NR = kSplit ? 1 : 2;      // rows of a thread
+    const auto compute = [&](uint32_t slot) {
+        const int32_t k0 = cur.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
+        if (k0 > kmax_last || k0 + static_cast<int32_t>(kWarpKeys) <= kmin_first) return;  // warp-uniform
+        const uint8_t *kb = ring + slot * Shape::kSlot, *vb = kb + kWarpKeys * DP;
+        const float *sc = sh_scale[warp][slot];
+        // scores of 4 x 8 keys: column c of tile 2i + tt is key 16i + 8tt + (c >> 1) + 4 (c & 1),
+        // so a thread's two columns are keys kq and kq + 4, the rows of V it reads below
+        float s[4][4];
+#pragma unroll
+        for (uint32_t t = 0; t < 4; ++t) {
+            s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
+            const uint32_t row = 8u * t + (n >> 1) + 4u * (n & 1u);
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g) {
+                const uint32_t ch = kq + 4u * g;
+                const uint32_t sw = DP == 64 ? ch ^ ((row >> 1) & 3u) : ch ^ (row & 7u);
+                const uint4 w = *reinterpret_cast<const uint4 *>(kb + row * DP + sw * 16u);
+                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    uint32_t b0, b1;
+                    codes_to_half4(word[e], b0, b1);
+                    mma_f16(s[t], aq[g][e][0], aq[g][e][1], aq[g][e][2], aq[g][e][3], b0, b1);
+                }
+            }
+        }
+        float lv[2], iv[2];
+        bool on[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float vs = sc[2 + i];
+            on[i] = vs > 0.0f;                 // a page of zeros has the scale 0
+            lv[i] = on[i] ? __log2f(vs) : 0.0f;
+            iv[i] = on[i] ? ex2(-lv[i]) : 1.0f;
+        }
+        const bool edge = k0 + static_cast<int32_t>(kWarpKeys) - 1 > kmax_first || k0 < kmin_last;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (uint32_t t = 0; t < 4; ++t)
+#pragma unroll
+            for (uint32_t r = 0; r < NR; ++r) {
+                const float f = qf[r] * sc[t >> 1];
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    float x = kSplit ? s[t][e] + s[t][2 + e] : s[t][2 * r + e];
+                    x = fmaf(x, f, lv[t >> 1]);
+                    if (edge) {
+                        const int32_t key = k0 + static_cast<int32_t>(8 * t + kq + 4 * e);
+                        if (key > kmax[r] || key < kmin[r]) x = -INFINITY;
+                    }
+                    s[t][2 * r + e] = x;
+                    top[r] = fmaxf(top[r], x);
+                }
+            }
+        bool grown = false;
+#pragma unroll
+        for (uint32_t r = 0; r < NR; ++r) {
+            top[r] = quad_max(top[r]);
+            grown |= top[r] > m[r] + kSlack;
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+            float f[2];
+#pragma unroll
+            for (uint32_t r = 0; r < NR; ++r) {
+                const float to = fmaxf(m[r], top[r]);
+                f[r] = to > m[r] ? ex2(m[r] - to) : 1.0f;
+                l[r] *= f[r];
+                m[r] = to;
+            }
+            const float f1 = kSplit ? f[0] : f[1];
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; ++j) {
+                acc[j][0] *= f[0];
+                acc[j][1] *= f[0];
+                acc[j][2] *= f1;
+                acc[j][3] *= f1;
+            }
+        }
+        float off[2];
+#pragma unroll
+        for (uint32_t r = 0; r < NR; ++r) off[r] = m[r] == -INFINITY ? 0.0f : m[r] - kLift;
+        uint32_t pa[2][4];
+#pragma unroll
+        for (uint32_t t = 0; t < 4; ++t)
+#pragma unroll
+            for (uint32_t r = 0; r < NR; ++r) {
+                const float x = ex2(s[t][2 * r] - off[r]), y = ex2(s[t][2 * r + 1] - off[r]);
+                l[r] = fmaf(x + y, iv[t >> 1], l[r]);
+                uint32_t h = pack_half2(x, y);
+                if constexpr (kSplit) {
+                    const float2 f = unpack_half2(h);
+                    uint32_t lo = pack_half2(x - f.x, y - f.y);
+                    if (!on[t >> 1]) h = lo = 0;
+                    pa[t >> 1][2 * (t & 1)] = h;
+                    pa[t >> 1][2 * (t & 1) + 1] = lo;
+                } else {
+                    if (!on[t >> 1]) h = 0;
+                    pa[t >> 1][2 * (t & 1) + r] = h;
+                }
+            }
+        // values: a thread's rows kq, +4, +8, +12 of a 16-key group and the dims of lane group n
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            constexpr uint32_t NW = DP / 32;       // words of a row for a thread
+            uint32_t w[4][NW];
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                const uint32_t row = 16u * i + kq + 4u * q;
+                if constexpr (DP == 64) {
+                    const uint32_t sw = (n >> 1) ^ ((row >> 1) & 3u);
+                    const uint2 x = *reinterpret_cast<const uint2 *>(vb + row * DP + sw * 16u + (n & 1u) * 8u);
+                    w[q][0] = x.x;
+                    w[q][1] = x.y;
+                } else {
+#pragma unroll
+                    for (uint32_t g = 0; g < DP / 128; ++g) {
+                        const uint32_t ch = 8u * g + (((n >> 1) + 4u * (n & 1u)) ^ (row & 7u));
+                        const uint4 x = *reinterpret_cast<const uint4 *>(vb + row * DP + ch * 16u);
+                        w[q][4 * g] = x.x;
+                        w[q][4 * g + 1] = x.y;
+                        w[q][4 * g + 2] = x.z;
+                        w[q][4 * g + 3] = x.w;
+                    }
+                }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < NW; ++k) {
+                uint32_t b0[4], b1[4];
+                codes_to_half4(__byte_perm(w[0][k], w[1][k], 0x5140), b0[0], b0[1]);
+                codes_to_half4(__byte_perm(w[0][k], w[1][k], 0x7362), b0[2], b0[3]);
+                codes_to_half4(__byte_perm(w[2][k], w[3][k], 0x5140), b1[0], b1[1]);
+                codes_to_half4(__byte_perm(w[2][k], w[3][k], 0x7362), b1[2], b1[3]);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    mma_f16(acc[4 * k + j], pa[i][0], pa[i][1], pa[i][2], pa[i][3], b0[j], b1[j]);
+            }
+        }
+    };
+
+    // The warps' sums of a row tile joined through their consumed slots, and
+    // written: as the output when this CTA saw all its keys, else as a part.
+    const auto end_rows = [&](uint32_t slot, bool more) {
+        const uint32_t rows = min(MR, static_cast<uint32_t>(cur.s.n) * p.group - cur.rt * MR);
+        float *const mine_o = reinterpret_cast<float *>(ring + slot * Shape::kSlot);
+#pragma unroll
+        for (uint32_t r = 0; r < NR; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (kq == 0) sh_ml[warp][n + 8 * r] = make_float2(m[r], l[r]);
+        }
+        __syncwarp();  // all lanes are done with the slot's codes
+#pragma unroll
+        for (uint32_t r = 0; r < NR; ++r) {
+            const uint32_t row = n + 8 * r;
+            if (row >= rows) continue;
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) {
+                // column 2 kq + e of tile j is dim j of the chunk that lane group 2 kq + e reads
+#pragma unroll
+                for (uint32_t j = 0; j < NJ; j += 4) {
+                    uint32_t d;
+                    if constexpr (DP == 64) d = 8u * (2u * kq + e) + j;
+                    else d = 128u * (j / 16u) + 16u * (kq + 4u * e) + j % 16u;
+                    float4 x;
+                    if constexpr (kSplit)
+                        x = make_float4(acc[j][e] + acc[j][2 + e], acc[j + 1][e] + acc[j + 1][2 + e],
+                                        acc[j + 2][e] + acc[j + 2][2 + e], acc[j + 3][e] + acc[j + 3][2 + e]);
+                    else
+                        x = make_float4(acc[j][2 * r + e], acc[j + 1][2 * r + e], acc[j + 2][2 * r + e],
+                                        acc[j + 3][2 * r + e]);
+                    reinterpret_cast<float4 *>(mine_o)[row * (DP / 4) + ((d / 4) ^ (row & 7u))] = x;
+                }
+            }
+        }
+        __syncthreads();
+        const bool started = first_tile == cur.lo;
+        const uint32_t part = 2 * cta + (started ? 1 : 0);
+        for (uint32_t i = tid; i < rows * (DP / 4); i += kThreadsA) {
+            const uint32_t row = i / (DP / 4), d4 = i % (DP / 4);
+            if (4u * d4 >= D) continue;
+            float2 ml[kWarps];
+            float mm = -INFINITY;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                ml[w] = sh_ml[w][row];
+                mm = fmaxf(mm, ml[w].x);
+            }
+            float4 o = make_float4(0, 0, 0, 0);
+            float ll = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                // a warp that saw no key holds zeros (or the NaN of its query): taken as they are
+                const float f = ml[w].x == -INFINITY ? 1.0f : ex2(ml[w].x - mm);
+                ll = fmaf(ml[w].y, f, ll);
+                const float4 x = reinterpret_cast<const float4 *>(
+                    smem + (w * S + slot) * Shape::kSlot)[row * (DP / 4) + (d4 ^ (row & 7u))];
+                o.x = fmaf(x.x, f, o.x);
+                o.y = fmaf(x.y, f, o.y);
+                o.z = fmaf(x.z, f, o.z);
+                o.w = fmaf(x.w, f, o.w);
+            }
+            if (started && !more) {
+                const uint32_t r = cur.rt * MR + row, token = r / p.group;
+                const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+                E *out = static_cast<E *>(p.O) +
+                         static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldo +
+                         (cur.h * p.group + (r - token * p.group)) * D + 4u * d4;
+                const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+                alignas(16) E e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) from_f32(v[k], e[k]);
+                if (p.vec & 2u) {
+                    if constexpr (sizeof(E) == 4) *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<uint4 *>(e);
+                    else *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<uint2 *>(e);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) out[k] = e[k];
+                }
+            } else {
+                reinterpret_cast<float4 *>(p.ws_o)[(static_cast<uint64_t>(part) * MR + row) * (DP / 4) + d4] = o;
+                if (d4 == 0) p.ws_ml[part * MR + row] = make_float2(mm, ll);
+            }
+        }
+        __syncthreads();  // the slots may be filled again
+    };
+
+    uint32_t slot = 0;
+    bool fresh = true;
+    uint32_t parts = 0;
+    for (; left; --left) {
+        cp_async_wait_group<S - 2>();
+        __syncwarp();
+        issue();  // into the slot that the last step consumed
+        fetch_pages();
+        if (fresh) begin_rows();
+        compute(slot);
+        const bool row_end = cur.tile + 1 == cur.lo + cur.nt;
+        fresh = row_end;
+        if (row_end || left == 1) {
+            if (!row_end && first_tile == cur.lo)   // the tile's first CTA joins its parts
+                parts = 1 + static_cast<uint32_t>((cur.lo + cur.nt - cur.tile - 1 + run - 1) / run);
+            end_rows(slot, !row_end);
+        } else {
+            __syncwarp();
+        }
+        if (left > 1) next_unit<MR>(p, cur);
+        slot = slot + 1 == S ? 0 : slot + 1;
+    }
+    cp_async_wait_group<0>();
+    if (tid == 0 && p.ws_meta) {
+        p.ws_meta[2 * cta] = make_uint4(parts, static_cast<uint32_t>(cur.s.row0), cur.rt * MR, cur.h);
+        p.ws_meta[2 * cta + 1] = make_uint4(
+            min(MR, static_cast<uint32_t>(cur.s.n) * p.group - cur.rt * MR), 0, 0, 0);
+    }
+}
+
+// Joins a row tile's parts: block (c, y) those of the tile that begins in CTA
+// c and goes on in the next ones, 32 groups of 4 values of it; 8 lanes share
+// the parts, added in a fixed order.
+template <RowType T, uint32_t DP>
+__global__ void __launch_bounds__(256) paged_attention_join_kernel(const AttnParams p) {
+    using E = typename RowOf<T>::type;
+    constexpr uint32_t MR = T == RowType::kF32 ? 8 : 16;
+    __shared__ float4 sh_o[8][32];
+    __shared__ float2 sh_ml[8][32];
+    pdl_enter();
+    const uint32_t cta = blockIdx.x;
+    const uint4 meta = p.ws_meta[2 * cta];
+    if (meta.x < 2) return;
+    const uint32_t rows = p.ws_meta[2 * cta + 1].x;
+    const uint32_t x = threadIdx.x & 31u, y = threadIdx.x >> 5;
+    const uint32_t i = blockIdx.y * 32u + x;
+    const uint32_t row = i / (DP / 4), d4 = i % (DP / 4);
+    const bool live = row < rows && 4u * d4 < p.c.head_dim;
+    float mm = -INFINITY, ll = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    if (live) {
+#pragma unroll 4
+        for (uint32_t k = y; k < meta.x; k += 8) {
+            const uint64_t part = k == 0 ? 2ull * cta + 1 : 2ull * (cta + k);
+            const float2 ml = p.ws_ml[part * MR + row];
+            const float4 v = reinterpret_cast<const float4 *>(p.ws_o)[(part * MR + row) * (DP / 4) + d4];
+            const float to = fmaxf(mm, ml.x);
+            const float f = mm == -INFINITY ? 1.0f : ex2(mm - to), g = ml.x == -INFINITY ? 1.0f : ex2(ml.x - to);
+            mm = to;
+            ll = ll * f + ml.y * g;
+            o.x = o.x * f + v.x * g;
+            o.y = o.y * f + v.y * g;
+            o.z = o.z * f + v.z * g;
+            o.w = o.w * f + v.w * g;
+        }
+    }
+    sh_o[y][x] = o;
+    sh_ml[y][x] = make_float2(mm, ll);
+    __syncthreads();
+    if (y != 0 || !live) return;
+    for (uint32_t k = 1; k < 8; ++k) mm = fmaxf(mm, sh_ml[k][x].x);
+    ll = 0.0f;
+    o = make_float4(0, 0, 0, 0);
+    for (uint32_t k = 0; k < 8; ++k) {
+        const float2 ml = sh_ml[k][x];
+        const float f = ml.x == -INFINITY ? 1.0f : ex2(ml.x - mm);
+        const float4 v = sh_o[k][x];
+        ll += ml.y * f;
+        o.x += v.x * f;
+        o.y += v.y * f;
+        o.z += v.z * f;
+        o.w += v.w * f;
+    }
+    const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+    const uint32_t r = meta.z + row, token = r / p.group;
+    E *out = static_cast<E *>(p.O) + static_cast<uint64_t>(meta.y + token) * p.ldo +
+             (meta.w * p.group + (r - token * p.group)) * p.c.head_dim + 4u * d4;
+    from_f32(o.x * inv, out[0]);
+    from_f32(o.y * inv, out[1]);
+    from_f32(o.z * inv, out[2]);
+    from_f32(o.w * inv, out[3]);
+}
+
+template <RowType T, uint32_t DP>
+cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
+    using Shape = AttnShape<DP>;
+    constexpr uint32_t MR = T == RowType::kF32 ? 8 : 16;
+    const uint32_t elem = T == RowType::kF32 ? 4 : 2;
+    AttnParams p{};
+    p.c = a.cache;
+    p.pb = a.batch;
+    p.Q = a.Q;
+    p.O = a.O;
+    p.ldq = a.ldq;
+    p.ldo = a.ldo;
+    p.group = a.q_heads / a.cache.heads;
+    p.causal = a.causal;
+    p.window = a.window;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.vec = (reinterpret_cast<uintptr_t>(a.Q) % 16u == 0 && 1ull * a.ldq * elem % 16u == 0 ? 1u : 0u) |
+            (reinterpret_cast<uintptr_t>(a.O) % (4u * elem) == 0 && a.ldo % 4u == 0 ? 2u : 0u);
+    p.err = ctx.err;
+    static thread_local int ready_device = -1;
+    int device = 0;
+    VNPU_LAUNCH(cudaGetDevice(&device));
+    if (ready_device != device) {
+        VNPU_LAUNCH(cudaFuncSetAttribute(paged_attention_kernel<T, DP>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem));
+        ready_device = device;
+    }
+    const uint32_t grid = static_cast<uint32_t>(ctx.num_sms) * Shape::kCtasPerSm;
+    // One key tile holds all that the table reaches: nothing is split, nothing to join.
+    const bool split = (static_cast<uint64_t>(a.batch.table_stride) << a.cache.page_shift) > kTile;
+    void *ws = nullptr;
+    const size_t o_bytes = 2ull * grid * MR * DP * sizeof(float);
+    const size_t ml_bytes = 2ull * grid * MR * sizeof(float2);
+    if (split) {
+        VNPU_LAUNCH(cudaMallocAsync(&ws, o_bytes + ml_bytes + 2ull * grid * sizeof(uint4), ctx.stream));
+        p.ws_o = static_cast<float *>(ws);
+        p.ws_ml = reinterpret_cast<float2 *>(static_cast<char *>(ws) + o_bytes);
+        p.ws_meta = reinterpret_cast<uint4 *>(static_cast<char *>(ws) + o_bytes + ml_bytes);
+    }
+    if (ctx.launch_counter) *ctx.launch_counter += split ? 2 : 1;
+    cudaError_t e = launch_pdl(ctx.stream, &paged_attention_kernel<T, DP>, dim3(grid), dim3(kThreadsA),
+                               Shape::kSmem, p, 1u);
+    if (split) {
+        const uint64_t rows = std::min<uint64_t>(MR, 1ull * a.batch.max_tokens * p.group);
+        const uint32_t y = static_cast<uint32_t>((rows * (DP / 4) + 31) / 32);
+        if (e == cudaSuccess)
+            e = launch_pdl(ctx.stream, &paged_attention_join_kernel<T, DP>, dim3(grid, y), dim3(256), 0, p);
+        const cudaError_t f = cudaFreeAsync(ws, ctx.stream);
+        if (e == cudaSuccess) e = f;
+    }
+    return e;
+}
+
+template <RowType T>
+cudaError_t launch_by_dim(const LaunchCtx &ctx, const PagedAttention &a) {
+    if (a.cache.head_dim <= 64) return launch_attention<T, 64>(ctx, a);
+    if (a.cache.head_dim <= 128) return launch_attention<T, 128>(ctx, a);
+    return launch_attention<T, 256>(ctx, a);
+}
+
+}  // namespace
+
+cudaError_t paged_attention(const LaunchCtx &ctx, const PagedAttention &a) {
+    switch (a.type) {
+    case RowType::kF32: return launch_by_dim<RowType::kF32>(ctx, a);
+    case RowType::kF16: return launch_by_dim<RowType::kF16>(ctx, a);
+    default: return launch_by_dim<RowType::kBF16>(ctx, a);
+    }
+}
+
+}  // namespace vnpu_b200

@@ -1,0 +1,416 @@
+// paged_kv.cu - the paged 8-bit key/value cache: append with rotation
+// (VNPU_B200_OP_PAGED_KV_APPEND) and read-back (VNPU_B200_OP_PAGED_KV_READ).
+//
+// Both are bound by memory: each row element is read once and each code
+// written once.  Work is split by segments: the part of one sequence's rows
+// that falls into one page.  A CTA owns one (segment, head, K or V), so it
+// alone sees all values that enter the page's scale: no atomics, and one
+// result whatever the order.  Segments of ragged sequences need no prefix sum:
+// a run of n rows touches at most floor(n / page_size) + 2 pages, so sequence
+// b's segments can start at floor(cu[b] / page_size) + 2 b, which any CTA can
+// search for; the numbers left over are CTAs that leave at once.
+#include "paged_common.cuh"
+
+namespace vnpu_b200 {
+namespace {
+
+struct PagedTurns {
+    uint64_t t[128];
+};
+
+// A page's part of a sequence's rows.
+struct Segment {
+    int32_t row0, n;    // rows
+    int32_t slot0;      // slot of row0
+    int32_t pos0;       // position of row0
+    int64_t page;
+};
+
+// Segment number `item` of the batch; false: no such segment, or a bad one.
+template <uint32_t NT>
+__device__ __forceinline__ bool find_segment(const PagedCache &c, const PagedBatch &pb,
+                                             uint32_t item, uint32_t *err, Segment &g) {
+    uint32_t b, seg = 0;
+    if (pb.max_tokens == 1) {
+        b = item;  // one segment a sequence: item b is sequence b's
+    } else {
+        const auto after = [&](uint32_t i) -> uint64_t {
+            const int32_t cu = __ldg(pb.cu + i + 1);
+            return (static_cast<uint64_t>(cu < 0 ? 0 : cu) >> c.page_shift) + 2ull * (i + 1);
+        };
+        b = find_seq<NT>(pb.batch, after, item);
+        if (b >= pb.batch) return false;
+        const int32_t c0 = __ldg(pb.cu + b);
+        const uint64_t base = (static_cast<uint64_t>(c0 < 0 ? 0 : c0) >> c.page_shift) + 2ull * b;
+        if (item < base) return false;  // only where cu falls
+        seg = static_cast<uint32_t>(item - base);
+    }
+    PagedSeq s;
+    if (!load_seq(pb, c.page_shift, b, s)) {
+        if (threadIdx.x == 0) record_error(err, kErrBadIndex);
+        return false;
+    }
+    if (s.n == 0) return false;
+    const uint64_t index = (static_cast<uint32_t>(s.start) >> c.page_shift) + static_cast<uint64_t>(seg);
+    const int64_t p0 = static_cast<int64_t>(index << c.page_shift);
+    if (p0 >= s.len) return false;
+    const int64_t lo = max(static_cast<int64_t>(s.start), p0);
+    const int64_t hi = min(static_cast<int64_t>(s.len), p0 + (static_cast<int64_t>(1) << c.page_shift));
+    g.page = __ldg(pb.table + static_cast<uint64_t>(b) * pb.table_stride + index);
+    if (g.page < 0 || g.page >= c.num_pages) {
+        if (threadIdx.x == 0) record_error(err, kErrBadIndex);
+        return false;
+    }
+    g.row0 = s.row0 + static_cast<int32_t>(lo - s.start);
+    g.n = static_cast<int32_t>(hi - lo);
+    g.slot0 = static_cast<int32_t>(lo - p0);
+    g.pos0 = static_cast<int32_t>(lo);
+    return true;
+}
+
+inline uint64_t segment_items(const PagedCache &c, const PagedBatch &b) {
+    return b.max_tokens == 1 ? b.batch : (static_cast<uint64_t>(b.tokens) >> c.page_shift) + 2ull * b.batch;
+}
+
+// cos and sin of `pos` times t 2^-64 turns.  The product is taken modulo one
+// turn (the 64-bit wrap), then rounded to 32 bits: off by 2^-24 of the angle
+// in (-pi, pi] at every position, where a 32-bit position * frequency is off
+// by 2^-24 of the whole angle, 1e-2 at position 1e5.
+__device__ __forceinline__ void turn_sincos(int32_t pos, uint64_t t, float *sn, float *cs) {
+    const int64_t a = static_cast<int64_t>(static_cast<uint64_t>(static_cast<int64_t>(pos)) * t);
+    sincospif(static_cast<float>(a) * 0x1p-63f, sn, cs);
+}
+
+// A head's 16 elements of unit u as two groups of 8 and their pairs' first
+// index: for the half-split rotation the groups are 8u.. and rotary/2 + 8u..,
+// else 16u.. and 16u + 8...  pair < 0: not rotated.
+struct Unit {
+    uint32_t o0, o1;
+    int32_t pair;
+};
+__device__ __forceinline__ Unit unit_of(uint32_t u, uint32_t rotary, bool interleaved) {
+    Unit x;
+    const bool turned = u * 16u < rotary;
+    x.o0 = turned && !interleaved ? 8u * u : 16u * u;
+    x.o1 = turned && !interleaved ? rotary / 2u + 8u * u : 16u * u + 8u;
+    x.pair = turned ? static_cast<int32_t>(8u * u) : -1;
+    return x;
+}
+
+// Rotates a unit; cs(i, sn, cs) gives the sine and cosine of pair x.pair + i.
+template <typename F>
+__device__ __forceinline__ void rotate_unit(float (&a)[8], float (&b)[8], bool interleaved,
+                                            const F &angle) {
+    if (!interleaved) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float sn, cs;
+            angle(i, &sn, &cs);
+            const float x = a[i], y = b[i];
+            a[i] = x * cs - y * sn;
+            b[i] = x * sn + y * cs;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float sn, cs;
+            angle(i, &sn, &cs);
+            float x = a[2 * i], y = a[2 * i + 1];
+            a[2 * i] = x * cs - y * sn;
+            a[2 * i + 1] = x * sn + y * cs;
+            angle(i + 4, &sn, &cs);
+            x = b[2 * i];
+            y = b[2 * i + 1];
+            b[2 * i] = x * cs - y * sn;
+            b[2 * i + 1] = x * sn + y * cs;
+        }
+    }
+}
+
+// Code of x: nearest, ties to even; NaN 0 (the conversion's own), infinities
+// the largest code.
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+    const int q = __float2int_rn(__fmul_rn(x, inv));
+    return static_cast<uint32_t>(max(-127, min(127, q))) & 0xffu;
+}
+__device__ __forceinline__ uint32_t codes4(const float *v, float inv) {
+    return code_of(v[0], inv) | (code_of(v[1], inv) << 8) | (code_of(v[2], inv) << 16) |
+           (code_of(v[3], inv) << 24);
+}
+__device__ __forceinline__ uint32_t rescaled4(uint32_t w, float ratio) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r |= code_of(static_cast<float>(static_cast<int8_t>(w >> (8 * i))), ratio) << (8 * i);
+    return r;
+}
+
+constexpr uint32_t kQueryRows(uint32_t nt) { return nt / 64; }  // query rows of a CTA
+
+// Grid: segments x heads x {K, V}, then the query rows.  A thread holds up to
+// U units (16 elements each) of its segment in registers between the maximum
+// and the rounding; a segment with more is read again, from L2.
+template <RowType T, uint32_t NT, uint32_t U>
+__global__ void __launch_bounds__(NT) paged_append_kernel(
+    const PagedCache c, const PagedBatch pb, const void *Qv, const void *Kv, const void *Vv,
+    void *Qov, uint32_t ldq, uint32_t ldk, uint32_t ldv, uint32_t ldqo, uint32_t q_heads,
+    uint32_t rotary, bool interleaved, uint32_t vec, uint32_t kv_ctas, const PagedTurns turns,
+    uint32_t *err) {
+    using E = typename RowOf<T>::type;
+    pdl_enter();
+    __shared__ float2 sh_turn[kQueryRows(NT)][128];
+    __shared__ float sh_max[NT / 32];
+    const uint32_t tid = threadIdx.x, D = c.head_dim;
+
+    if (blockIdx.x >= kv_ctas) {
+        // ---- queries: rotate rows r0 .. r0 + kQueryRows - 1, angles shared by the heads
+        const uint32_t r0 = (blockIdx.x - kv_ctas) * kQueryRows(NT);
+        int32_t pos[kQueryRows(NT)];
+#pragma unroll
+        for (uint32_t i = 0; i < kQueryRows(NT); ++i) {
+            const uint32_t r = r0 + i;
+            pos[i] = -1;
+            if (r >= pb.tokens) continue;
+            // the row's sequence: row b itself when every sequence has one
+            uint32_t b = r;
+            const bool own = r < pb.batch && __ldg(pb.cu + r) == static_cast<int32_t>(r) &&
+                             __ldg(pb.cu + r + 1) == static_cast<int32_t>(r) + 1;
+            if (!own)  // block-uniform
+                b = find_seq<NT>(pb.batch, [&](uint32_t j) -> uint64_t {
+                    const int32_t cu = __ldg(pb.cu + j + 1);
+                    return cu < 0 ? 0u : static_cast<uint64_t>(cu);
+                }, r);
+            if (b >= pb.batch) continue;  // a row of no sequence
+            PagedSeq s;
+            if (!load_seq(pb, c.page_shift, b, s) || static_cast<int32_t>(r) < s.row0 ||
+                static_cast<int32_t>(r) >= s.row0 + s.n) {
+                if (tid == 0) record_error(err, kErrBadIndex);
+                continue;
+            }
+            pos[i] = s.start + static_cast<int32_t>(r) - s.row0;
+        }
+        const uint32_t pairs = rotary / 2u;
+#pragma unroll
+        for (uint32_t i = 0; i < kQueryRows(NT); ++i)
+            for (uint32_t j = tid; j < pairs; j += NT)
+                turn_sincos(pos[i], turns.t[j], &sh_turn[i][j].y, &sh_turn[i][j].x);
+        __syncthreads();
+        const uint32_t per_row = q_heads * (D / 16u);
+        const bool vin = vec & 1u, vout = vec & 8u;
+#pragma unroll
+        for (uint32_t i = 0; i < kQueryRows(NT); ++i) {
+            if (pos[i] < 0) continue;
+            const E *in = static_cast<const E *>(Qv) + static_cast<uint64_t>(r0 + i) * ldq;
+            E *out = static_cast<E *>(Qov) + static_cast<uint64_t>(r0 + i) * ldqo;
+#pragma unroll 2
+            for (uint32_t k = tid; k < per_row; k += NT) {
+                const uint32_t h = k / (D / 16u);
+                const Unit x = unit_of(k - h * (D / 16u), rotary, interleaved);
+                float a[8], b[8];
+                load8(in + h * D + x.o0, vin, a);
+                load8(in + h * D + x.o1, vin, b);
+                if (x.pair >= 0)
+                    rotate_unit(a, b, interleaved, [&](int e, float *sn, float *cs) {
+                        const float2 t = sh_turn[i][x.pair + e];
+                        *cs = t.x;
+                        *sn = t.y;
+                    });
+                store8(out + h * D + x.o0, vout, a);
+                store8(out + h * D + x.o1, vout, b);
+            }
+        }
+        return;
+    }
+
+    const uint32_t item = blockIdx.x / (2u * c.heads);
+    const uint32_t which = blockIdx.x - item * 2u * c.heads;
+    const bool value = which >= c.heads;
+    const uint32_t h = value ? which - c.heads : which;
+    Segment g;
+    if (!find_segment<NT>(c, pb, item, err, g)) return;
+    const uint32_t ld = value ? ldv : ldk;
+    const bool vin = vec & (value ? 4u : 2u);
+    const E *in = static_cast<const E *>(value ? Vv : Kv) + static_cast<uint64_t>(g.row0) * ld + h * D;
+    const uint64_t at = static_cast<uint64_t>(g.page) * c.heads + h;
+    int8_t *page = (value ? c.V : c.K) + ((at << c.page_shift) * D);
+    float *scale = (value ? c.V_scale : c.K_scale) + at;
+    const float held = g.slot0 ? *scale : 0.0f;
+    const uint32_t rot = value ? 0u : rotary;
+    const uint32_t per_row = D / 16u, units = g.n * per_row;
+
+    const auto fetch = [&](uint32_t k, float (&a)[8], float (&b)[8]) {
+        const uint32_t r = k / per_row;
+        const Unit x = unit_of(k - r * per_row, rot, interleaved);
+        const E *row = in + static_cast<uint64_t>(r) * ld;
+        load8(row + x.o0, vin, a);
+        load8(row + x.o1, vin, b);
+    };
+    const auto turn = [&](uint32_t k, float (&a)[8], float (&b)[8]) {
+        const uint32_t r = k / per_row;
+        const Unit x = unit_of(k - r * per_row, rot, interleaved);
+        if (x.pair >= 0)
+            rotate_unit(a, b, interleaved, [&](int e, float *sn, float *cs) {
+                turn_sincos(g.pos0 + static_cast<int32_t>(r), turns.t[x.pair + e], sn, cs);
+            });
+    };
+    float most = 0.0f;
+    const auto widen = [&](const float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = fabsf(a[i]), y = fabsf(b[i]);
+            if (x <= 3.402823466e38f) most = fmaxf(most, x);  // NaN and infinity do not count
+            if (y <= 3.402823466e38f) most = fmaxf(most, y);
+        }
+    };
+    float a[U][8], b[U][8];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)  // all loads in flight before the first is used
+        if (tid + u * NT < units) fetch(tid + u * NT, a[u], b[u]);
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+        if (tid + u * NT < units) {
+            turn(tid + u * NT, a[u], b[u]);
+            widen(a[u], b[u]);
+        }
+    for (uint32_t k = tid + U * NT; k < units; k += NT) {
+        float x[8], y[8];
+        fetch(k, x, y);
+        turn(k, x, y);
+        widen(x, y);
+    }
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));  // >= 0
+    if ((tid & 31u) == 0) sh_max[tid >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < NT / 32u; ++i) most = fmaxf(most, sh_max[i]);
+
+    // A scale below the smallest normal number has no finite reciprocal: such a page is zero.
+    const float fresh = __fdiv_rn(most, 127.0f);
+    const float now = fmaxf(held, fresh < 1.17549435e-38f ? 0.0f : fresh);
+    const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
+    if (tid == 0) *scale = now;
+    const auto put = [&](uint32_t k, const float (&a)[8], const float (&b)[8]) {
+        const uint32_t r = k / per_row;
+        const Unit x = unit_of(k - r * per_row, rot, interleaved);
+        int8_t *row = page + static_cast<uint32_t>(g.slot0 + r) * D;
+        *reinterpret_cast<uint2 *>(row + x.o0) = make_uint2(codes4(a, inv), codes4(a + 4, inv));
+        *reinterpret_cast<uint2 *>(row + x.o1) = make_uint2(codes4(b, inv), codes4(b + 4, inv));
+    };
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+        if (tid + u * NT < units) put(tid + u * NT, a[u], b[u]);
+    for (uint32_t k = tid + U * NT; k < units; k += NT) {
+        float x[8], y[8];
+        fetch(k, x, y);
+        turn(k, x, y);
+        put(k, x, y);
+    }
+    if (g.slot0 && now > held) {  // the scale grew: round the page's older codes to it
+        const float ratio = __fdiv_rn(held, now);
+        uint4 *old = reinterpret_cast<uint4 *>(page);
+        for (uint32_t k = tid; k < static_cast<uint32_t>(g.slot0) * per_row; k += NT) {
+            uint4 w = old[k];
+            w.x = rescaled4(w.x, ratio);
+            w.y = rescaled4(w.y, ratio);
+            w.z = rescaled4(w.z, ratio);
+            w.w = rescaled4(w.w, ratio);
+            old[k] = w;
+        }
+    }
+}
+
+// A CTA reads one segment of one head, K and V.
+template <RowType T, uint32_t NT>
+__global__ void __launch_bounds__(NT) paged_read_kernel(
+    const PagedCache c, const PagedBatch pb, void *Kv, void *Vv, uint64_t ld_row, uint64_t ld_head,
+    bool vec, uint32_t *err) {
+    using E = typename RowOf<T>::type;
+    pdl_enter();
+    const uint32_t item = blockIdx.x / c.heads, h = blockIdx.x - item * c.heads;
+    Segment g;
+    if (!find_segment<NT>(c, pb, item, err, g)) return;
+    const uint32_t D = c.head_dim, per_row = D / 16u, units = g.n * per_row;
+    const uint64_t at = static_cast<uint64_t>(g.page) * c.heads + h;
+    const uint64_t first = (at << c.page_shift) * D + static_cast<uint32_t>(g.slot0) * D;
+    const uint64_t out0 = static_cast<uint64_t>(g.row0) * ld_row + h * ld_head;
+    const float ks = Kv ? __ldg(c.K_scale + at) : 0.0f, vs = Vv ? __ldg(c.V_scale + at) : 0.0f;
+    const auto put = [&](const uint4 &w, float s, E *out) {
+        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = static_cast<float>(static_cast<int8_t>(word[2 * half + (i >> 2)] >> (8 * (i & 3)))) * s;
+            store8(out + 8 * half, vec, v);
+        }
+    };
+#pragma unroll 2
+    for (uint32_t k = threadIdx.x; k < units; k += NT) {
+        const uint32_t r = k / per_row, d = (k - r * per_row) * 16u;
+        const uint64_t o = out0 + r * ld_row + d;
+        uint4 kw, vw;
+        if (Kv) kw = __ldg(reinterpret_cast<const uint4 *>(c.K + first) + k);
+        if (Vv) vw = __ldg(reinterpret_cast<const uint4 *>(c.V + first) + k);
+        if (Kv) put(kw, ks, static_cast<E *>(Kv) + o);
+        if (Vv) put(vw, vs, static_cast<E *>(Vv) + o);
+    }
+}
+
+template <typename F>
+cudaError_t by_type(RowType t, const F &f) {
+    switch (t) {
+    case RowType::kF32: return f(std::integral_constant<RowType, RowType::kF32>{});
+    case RowType::kF16: return f(std::integral_constant<RowType, RowType::kF16>{});
+    default: return f(std::integral_constant<RowType, RowType::kBF16>{});
+    }
+}
+
+bool aligned16(const void *p, uint64_t stride_bytes) {
+    return reinterpret_cast<uintptr_t>(p) % 16u == 0 && stride_bytes % 16u == 0;
+}
+
+}  // namespace
+
+cudaError_t paged_kv_append(const LaunchCtx &ctx, const PagedAppend &p) {
+    const uint32_t elem = p.type == RowType::kF32 ? 4 : 2;
+    const uint32_t vec = (aligned16(p.Q, 1ull * p.ldq * elem) ? 1u : 0u) |
+                         (aligned16(p.K, 1ull * p.ldk * elem) ? 2u : 0u) |
+                         (aligned16(p.V, 1ull * p.ldv * elem) ? 4u : 0u) |
+                         (aligned16(p.Q_out, 1ull * p.ldqo * elem) ? 8u : 0u);
+    PagedTurns turns{};
+    for (uint32_t j = 0; j < p.rotary / 2; ++j) turns.t[j] = p.turns[j];
+    const uint64_t kv = segment_items(p.cache, p.batch) * 2 * p.cache.heads;
+    const bool single = p.batch.max_tokens == 1;
+    const uint32_t nt = single ? 128 : 256, rows = kQueryRows(nt);
+    const uint64_t grid = kv + (p.Q ? (p.batch.tokens + rows - 1) / rows : 0);
+    if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+    // Units a thread holds: a page's worth, at most 4 (64 registers).
+    const uint64_t units = (static_cast<uint64_t>(p.cache.head_dim) << p.cache.page_shift) / 16 / 256;
+    if (ctx.launch_counter) ++*ctx.launch_counter;
+    return by_type(p.type, [&](auto t) -> cudaError_t {
+        constexpr RowType T = decltype(t)::value;
+        auto kernel = single ? &paged_append_kernel<T, 128, 1>
+                      : units <= 2 ? &paged_append_kernel<T, 256, 2>
+                                   : &paged_append_kernel<T, 256, 4>;
+        return launch_pdl(ctx.stream, kernel, dim3(static_cast<uint32_t>(grid)), dim3(nt), 0, p.cache,
+                          p.batch, p.Q, p.K, p.V, p.Q_out, p.ldq, p.ldk, p.ldv, p.ldqo, p.q_heads,
+                          p.rotary, p.interleaved, vec, static_cast<uint32_t>(kv), turns, ctx.err);
+    });
+}
+
+cudaError_t paged_kv_read(const LaunchCtx &ctx, const PagedRead &p) {
+    const uint32_t elem = p.type == RowType::kF32 ? 4 : 2;
+    const bool vec = aligned16(p.K_out, p.ld_row * elem) && aligned16(p.V_out, p.ld_head * elem);
+    const uint64_t grid = segment_items(p.cache, p.batch) * p.cache.heads;
+    if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+    if (ctx.launch_counter) ++*ctx.launch_counter;
+    return by_type(p.type, [&](auto t) -> cudaError_t {
+        constexpr RowType T = decltype(t)::value;
+        return launch_pdl(ctx.stream, &paged_read_kernel<T, 128>, dim3(static_cast<uint32_t>(grid)),
+                          dim3(128), 0, p.cache, p.batch, p.K_out, p.V_out, p.ld_row, p.ld_head,
+                          vec, ctx.err);
+    });
+}
+
+}  // namespace vnpu_b200

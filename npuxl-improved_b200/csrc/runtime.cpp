@@ -996,6 +996,219 @@ void exec_qkv_rope_append(vnpu_stream_t *s, const vnpu_command_t &cmd, uint32_t 
     acc.dma = st.staged_bytes();
 }
 
+static_assert(sizeof(vnpu_b200_paged_kv_append_args_t) <= sizeof(vnpu_command_t::args) &&
+                  sizeof(vnpu_b200_paged_kv_read_args_t) <= sizeof(vnpu_command_t::args) &&
+                  sizeof(vnpu_b200_paged_attention_args_t) <= sizeof(vnpu_command_t::args),
+              "paged cache args fit the command");
+
+// Host-side checks of a paged command's cache; the pool itself has to be in
+// device memory (staging a pool through the host for each command is no use).
+PagedCache paged_cache_of(const vnpu_stream_t *s, const vnpu_b200_paged_cache_t &c) {
+    if (!c.K || !c.V || !c.K_scale || !c.V_scale || !c.num_pages || !c.heads)
+        throw CommandError("invalid paged cache", VNPU_ERR_INVALID_ARGUMENT);
+    if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1)) ||
+        c.head_dim < 16 || c.head_dim > 256 || c.head_dim % 16u)
+        throw CommandError("paged cache page_size or head_dim", VNPU_ERR_UNSUPPORTED);
+    if (c.num_pages > 0x7fffffffu || c.heads > 65535u ||
+        reinterpret_cast<uintptr_t>(c.K) % 16u || reinterpret_cast<uintptr_t>(c.V) % 16u ||
+        reinterpret_cast<uintptr_t>(c.K_scale) % 4u || reinterpret_cast<uintptr_t>(c.V_scale) % 4u)
+        throw CommandError("paged cache size or alignment", VNPU_ERR_INVALID_ARGUMENT);
+    for (const void *p : {static_cast<const void *>(c.K), static_cast<const void *>(c.V),
+                          static_cast<const void *>(c.K_scale), static_cast<const void *>(c.V_scale)})
+        if (classify(p, s->device->ordinal) != Mem::kDevice)
+            throw CommandError("a paged cache lives in this device's memory",
+                               VNPU_ERR_INVALID_ARGUMENT);
+    PagedCache out;
+    out.K = c.K;
+    out.V = c.V;
+    out.K_scale = c.K_scale;
+    out.V_scale = c.V_scale;
+    out.num_pages = c.num_pages;
+    out.heads = c.heads;
+    while ((1u << out.page_shift) < c.page_size) ++out.page_shift;
+    out.head_dim = c.head_dim;
+    return out;
+}
+
+PagedBatch paged_batch_of(const vnpu_b200_paged_batch_t &b, Staging &st) {
+    if (!b.block_table || !b.cu_tokens || !b.seq_lens || !b.table_stride ||
+        b.table_stride > 0x7fffffffu || b.batch > (1u << 24) || b.tokens > 0x7fffffffu)
+        throw CommandError("invalid paged batch", VNPU_ERR_INVALID_ARGUMENT);
+    PagedBatch out;
+    out.table = st.in(b.block_table, sizeof(int32_t) * static_cast<uint64_t>(b.batch) * b.table_stride);
+    out.cu = st.in(b.cu_tokens, sizeof(int32_t) * (static_cast<uint64_t>(b.batch) + 1));
+    out.lens = st.in(b.seq_lens, sizeof(int32_t) * static_cast<uint64_t>(b.batch));
+    out.batch = b.batch;
+    out.table_stride = b.table_stride;
+    out.tokens = b.tokens;
+    out.max_tokens = b.max_tokens && b.max_tokens < b.tokens ? b.max_tokens : b.tokens;
+    return out;
+}
+
+uint32_t paged_row_bytes(uint32_t dtype) {
+    if (dtype == VNPU_DTYPE_F32) return 4;
+    if (dtype == VNPU_DTYPE_F16 || dtype == VNPU_DTYPE_BF16) return 2;
+    throw CommandError("paged rows are f32, f16 or bf16", VNPU_ERR_UNSUPPORTED);
+}
+
+RowType paged_row_type(uint32_t dtype) {
+    return dtype == VNPU_DTYPE_F32 ? RowType::kF32
+           : dtype == VNPU_DTYPE_F16 ? RowType::kF16 : RowType::kBF16;
+}
+
+// Bytes from the first to the last element of `rows` rows of `width` elements
+// `ld` apart; ld 0 becomes dense.
+uint64_t row_span(uint32_t rows, uint64_t width, uint32_t &ld, uint32_t elem) {
+    if (width > 0x7fffffffu) throw CommandError("paged row too wide", VNPU_ERR_INVALID_ARGUMENT);
+    if (!ld) ld = static_cast<uint32_t>(width);
+    if (ld < width) throw CommandError("paged row stride below its width", VNPU_ERR_INVALID_ARGUMENT);
+    return (static_cast<uint64_t>(rows - 1) * ld + width) * elem;
+}
+
+void check_rows(const void *p, uint32_t elem, const char *what) {
+    if (reinterpret_cast<uintptr_t>(p) % elem) throw CommandError(what, VNPU_ERR_INVALID_ARGUMENT);
+}
+
+void exec_paged_kv_append(vnpu_stream_t *s, const vnpu_command_t &cmd, const LaunchCtx &ctx,
+                          Accounting &acc) {
+    vnpu_b200_paged_kv_append_args_t a;
+    std::memcpy(&a, cmd.args.raw, sizeof(a));
+    PagedAppend p;
+    p.cache = paged_cache_of(s, a.cache);
+    const uint32_t elem = paged_row_bytes(a.dtype), d = a.cache.head_dim;
+    if (!a.K || !a.V || !a.Q != !a.Q_out || (a.Q && !a.q_heads) || a.q_heads > 65535u ||
+        (a.flags & ~(VNPU_B200_PAGED_INTERLEAVED | VNPU_B200_PAGED_NO_ROPE)))
+        throw CommandError("invalid paged_kv_append arguments", VNPU_ERR_INVALID_ARGUMENT);
+    if (a.rotary_dim > d || a.rotary_dim % 16u)
+        throw CommandError("paged_kv_append rotary_dim", VNPU_ERR_UNSUPPORTED);
+    check_rows(a.Q, elem, "Q alignment");
+    check_rows(a.K, elem, "K alignment");
+    check_rows(a.V, elem, "V alignment");
+    check_rows(a.Q_out, elem, "Q_out alignment");
+    Staging st(s);
+    p.batch = paged_batch_of(a.batch, st);
+    const uint32_t T = p.batch.tokens;
+    if (!T || !p.batch.batch) return;
+    const uint64_t qw = static_cast<uint64_t>(a.q_heads) * d;
+    const uint64_t kw = static_cast<uint64_t>(a.cache.heads) * d;
+    p.ldk = a.ldk;
+    p.ldv = a.ldv;
+    const char *const K = static_cast<const char *>(a.K), *const V = static_cast<const char *>(a.V);
+    p.K = st.in(K, row_span(T, kw, p.ldk, elem));
+    p.V = st.in(V, row_span(T, kw, p.ldv, elem));
+    if (a.Q) {
+        p.q_heads = a.q_heads;
+        p.ldq = a.ldq;
+        p.ldqo = a.ldqo;
+        const uint64_t in_span = row_span(T, qw, p.ldq, elem);
+        const uint64_t out_span = row_span(T, qw, p.ldqo, elem);
+        if (a.Q == a.Q_out && p.ldq != p.ldqo)
+            throw CommandError("in-place rotation needs one row stride", VNPU_ERR_INVALID_ARGUMENT);
+        // rows of no sequence are not written: they have to survive staging
+        p.Q_out = st.out(static_cast<char *>(a.Q_out), out_span, true);
+        p.Q = st.in(static_cast<const char *>(a.Q), in_span);
+    }
+    p.type = paged_row_type(a.dtype);
+    p.interleaved = (a.flags & VNPU_B200_PAGED_INTERLEAVED) != 0;
+    p.rotary = (a.flags & VNPU_B200_PAGED_NO_ROPE) ? 0 : (a.rotary_dim ? a.rotary_dim : d);
+    // 2^-64 turns per position of pair j: scaling * theta^(-2j/rotary) / (2 pi), modulo one turn.
+    // Powers by repeated multiplication in 64-bit mantissas: 128 of them are off by 2^-56 at most.
+    uint64_t turns[128];
+    if (p.rotary) {
+        const long double theta = a.theta_base > 0.0f ? a.theta_base : 10000.0f;
+        const long double ratio = std::pow(theta, -2.0L / p.rotary);
+        long double t = (a.scaling > 0.0f ? a.scaling : 1.0f) / 6.283185307179586476925286766559L;
+        for (uint32_t j = 0; j < p.rotary / 2; ++j, t *= ratio)
+            turns[j] = static_cast<uint64_t>((t - std::floor(t)) * 18446744073709551616.0L);
+    }
+    p.turns = turns;
+    cuda_check(paged_kv_append(ctx, p), "paged_kv_append launch");
+    st.finish();
+    acc.bytes_read = T * (qw * (a.Q ? 1 : 0) + 2 * kw) * elem;
+    acc.bytes_written = T * (qw * (a.Q ? 1 : 0) * elem + 2 * kw);
+    acc.flops = T * (qw * (a.Q ? 3 : 0) + 7 * kw);
+    acc.dma = st.staged_bytes();
+}
+
+void exec_paged_kv_read(vnpu_stream_t *s, const vnpu_command_t &cmd, const LaunchCtx &ctx,
+                        Accounting &acc) {
+    vnpu_b200_paged_kv_read_args_t a;
+    std::memcpy(&a, cmd.args.raw, sizeof(a));
+    PagedRead p;
+    p.cache = paged_cache_of(s, a.cache);
+    const uint32_t elem = paged_row_bytes(a.dtype), d = a.cache.head_dim, h = a.cache.heads;
+    if (!a.K_out && !a.V_out)
+        throw CommandError("paged_kv_read without an output", VNPU_ERR_INVALID_ARGUMENT);
+    check_rows(a.K_out, elem, "K_out alignment");
+    check_rows(a.V_out, elem, "V_out alignment");
+    Staging st(s);
+    p.batch = paged_batch_of(a.batch, st);
+    const uint64_t T = p.batch.tokens;
+    if (!T || !p.batch.batch) return;
+    p.ld_row = a.ld_row ? a.ld_row : static_cast<uint64_t>(h) * d;
+    p.ld_head = a.ld_head ? a.ld_head : d;
+    // rows and heads must not overlap: one of the two strides steps over the other's extent
+    const uint64_t row_extent = (h - 1) * p.ld_head + d, head_extent = (T - 1) * p.ld_row + d;
+    if (p.ld_row > UINT64_MAX / 8 / T || p.ld_head > UINT64_MAX / 8 / h || p.ld_head < d ||
+        p.ld_row < d || (T > 1 && h > 1 && p.ld_row < row_extent && p.ld_head < head_extent))
+        throw CommandError("paged_kv_read strides", VNPU_ERR_INVALID_ARGUMENT);
+    const uint64_t span = ((T - 1) * p.ld_row + (h - 1) * p.ld_head + d) * elem;
+    p.K_out = st.out(static_cast<char *>(a.K_out), span, true);  // gaps survive staging
+    p.V_out = st.out(static_cast<char *>(a.V_out), span, true);
+    p.type = paged_row_type(a.dtype);
+    cuda_check(paged_kv_read(ctx, p), "paged_kv_read launch");
+    st.finish();
+    const uint64_t n = T * h * d * ((a.K_out ? 1 : 0) + (a.V_out ? 1 : 0));
+    acc.bytes_read = n;
+    acc.bytes_written = n * elem;
+    acc.flops = n;
+    acc.dma = st.staged_bytes();
+}
+
+void exec_paged_attention(vnpu_stream_t *s, const vnpu_command_t &cmd, const LaunchCtx &ctx,
+                          Accounting &acc) {
+    vnpu_b200_paged_attention_args_t a;
+    std::memcpy(&a, cmd.args.raw, sizeof(a));
+    PagedAttention p;
+    p.cache = paged_cache_of(s, a.cache);
+    const uint32_t elem = paged_row_bytes(a.dtype), d = a.cache.head_dim;
+    if (!a.Q || !a.O || !a.q_heads || a.q_heads > 65535u || a.q_heads % a.cache.heads ||
+        a.causal > 1 || !std::isfinite(a.scale))
+        throw CommandError("invalid paged_attention arguments", VNPU_ERR_INVALID_ARGUMENT);
+    check_rows(a.Q, elem, "Q alignment");
+    check_rows(a.O, elem, "O alignment");
+    Staging st(s);
+    p.batch = paged_batch_of(a.batch, st);
+    const uint32_t T = p.batch.tokens;
+    if (!T || !p.batch.batch) return;
+    if (static_cast<uint64_t>(T) * a.q_heads > 0x7fffffffu)
+        throw CommandError("paged_attention has too many query rows", VNPU_ERR_UNSUPPORTED);
+    const uint64_t qw = static_cast<uint64_t>(a.q_heads) * d;
+    p.ldq = a.ldq;
+    p.ldo = a.ldo;
+    const uint64_t in_span = row_span(T, qw, p.ldq, elem);
+    const uint64_t out_span = row_span(T, qw, p.ldo, elem);
+    if (a.Q == a.O && p.ldq != p.ldo)
+        throw CommandError("in-place attention needs one row stride", VNPU_ERR_INVALID_ARGUMENT);
+    p.O = st.out(static_cast<char *>(a.O), out_span, true);
+    p.Q = st.in(static_cast<const char *>(a.Q), in_span);
+    p.q_heads = a.q_heads;
+    p.type = paged_row_type(a.dtype);
+    p.causal = a.causal != 0;
+    p.window = a.window;
+    p.max_length = a.max_length;
+    p.scale = a.scale != 0.0f ? a.scale : 1.0f / std::sqrt(static_cast<float>(d));
+    cuda_check(paged_attention(ctx, p), "paged_attention launch");
+    st.finish();
+    // The lengths are device data: the accounting counts the rows, and max_length keys for each
+    // sequence where the caller gave it.
+    const uint64_t keys = static_cast<uint64_t>(a.max_length) * p.batch.batch;
+    acc.bytes_read = T * qw * elem + 2 * keys * a.cache.heads * d;
+    acc.bytes_written = T * qw * elem;
+    acc.flops = 4ull * T * a.max_length * qw;
+    acc.dma = st.staged_bytes();
+}
+
 // C = R + MATMUL_I8(A, B): the GEMV epilogue for one row, else MATMUL_I8
 // then ADD_F32's addition.
 void exec_matmul_i8_residual(vnpu_stream_t *s, const vnpu_command_t &cmd, uint32_t flags,
@@ -1208,7 +1421,9 @@ vnpu_status_t execute_command(vnpu_stream_t *s, const vnpu_command_t &cmd, uint3
         cmd.opcode != VNPU_B200_OP_SWIGLU_QUANTIZE_I8 && cmd.opcode != VNPU_B200_OP_KV_APPEND &&
         cmd.opcode != VNPU_B200_OP_MATMUL_I8_SCATTER &&
         cmd.opcode != VNPU_B200_OP_QKV_ROPE_APPEND && cmd.opcode != VNPU_B200_OP_MATMUL_I8_RESIDUAL &&
-        cmd.opcode != VNPU_B200_OP_MATMUL_I8_SHARD && cmd.opcode != VNPU_B200_OP_MATMUL_I8_SWIGLU)
+        cmd.opcode != VNPU_B200_OP_MATMUL_I8_SHARD && cmd.opcode != VNPU_B200_OP_MATMUL_I8_SWIGLU &&
+        cmd.opcode != VNPU_B200_OP_PAGED_KV_APPEND && cmd.opcode != VNPU_B200_OP_PAGED_KV_READ &&
+        cmd.opcode != VNPU_B200_OP_PAGED_ATTENTION)
         return VNPU_ERR_INVALID_COMMAND;
     dev->last_opcode.store(cmd.opcode);
     const bool tracing = dev->trace.enabled.load();
@@ -1254,6 +1469,9 @@ vnpu_status_t execute_command(vnpu_stream_t *s, const vnpu_command_t &cmd, uint3
         case VNPU_B200_OP_MATMUL_I8_RESIDUAL: exec_matmul_i8_residual(s, cmd, flags, ctx, acc); break;
         case VNPU_B200_OP_MATMUL_I8_SHARD: exec_matmul_i8_shard(s, cmd, flags, ctx, acc); break;
         case VNPU_B200_OP_MATMUL_I8_SWIGLU: exec_matmul_i8_swiglu(s, cmd, flags, ctx, acc); break;
+        case VNPU_B200_OP_PAGED_KV_APPEND: exec_paged_kv_append(s, cmd, ctx, acc); break;
+        case VNPU_B200_OP_PAGED_KV_READ: exec_paged_kv_read(s, cmd, ctx, acc); break;
+        case VNPU_B200_OP_PAGED_ATTENTION: exec_paged_attention(s, cmd, ctx, acc); break;
         case VNPU_OP_MEMSET: exec_memset(s, cmd, acc); break;
         case VNPU_OP_PACK_WEIGHTS_I8: exec_pack(s, cmd, acc); break;
         default:
@@ -1367,6 +1585,9 @@ const char *opcode_name(uint32_t op) {
     if (op == VNPU_B200_OP_MATMUL_I8_RESIDUAL) return "MATMUL_I8_RESIDUAL";
     if (op == VNPU_B200_OP_MATMUL_I8_SHARD) return "MATMUL_I8_SHARD";
     if (op == VNPU_B200_OP_MATMUL_I8_SWIGLU) return "MATMUL_I8_SWIGLU";
+    if (op == VNPU_B200_OP_PAGED_KV_APPEND) return "PAGED_KV_APPEND";
+    if (op == VNPU_B200_OP_PAGED_KV_READ) return "PAGED_KV_READ";
+    if (op == VNPU_B200_OP_PAGED_ATTENTION) return "PAGED_ATTENTION";
     return op < sizeof(names) / sizeof(names[0]) ? names[op] : "UNKNOWN";
 }
 

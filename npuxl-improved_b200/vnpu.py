@@ -281,6 +281,133 @@ class MatmulI8SwigluArgs(C.Structure):
                 ("alpha", C.c_float), ("reserved0", u32)]
 
 
+# Paged 8-bit key/value cache (include/vnpu_b200.h)
+OP_B200_PAGED_KV_APPEND = 0x109
+OP_B200_PAGED_KV_READ = 0x10A
+OP_B200_PAGED_ATTENTION = 0x10B
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+PAGED_INTERLEAVED = 1 << 0
+PAGED_NO_ROPE = 1 << 1
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("K", vp), ("V", vp), ("K_scale", vp), ("V_scale", vp), ("num_pages", u32),
+                ("heads", u32), ("page_size", u32), ("head_dim", u32)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("block_table", vp), ("cu_tokens", vp), ("seq_lens", vp), ("batch", u32),
+                ("table_stride", u32), ("tokens", u32), ("max_tokens", u32)]
+
+
+class PagedKvAppendArgs(C.Structure):
+    _fields_ = [("cache", PagedCache), ("batch", PagedBatch), ("Q", vp), ("K", vp), ("V", vp),
+                ("Q_out", vp), ("ldq", u32), ("ldk", u32), ("ldv", u32), ("ldqo", u32),
+                ("q_heads", u32), ("dtype", u32), ("flags", u32), ("rotary_dim", u32),
+                ("theta_base", f32), ("scaling", f32)]
+
+
+class PagedKvReadArgs(C.Structure):
+    _fields_ = [("cache", PagedCache), ("batch", PagedBatch), ("K_out", vp), ("V_out", vp),
+                ("ld_row", u64), ("ld_head", u64), ("dtype", u32), ("reserved0", u32)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [("cache", PagedCache), ("batch", PagedBatch), ("Q", vp), ("O", vp), ("ldq", u32),
+                ("ldo", u32), ("q_heads", u32), ("dtype", u32), ("causal", u32), ("window", u32),
+                ("max_length", u32), ("scale", f32)]
+
+
+def _paged_dtype(*tensors) -> int:
+    """The vnpu dtype that all of the given torch tensors (None left out) have."""
+    names = {str(t.dtype).rsplit(".", 1)[-1] for t in tensors if t is not None}
+    known = {"float32": DTYPE_F32, "float16": DTYPE_F16, "bfloat16": DTYPE_BF16}
+    if len(names) != 1 or not names <= set(known):
+        raise TypeError(f"rows of one type among {sorted(known)}: got {sorted(names)}")
+    return known[names.pop()]
+
+
+def _int32(name, t):
+    if not str(t.dtype).endswith("int32"):
+        raise TypeError(f"{name}: int32, got {t.dtype}")
+    return t
+
+
+def _row_stride(name, t, width: int) -> int:
+    """Row stride in elements of a [rows][width] or [rows][heads][dim] tensor, rows dense inside."""
+    inner = 1
+    for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n > 1 and st != inner:
+            raise ValueError(f"{name}: the elements of a row lie one after the other, got "
+                             f"strides {tuple(t.stride())}")
+        inner *= n
+    if inner != width:
+        raise ValueError(f"{name}: rows of {width} elements, got {inner}")
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
+def paged_cache(k, v, k_scale, v_scale) -> PagedCache:
+    """A paged cache over torch tensors: int8 codes [pages][heads][page_size][head_dim] and f32
+    scales [pages][heads], all contiguous on the device."""
+    pages, heads, page_size, head_dim = k.shape
+    for name, t, shape, kind in (("k", k, tuple(k.shape), "int8"), ("v", v, tuple(k.shape), "int8"),
+                                 ("k_scale", k_scale, (pages, heads), "float32"),
+                                 ("v_scale", v_scale, (pages, heads), "float32")):
+        if tuple(t.shape) != shape or not str(t.dtype).endswith(kind) or not t.is_contiguous():
+            raise ValueError(f"{name}: contiguous {kind} of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    return PagedCache(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, heads, page_size, head_dim)
+
+
+def paged_batch(block_table, cu_tokens, seq_lens, tokens: int, max_tokens: int = 0) -> PagedBatch:
+    """The sequences of a paged command (vnpu_b200_paged_batch_t): int32 tensors block_table
+    [batch][stride], cu_tokens [batch + 1] and seq_lens [batch] (lengths with the rows counted in)."""
+    n = seq_lens.shape[0]
+    if block_table.shape[0] != n or cu_tokens.shape[0] != n + 1:
+        raise ValueError(f"block_table [{n}][...] and cu_tokens [{n + 1}] for {n} lengths")
+    for name, t in (("block_table", block_table), ("cu_tokens", cu_tokens), ("seq_lens", seq_lens)):
+        _int32(name, t)
+        if t.shape and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name}: entries lie one after the other")
+    stride = block_table.stride(0) if n > 1 else block_table.shape[1]
+    return PagedBatch(ptr(block_table), ptr(cu_tokens), ptr(seq_lens), n, stride, tokens, max_tokens)
+
+
+def paged_kv_append_cmd(cache: PagedCache, batch: PagedBatch, q, k, v, q_out, *, q_heads: int = 0,
+                        interleaved: bool = False, rope: bool = True, rotary_dim: int = 0,
+                        theta: float = 10000.0, scaling: float = 1.0) -> "Command":
+    """VNPU_B200_OP_PAGED_KV_APPEND: rotates q into q_out (or q None: no queries) and k, and
+    appends k and v ([tokens][heads * head_dim], row-strided views allowed) to the cache."""
+    d, h = cache.head_dim, cache.heads
+    flags = (PAGED_INTERLEAVED if interleaved else 0) | (0 if rope else PAGED_NO_ROPE)
+    return b200_command(OP_B200_PAGED_KV_APPEND, PagedKvAppendArgs(
+        cache, batch, ptr(q), ptr(k), ptr(v), ptr(q_out),
+        _row_stride("q", q, q_heads * d) if q is not None else 0, _row_stride("k", k, h * d),
+        _row_stride("v", v, h * d), _row_stride("q_out", q_out, q_heads * d) if q_out is not None else 0,
+        q_heads, _paged_dtype(q, k, v, q_out), flags, rotary_dim, theta, scaling))
+
+
+def paged_kv_read_cmd(cache: PagedCache, batch: PagedBatch, k_out, v_out) -> "Command":
+    """VNPU_B200_OP_PAGED_KV_READ into k_out and v_out, [tokens][heads][head_dim] views of one
+    layout with dense head_dim (token-major, or head-major through a transposed view)."""
+    outs = [t for t in (k_out, v_out) if t is not None]
+    if not outs or any(tuple(t.shape[1:]) != (cache.heads, cache.head_dim) or t.stride(2) != 1 or
+                       t.stride() != outs[0].stride() for t in outs):
+        raise ValueError("k_out, v_out: [tokens][heads][head_dim] of one layout, dense head_dim")
+    return b200_command(OP_B200_PAGED_KV_READ, PagedKvReadArgs(
+        cache, batch, ptr(k_out), ptr(v_out), outs[0].stride(0), outs[0].stride(1),
+        _paged_dtype(*outs), 0))
+
+
+def paged_attention_cmd(cache: PagedCache, batch: PagedBatch, q, o, *, causal: bool = True,
+                        window: int = 0, scale: float = 0.0, max_length: int = 0) -> "Command":
+    """VNPU_B200_OP_PAGED_ATTENTION: q, o [tokens][q_heads][head_dim] (rows may be strided)."""
+    heads = q.shape[1]
+    width = heads * cache.head_dim
+    return b200_command(OP_B200_PAGED_ATTENTION, PagedAttentionArgs(
+        cache, batch, ptr(q), ptr(o), _row_stride("q", q, width), _row_stride("o", o, width), heads,
+        _paged_dtype(q, o), int(causal), window, max_length, scale))
+
+
 def b200_command(opcode: int, args: C.Structure) -> "Command":
     """A command whose arguments are a B200 extension struct (copied into args.raw)."""
     c = Command()
@@ -636,6 +763,20 @@ class Device:
             self.lib.check(rc, "attention_f32")
         else:
             self.lib.check(self.lib.attention_f32(self.stream, C.byref(a)), "attention_f32")
+
+    # -- paged 8-bit key/value cache -------------------------------------------
+    def paged_kv_append(self, cache, batch, q, k, v, q_out, **options) -> None:
+        self._run(paged_kv_append_cmd(cache, batch, q, k, v, q_out, **options), "paged_kv_append")
+
+    def paged_kv_read(self, cache, batch, k_out, v_out) -> None:
+        self._run(paged_kv_read_cmd(cache, batch, k_out, v_out), "paged_kv_read")
+
+    def paged_attention(self, cache, batch, q, o, **options) -> None:
+        self._run(paged_attention_cmd(cache, batch, q, o, **options), "paged_attention")
+
+    def _run(self, cmd, what: str) -> None:
+        self.lib.check(self.submit([cmd]), what)
+        self.lib.check(self.sync(), what)
 
     def submit(self, cmds, event=None) -> int:
         arr = (Command * len(cmds))(*cmds)
