@@ -20,7 +20,7 @@
 // the accumulators are rescaled a few times a row instead of at every step.
 #include <algorithm>
 
-#include "paged_common.cuh"
+#include "paged_attention.cuh"
 
 namespace vnpu_b200 {
 namespace {
@@ -28,23 +28,6 @@ namespace {
 constexpr uint32_t kWarps = 4, kThreadsA = kWarps * 32;
 constexpr uint32_t kTile = 128;      // keys of a work unit, 32 for each warp
 constexpr uint32_t kWarpKeys = kTile / kWarps;
-constexpr float kSlack = 6.0f;       // growth of the maximum before a rescale (log2)
-constexpr float kLift = 8.0f;        // weights are scaled by 2^8: small ones stay normal numbers
-
-struct AttnParams {
-    PagedCache c;
-    PagedBatch pb;
-    const void *Q;
-    void *O;
-    uint32_t ldq, ldo, group;
-    uint32_t causal, window;
-    float scale_log2;
-    uint32_t vec;          // bit 0: Q 16-byte accesses, bit 1: O 4-element accesses
-    float *ws_o;           // [2 * grid][MR][DP] partial sums
-    float2 *ws_ml;         // [2 * grid][MR] their m and l
-    uint4 *ws_meta;        // [2 * grid]: who joins what
-    uint32_t *err;
-};
 
 template <uint32_t DP>
 struct AttnShape {
@@ -63,18 +46,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack_half2(uint32_t w) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 __device__ __forceinline__ float quad_max(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
@@ -220,14 +191,6 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
 
     uint8_t *const ring = smem + warp * (S * Shape::kSlot);
 
-    // Positions the row tile's first and last row see (the last row's limits
-    // are the widest above, the first row's the widest below).
-    const auto row_limits = [&](const Cursor &k, uint32_t r, int32_t &kmin, int32_t &kmax) {
-        const uint32_t rows = static_cast<uint32_t>(k.s.n) * p.group;
-        const int32_t pos = k.s.start + static_cast<int32_t>(min(r, rows - 1) / p.group);
-        kmax = p.causal ? pos : k.s.len - 1;
-        kmin = p.window && static_cast<uint32_t>(pos) + 1u > p.window ? pos + 1 - static_cast<int32_t>(p.window) : 0;
-    };
     // Pages of the two 16-key groups of `ahead`'s part of this warp.
     int32_t page_next[2];
     const auto fetch_pages = [&]() {
@@ -247,8 +210,8 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
             const int32_t k0 = ahead.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
             uint8_t *const dst = ring + slot_in * Shape::kSlot;
             int32_t kmin0, kmax1, unused;
-            row_limits(ahead, ahead.rt * MR, kmin0, unused);
-            row_limits(ahead, ahead.rt * MR + MR - 1, unused, kmax1);
+            row_limits(p, ahead.s, ahead.rt * MR, kmin0, unused);
+            row_limits(p, ahead.s, ahead.rt * MR + MR - 1, unused, kmax1);
             uint64_t base[2];
             bool ok[2];
 #pragma unroll
@@ -299,13 +262,13 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
     const auto begin_rows = [&]() {
         first_tile = cur.tile;
         const uint32_t rows = static_cast<uint32_t>(cur.s.n) * p.group;
-        row_limits(cur, cur.rt * MR, kmin_first, kmax_first);
-        row_limits(cur, cur.rt * MR + MR - 1, kmin_last, kmax_last);
+        row_limits(p, cur.s, cur.rt * MR, kmin_first, kmax_first);
+        row_limits(p, cur.s, cur.rt * MR + MR - 1, kmin_last, kmax_last);
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
             if (kSplit && i == 1) break;
             const uint32_t r = cur.rt * MR + n + 8 * i;
-            row_limits(cur, r, kmin[i], kmax[i]);
+            row_limits(p, cur.s, r, kmin[i], kmax[i]);
             m[i] = -INFINITY;
             l[i] = 0.0f;
             float v[NG][16];
@@ -332,11 +295,9 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
                 for (uint32_t e = 0; e < 16; ++e) most = fmaxf(most, fabsf(v[g][e]));
             }
             most = quad_max(most);
-            // 2^k with most * 2^k in [2^13, 2^14); rows of zeros, and of infinities, stay
-            int ex = static_cast<int>((__float_as_uint(most) >> 23) & 255u) - 127;
-            ex = most > 0.0f && most <= 3.402823466e38f ? max(-114, min(100, 13 - ex)) : 0;
-            const float up = __int_as_float((127 + ex) << 23);
-            qf[i] = p.scale_log2 * __int_as_float((127 - ex) << 23);
+            const int ex = row_exponent(most);
+            const float up = pow2(ex);
+            qf[i] = p.scale_log2 * pow2(-ex);
 #pragma unroll
             for (uint32_t g = 0; g < NG; ++g)
 #pragma unroll
@@ -741,6 +702,10 @@ cudaError_t launch_by_dim(const LaunchCtx &ctx, const PagedAttention &a) {
 }  // namespace
 
 cudaError_t paged_attention(const LaunchCtx &ctx, const PagedAttention &a) {
+    if (1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > 32) {
+        const cudaError_t e = paged_attention_many_rows(ctx, a);
+        if (e != cudaErrorNotSupported) return e;
+    }
     switch (a.type) {
     case RowType::kF32: return launch_by_dim<RowType::kF32>(ctx, a);
     case RowType::kF16: return launch_by_dim<RowType::kF16>(ctx, a);

@@ -1,0 +1,66 @@
+// paged_attention.cuh - shared by the two kernels of PAGED_ATTENTION: the one
+// for few query rows (paged_attention.cu) and the tensor-memory one for many
+// (paged_prefill.cu).
+#pragma once
+
+#include "paged_common.cuh"
+
+namespace vnpu_b200 {
+
+// The kernel for many rows: takes a shape or answers cudaErrorNotSupported.
+cudaError_t paged_attention_many_rows(const LaunchCtx &ctx, const PagedAttention &a);
+
+namespace {
+
+// What the attention kernels share: scaled weights (paged_attention.cu has the
+// mathematics) and the parameters.
+constexpr float kSlack = 6.0f;       // growth of the maximum before a rescale (log2)
+constexpr float kLift = 8.0f;        // weights are scaled by 2^8: small ones stay normal numbers
+
+struct AttnParams {
+    PagedCache c;
+    PagedBatch pb;
+    const void *Q;
+    void *O;
+    uint32_t ldq, ldo, group;
+    uint32_t causal, window;
+    float scale_log2;
+    uint32_t vec;          // bit 0: Q 16-byte accesses, bit 1: O 4-element, bit 2: O 16-byte accesses
+    float *ws_o;           // [2 * grid][tile rows][DP] partial sums
+    float2 *ws_ml;         // [2 * grid][tile rows] their m and l
+    uint4 *ws_meta;        // [2 * grid]: who joins what
+    uint32_t *err;
+    uint64_t limit_ns;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+// The power of two that brings a row's largest element to [2^13, 2^14), as an
+// exponent; rows of zeros, and of infinities, stay as they are.
+__device__ __forceinline__ int row_exponent(float most) {
+    const int ex = static_cast<int>((__float_as_uint(most) >> 23) & 255u) - 127;
+    return most > 0.0f && most <= 3.402823466e38f ? max(-114, min(100, 13 - ex)) : 0;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+
+// Positions that row r (clamped to the sequence's last) of a sequence sees.
+__device__ __forceinline__ void row_limits(const AttnParams &p, const PagedSeq &s, uint32_t r,
+                                           int32_t &kmin, int32_t &kmax) {
+    const uint32_t rows = static_cast<uint32_t>(s.n) * p.group;
+    const int32_t pos = s.start + static_cast<int32_t>(min(r, rows - 1) / p.group);
+    kmax = p.causal ? pos : s.len - 1;
+    kmin = p.window && static_cast<uint32_t>(pos) + 1u > p.window ? pos + 1 - static_cast<int32_t>(p.window) : 0;
+}
+
+}  // namespace
+}  // namespace vnpu_b200

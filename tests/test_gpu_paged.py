@@ -521,7 +521,7 @@ def test_step_in_a_graph_follows_the_device_arrays(gpu, torch):
         s.ks, s.vs = s.dks.cpu().numpy(), s.dvs.cpu().numpy()
         s.spans = [(1, 10 + step), (1, 31 + step)]
         q64 = q_rot.double().cpu().numpy().reshape(2, -1)
-        check_attention(o, *attention64(s2, q64, hq, True, 0), "bf16")
+        check_attention(o, *attention64(s, q64, hq, True, 0), "bf16")
         s.dlens.add_(1)
     gpu.lib.b200_graph_destroy(graph)
 
