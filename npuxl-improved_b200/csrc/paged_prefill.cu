@@ -1,25 +1,30 @@
 // paged_prefill.cu - PAGED_ATTENTION for many query rows: both products on the
 // 5th-generation tensor cores, accumulators in tensor memory.
 //
-// The mathematics is paged_attention.cu's.  A CTA works on 128 query rows of
-// one key/value head (tokens x grouped heads, packed) and walks their keys in
-// tiles of KT: four converter warps turn the tile's codes into f16 in shared
-// memory (exact), one thread issues S = Q K^T and O += P V, and four softmax
-// warps, one row a thread, read S from tensor memory, write the weights P back
-// over it as f16 (the A operand of the second product comes from tensor
-// memory), and rescale O there when a maximum grew.  Two CTAs share an SM, so
-// one's softmax runs under the other's products and under its own first and
-// last tiles.
+// The mathematics is paged_attention.cu's.  A CTA, one an SM, works on 256 query
+// rows of one key/value head (tokens x grouped heads, packed) and walks their
+// keys in tiles of KT.  Its warps:
+//   13      copies a tile's codes to shared memory (bulk copies of 16 keys, two
+//           tiles ahead) and its page scales beside them;
+//   8-11    turn the codes into f16 (exact), in the swizzled layout of the
+//           tensor core's operands;
+//   12      one thread issues S = Q K^T and O += P V for both halves of the rows;
+//   0-3, 4-7  softmax of 128 rows each, one row a thread: S is read from tensor
+//           memory, the weights go back over it as f16 (the second product takes
+//           its A operand from there), and O is rescaled there when a row's
+//           maximum grew.  One half's softmax runs under the other's products.
+// The weights of a tile are first computed with the maximum so far; only when
+// some row exceeds it by 2^6 are they computed again, so a tile is read once.
 //
 // f32 rows: Q = hi + lo in f16 (22 bits), P likewise; each product is two
 // tensor instructions on the same accumulator, with tiles of 64 keys so that S
 // and both halves of P fit beside each other.
 //
-// What bounds it: at head_dim 128 a 128 x 128 tile costs 16384 exponentials at
-// 16 a clock (1024 clocks) against 512 clocks of the tensor core, and about as
-// much again in issue slots for the conversion, the maxima and the scaling.
+// What bounds it: at head_dim 128 a 256 x 128 tile costs 32768 exponentials at
+// 16 a clock (2048 clocks) against 2048 clocks of the tensor core, with about
+// 1400 issue slots a scheduler beside them.
 //
-// Work units are (head, block of 128 rows, key tile), counted exactly by a
+// Work units are (head, block of 256 rows, key tile), counted exactly by a
 // planning kernel of one block; every CTA gets an equal run of them, whatever
 // the sequences' lengths, the mask and the number of rows, and blocks that
 // are split over CTAs are joined afterwards.
@@ -30,8 +35,10 @@
 namespace vnpu_b200 {
 namespace {
 
-constexpr uint32_t kRows = 128;              // query rows of a block (UMMA M)
-constexpr uint32_t kManyThreads = 288;       // 4 softmax, 4 converter, 1 tensor-issue warps
+constexpr uint32_t kHalf = 128;              // rows of one accumulator (UMMA M)
+constexpr uint32_t kRows = 2 * kHalf;        // query rows of a block
+constexpr uint32_t kManyThreads = 512;       // 8 softmax, 4 converter, tensor-issue, copy and 2 spare warps
+constexpr uint32_t kScaleRing = 4;           // tiles whose scales are kept
 constexpr uint32_t kPlanThreads = 1024;
 
 // A block of rows and the key tiles that any of its rows sees.
@@ -161,14 +168,6 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t 
     d &= ~(0x3fffull << 16);
     return d | (static_cast<uint64_t>(chunk >> 4) << 16);
 }
-__device__ __forceinline__ void tmem_st_16cols(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st_32cols(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -184,16 +183,23 @@ __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 template <RowType T, uint32_t DP>
 struct ManyShape {
     static constexpr bool kSplit = T == RowType::kF32;
     static constexpr uint32_t KT = kSplit ? 64 : 128;          // keys of a tile
-    static constexpr uint32_t NB = DP / 64;                     // 64-element column blocks
-    static constexpr uint32_t kQBytes = kRows * DP * 2 * (kSplit ? 2 : 1);
-    static constexpr uint32_t kKvBytes = KT * DP * 2;
-    static constexpr uint32_t kSmem = kQBytes + 2 * kKvBytes + 1024;
-    // tensor memory: S (KT columns; P over it, or for f32 hi and lo after it), O from column 128
-    static constexpr uint32_t kPCol = kSplit ? 64 : 0, kOCol = 128, kCols = 256;
+    static constexpr uint32_t kQHalf = kHalf * DP * 2 * (kSplit ? 2 : 1);
+    static constexpr uint32_t kKvBytes = KT * DP * 2;           // a tile of K or V in f16
+    static constexpr uint32_t kRawBytes = KT * DP;              // its codes
+    // queries, K, two of V, two tiles' codes of each
+    static constexpr uint32_t kSmem = 2 * kQHalf + 3 * kKvBytes + 4 * kRawBytes + 1024;
+    // tensor memory of a half: S (KT columns; P over it, or for f32 hi and lo after it), O
+    static constexpr uint32_t kPCol = kSplit ? 64 : 0, kOCol = 128, kHalfCols = 256;
 };
 
 // Where a CTA stands in the units: head, block, tile; the roles walk alike.
@@ -229,16 +235,23 @@ struct Walk {
 };
 
 template <RowType T, uint32_t DP>
-__global__ void __launch_bounds__(kManyThreads, 2)
-    paged_prefill_kernel(const AttnParams p, const Plan plan) {
+__global__ void __launch_bounds__(kManyThreads, 1)
+    paged_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ Plan plan) {
     using E = typename RowOf<T>::type;
     using Shape = ManyShape<T, DP>;
     constexpr bool kSplit = Shape::kSplit;
-    constexpr uint32_t KT = Shape::KT, NB = Shape::NB;
+    constexpr uint32_t KT = Shape::KT, kGroups = KT / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *const sq = smem, *const sk = smem + Shape::kQBytes, *const sv = sk + Shape::kKvBytes;
-    __shared__ uint64_t bar_q, bar_o, bar_s, bar_p, bar_k, bar_k_free, bar_v, bar_v_free;
+    uint8_t *const sq = smem, *const sk = smem + 2 * Shape::kQHalf, *const sv = sk + Shape::kKvBytes;
+    uint8_t *const raw_k = sv + 2 * Shape::kKvBytes, *const raw_v = raw_k + 2 * Shape::kRawBytes;
+    __shared__ uint64_t bar_q[2], bar_o[2], bar_s[2], bar_p[2];          // of a half
+    __shared__ uint64_t bar_k, bar_k_free, bar_v[2], bar_v_free[2];      // f16 tiles
+    __shared__ uint64_t bar_rk[2], bar_rk_free[2], bar_rv[2], bar_rv_free[2];  // codes
+    __shared__ uint64_t bar_sc[kScaleRing];
+    // a tile's 16-key groups: K scale, log2 of the V scale, 1 / V scale; pages of zeros as bits
+    __shared__ __align__(16) float sh_k[kScaleRing][8], sh_lv[kScaleRing][8], sh_iv[kScaleRing][8];
+    __shared__ uint32_t sh_zeros[kScaleRing];
     __shared__ uint32_t sh_tmem;
     __shared__ int sh_abort;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, cta = blockIdx.x;
@@ -246,18 +259,27 @@ __global__ void __launch_bounds__(kManyThreads, 2)
 
     if (tid == 0) {
         sh_abort = 0;
-        mbar_init(&bar_q, 128);
-        mbar_init(&bar_p, 128);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(&bar_q[i], 128);
+            mbar_init(&bar_p[i], 128);
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_o[i], 1);
+            mbar_init(&bar_v[i], 128);
+            mbar_init(&bar_v_free[i], 1);
+            mbar_init(&bar_rk[i], 1);
+            mbar_init(&bar_rv[i], 1);
+            mbar_init(&bar_rk_free[i], 128);
+            mbar_init(&bar_rv_free[i], 128);
+        }
         mbar_init(&bar_k, 128);
-        mbar_init(&bar_v, 128);
-        mbar_init(&bar_s, 1);
-        mbar_init(&bar_o, 1);
         mbar_init(&bar_k_free, 1);
-        mbar_init(&bar_v_free, 1);
+#pragma unroll
+        for (uint32_t i = 0; i < kScaleRing; ++i) mbar_init(&bar_sc[i], 1);
         fence_barrier_init();
     }
-    if (warp == 8) {
-        tmem_alloc(&sh_tmem, Shape::kCols);
+    if (warp == 12) {
+        tmem_alloc(&sh_tmem, 2 * Shape::kHalfCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -299,127 +321,189 @@ __global__ void __launch_bounds__(kManyThreads, 2)
         w.e = lo;
         w.take(off - __ldcg(plan.before + lo));
     }
-    // who joins what: the last segment, when its block begins here and goes on
-    uint32_t parts = 0;
 
-    if (busy && warp < 4) {
+    // The block's 65536 registers go where they are needed: 256 x 168 + 256 x 88.  (The spare
+    // warps make up the fourth warpgroup, so that every scheduler's share adds up, too.)
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+
+    if (busy && warp < 8) {
         // =============================== softmax ===============================
-        const uint32_t row = tid;                                   // of the block; its TMEM lane
-        const uint32_t lanes = tmem + (warp * 32u << 16);
+        const uint32_t half = warp >> 2, quad = warp & 3u;
+        const uint32_t row = half * kHalf + quad * 32u + lane;       // of the block
+        const uint32_t lanes = tmem + half * Shape::kHalfCols + (quad << 21);   // lane quad * 32
+        uint8_t *const q_half = sq + half * Shape::kQHalf;
+        uint64_t *const full_s = &bar_s[half], *const full_p = &bar_p[half];
         float f_next = 0.0f;
-        // Query rows of a block to shared memory as f16, scaled by a power of two.
+        // Query rows to shared memory as f16, scaled by a power of two.  DP / 8 lanes take a
+        // row, so a warp reads whole rows, 64 registers of them in flight.
         const auto load_q = [&](const Walk &k) {
-            const uint32_t r = k.x.rb * kRows + row, token = r / p.group;
-            const bool live = r < static_cast<uint32_t>(k.s.n) * p.group;
-            const E *q = static_cast<const E *>(p.Q) +
-                         static_cast<uint64_t>(k.s.row0 + static_cast<int32_t>(token)) * p.ldq +
-                         (k.h * p.group + (r - token * p.group)) * D;
+            constexpr uint32_t LR = DP / 8, RI = 32 / LR;            // lanes a row, rows a step
+            constexpr uint32_t NS = kSplit ? (LR < 8 ? LR : 8) : LR; // steps in flight
+            const uint32_t d = (lane % LR) * 8, rows = static_cast<uint32_t>(k.s.n) * p.group;
             const bool vec = p.vec & 1u;
-            float most = 0.0f;
-            if (live)
-                for (uint32_t d = 0; d < D; d += 8) {
-                    float x[8];
-                    load8(q + d, vec, x);
+            int ex_mine = 0;
+            const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < LR; i0 += NS) {
+                alignas(16) E x[NS][8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[i]));
-                }
-            const int ex = row_exponent(most);
-            const float up = p.scale_log2 < 0.0f ? -pow2(ex) : pow2(ex);
-            f_next = fabsf(p.scale_log2) * pow2(-ex);
-#pragma unroll 4
-            for (uint32_t d = 0; d < DP; d += 8) {
-                float x[8] = {};
-                if (live && d < D) load8(q + d, vec, x);
-                uint4 hi, lo;
-                uint32_t *h = reinterpret_cast<uint32_t *>(&hi), *l = reinterpret_cast<uint32_t *>(&lo);
+                for (uint32_t i = 0; i < NS; ++i) {
+                    const uint32_t r = k.x.rb * kRows + (row & ~31u) + (i0 + i) * RI + lane / LR;
+                    const uint32_t token = r / p.group;
+                    uint4 *v = reinterpret_cast<uint4 *>(x[i]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
-                    h[i] = pack_half2(a, b);
-                    if constexpr (kSplit) {
-                        const float2 g = unpack_half2(h[i]);
-                        l[i] = pack_half2(a - g.x, b - g.y);
+                    for (uint32_t e = 0; e < sizeof(E) / 2; ++e) v[e] = make_uint4(0, 0, 0, 0);
+                    if (r < rows && d < D) {
+                        const E *src = static_cast<const E *>(p.Q) +
+                                       static_cast<uint64_t>(k.s.row0 + static_cast<int32_t>(token)) * p.ldq +
+                                       (k.h * p.group + (r - token * p.group)) * D + d;
+                        if (vec) {
+#pragma unroll
+                            for (uint32_t e = 0; e < sizeof(E) / 2; ++e)
+                                v[e] = __ldg(reinterpret_cast<const uint4 *>(src) + e);
+                        } else {
+#pragma unroll
+                            for (uint32_t e = 0; e < 8; ++e) x[i][e] = src[e];
+                        }
                     }
                 }
-                uint8_t *dst = sq + (d / 64) * (kRows * 128) + row * 128 + ((((d / 8) & 7u) ^ (row & 7u)) * 16);
-                *reinterpret_cast<uint4 *>(dst) = hi;
-                if constexpr (kSplit) *reinterpret_cast<uint4 *>(dst + kRows * DP * 2) = lo;
+#pragma unroll
+                for (uint32_t i = 0; i < NS; ++i) {
+                    float y[8], most = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        y[e] = to_f32(x[i][e]);
+                        most = fmaxf(most, fabsf(y[e]));
+                    }
+#pragma unroll
+                    for (uint32_t o = 1; o < LR; o <<= 1)
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    const int ex = row_exponent(most);
+                    const float up = sign * pow2(ex);
+                    // the lane that owns the row takes its exponent
+                    const uint32_t first = (i0 + i) * RI;
+                    const int got = __shfl_sync(0xffffffffu, ex, ((lane - first) * LR) & 31u);
+                    if (lane / RI == i0 + i) ex_mine = got;
+                    uint4 hi, lo;
+                    uint32_t *h = reinterpret_cast<uint32_t *>(&hi), *l = reinterpret_cast<uint32_t *>(&lo);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = y[2 * e] * up, b = y[2 * e + 1] * up;
+                        h[e] = pack_half2(a, b);
+                        if constexpr (kSplit) {
+                            const float2 g = unpack_half2(h[e]);
+                            l[e] = pack_half2(a - g.x, b - g.y);
+                        }
+                    }
+                    const uint32_t rr = quad * 32u + first + lane / LR;
+                    uint8_t *dst = q_half + (d / 64) * (kHalf * 128) + rr * 128 + ((((d / 8) & 7u) ^ (rr & 7u)) * 16);
+                    *reinterpret_cast<uint4 *>(dst) = hi;
+                    if constexpr (kSplit) *reinterpret_cast<uint4 *>(dst + kHalf * DP * 2) = lo;
+                }
             }
+            f_next = fabsf(p.scale_log2) * pow2(-ex_mine);
             fence_proxy_async_smem();
-            mbar_arrive(&bar_q);
+            mbar_arrive(&bar_q[half]);
         };
-        // A tile's 16-key groups: lane g < KT / 16 holds group g's K scale, log2 of its V scale,
-        // and 1 / V scale (0: a page of zeros, whose weights only count in the sum).
-        constexpr uint32_t kGroups = KT / 16;
-        float g_k = 0.0f, g_lv = 0.0f, g_iv = 1.0f, n_k = 0.0f, n_v = 0.0f;
-        const auto fetch_scales = [&](const Walk &k, int32_t tile) {
-            n_k = n_v = 0.0f;
-            const int32_t key = tile * static_cast<int32_t>(KT) + static_cast<int32_t>(lane * 16u);
-            if (lane >= kGroups || key >= k.s.len) return;
-            const int32_t page = __ldg(p.pb.table + static_cast<uint64_t>(k.x.b) * p.pb.table_stride +
-                                       (static_cast<uint32_t>(key) >> p.c.page_shift));
-            if (page < 0 || static_cast<uint32_t>(page) >= p.c.num_pages) return;  // converters report it
-            const uint64_t at = static_cast<uint64_t>(page) * p.c.heads + k.h;
-            n_k = __ldg(p.c.K_scale + at);
-            n_v = __ldg(p.c.V_scale + at);
+        const auto takes = [&](const Walk &k) {   // this half has rows of the block
+            return half == 0 || static_cast<uint32_t>(k.s.n) * p.group > k.x.rb * kRows + kHalf;
         };
-        load_q(w);
-        fetch_scales(w, w.tile);
-        uint32_t it = 0, seg = 0;
+        uint32_t tile_no = 0, done = 0, seg = 0;  // tiles of the run; tiles and segments of this half
         bool more = true;
+        if (takes(w)) load_q(w);
         while (more) {
             const float f = f_next;
             const Walk cur = w;
+            more = w.next();
+            const bool started = cur.tile == cur.x.lo;
+            const bool whole = started && cur.count == cur.x.nt;
+            const uint32_t rows = static_cast<uint32_t>(cur.s.n) * p.group;
+            if (tid == 0 && !more) {
+                // joined with the CTAs that go on with the block, when it begins here
+                const uint32_t parts = started && !whole
+                                           ? 1 + static_cast<uint32_t>((cur.x.nt - cur.count + run - 1) / run)
+                                           : 0;
+                p.ws_meta[2 * cta] = make_uint4(parts, static_cast<uint32_t>(cur.s.row0), cur.x.rb * kRows, cur.h);
+                p.ws_meta[2 * cta + 1] = make_uint4(min(kRows, rows - cur.x.rb * kRows), 0, 0, 0);
+            }
+            if (!takes(cur)) {
+                tile_no += static_cast<uint32_t>(cur.count);
+                if (more && takes(w)) load_q(w);
+                continue;
+            }
             int32_t kmin, kmax, kmin_last, kmax_first, unused;
             row_limits(p, cur.s, cur.x.rb * kRows + row, kmin, kmax);
-            row_limits(p, cur.s, cur.x.rb * kRows, unused, kmax_first);
-            row_limits(p, cur.s, cur.x.rb * kRows + kRows - 1, kmin_last, unused);
+            row_limits(p, cur.s, cur.x.rb * kRows + half * kHalf, unused, kmax_first);
+            row_limits(p, cur.s, cur.x.rb * kRows + half * kHalf + kHalf - 1, kmin_last, unused);
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
-            for (int32_t j = 0; j < cur.count; ++j, ++it) {
+            for (int32_t j = 0; j < cur.count; ++j, ++tile_no, ++done) {
                 const int32_t k0 = (cur.tile + j) * static_cast<int32_t>(KT);
-                g_k = n_k;
-                g_lv = n_v > 0.0f ? __log2f(n_v) : 0.0f;
-                g_iv = n_v > 0.0f ? ex2(-g_lv) : 1.0f;
-                const uint32_t zeros = __ballot_sync(0xffffffffu, lane < kGroups && !(n_v > 0.0f));
-                if (j + 1 < cur.count) fetch_scales(cur, cur.tile + j + 1);
+                const uint32_t ring = tile_no % kScaleRing;
                 const bool edge = k0 + static_cast<int32_t>(KT) - 1 > kmax_first || k0 < kmin_last;
-                if (!(ok = wait_warp(&bar_s, it))) break;
+                if (!(ok = wait_warp(&bar_sc[ring], tile_no / kScaleRing) && wait_warp(full_s, done))) break;
                 tc_fence_after();
-                // ---- the tile's maximum
-                float top = -INFINITY;
+                const uint32_t zeros = sh_zeros[ring];
+                uint32_t h[KT / 2], lo[kSplit ? KT / 2 : 1];
+                float sum;
+#pragma unroll 1
+                for (;;) {
+                    const float off = m == -INFINITY ? 0.0f : m - kLift;
+                    float top = -INFINITY;
+                    sum = 0.0f;
 #pragma unroll
-                for (uint32_t c = 0; c < KT / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_ld_32cols(lanes + 32 * c, r);
-                    tmem_wait_ld();
-                    if (edge) {
+                    for (uint32_t c = 0; c < KT / 32; ++c) {
+                        uint32_t r[32];
+                        tmem_ld_32cols(lanes + 32 * c, r);
+                        tmem_wait_ld();
+                        if (edge) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i) {
-                            const int32_t key = k0 + static_cast<int32_t>(32 * c + i);
-                            if (key > kmax || key < kmin) r[i] = 0xff800000u;  // -infinity
+                            for (uint32_t i = 0; i < 32; ++i) {
+                                const int32_t key = k0 + static_cast<int32_t>(32 * c + i);
+                                if (key > kmax || key < kmin) r[i] = 0xff800000u;  // -infinity
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t g = 0; g < 2; ++g) {
+                            const uint32_t gg = 2 * c + g;
+                            // a factor of zero would make masked scores NaN
+                            const float fg = fmaxf(f * sh_k[ring][gg], 1e-38f);
+                            const float b = sh_lv[ring][gg] - off;
+                            float x[4];
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i)
+                                x[i] = fmaxf(fmaxf(__uint_as_float(r[16 * g + i]), __uint_as_float(r[16 * g + 4 + i])),
+                                             fmaxf(__uint_as_float(r[16 * g + 8 + i]), __uint_as_float(r[16 * g + 12 + i])));
+                            // scales are not negative: the largest product is the largest score
+                            top = fmaxf(top, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fg, b));
+                            const uint64_t f2 = pack_f32x2(fg, fg), b2 = pack_f32x2(b, b);
+                            uint64_t s2 = 0;
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i) {
+                                const uint64_t t = fma_f32x2(
+                                    pack_f32x2(__uint_as_float(r[16 * g + 2 * i]), __uint_as_float(r[16 * g + 2 * i + 1])),
+                                    f2, b2);
+                                const float u = ex2(half_f32x2(t, 0)), v = ex2(half_f32x2(t, 1));
+                                s2 = add_f32x2(s2, pack_f32x2(u, v));
+                                h[8 * gg + i] = pack_half2(u, v);
+                                if constexpr (kSplit) {
+                                    const float2 y = unpack_half2(h[8 * gg + i]);
+                                    lo[8 * gg + i] = pack_half2(u - y.x, v - y.y);
+                                }
+                            }
+                            sum = fmaf(half_f32x2(s2, 0) + half_f32x2(s2, 1), sh_iv[ring][gg], sum);
                         }
                     }
-#pragma unroll
-                    for (uint32_t g = 0; g < 2; ++g) {
-                        float x = __uint_as_float(r[16 * g]);
-#pragma unroll
-                        for (uint32_t i = 1; i < 16; ++i) x = fmaxf(x, __uint_as_float(r[16 * g + i]));
-                        // scales are not negative: the largest product is the largest score
-                        const float fg = f * __shfl_sync(0xffffffffu, g_k, 2 * c + g);
-                        const float t = fmaf(x, fg, __shfl_sync(0xffffffffu, g_lv, 2 * c + g));
-                        top = fmaxf(top, x == -INFINITY ? x : t);
-                    }
-                }
-                // ---- rescale when some row's maximum grew by more than the slack
-                const bool grown = top > m + kSlack;
-                if (__any_sync(0xffffffffu, grown)) {
+                    top += off;
+                    if (!__any_sync(0xffffffffu, top > m + kSlack)) break;
+                    // some row's maximum grew by more than the slack: rescale, and again
                     const float to = fmaxf(m, top);
                     const float a = to > m ? ex2(m - to) : 1.0f;
                     l *= a;
                     m = to;
                     if (j) {   // S of this tile is done, so the products before it are
-#pragma unroll
+#pragma unroll 1
                         for (uint32_t c = 0; c < DP / 32; ++c) {
                             uint32_t r[32];
                             tmem_ld_32cols(lanes + Shape::kOCol + 32 * c, r);
@@ -431,67 +515,33 @@ __global__ void __launch_bounds__(kManyThreads, 2)
                         }
                     }
                 }
-                const float off = m == -INFINITY ? 0.0f : m - kLift;
-                // ---- weights
+                l += sum;
+                if (zeros) {   // pages of zeros count in the sum alone
 #pragma unroll
-                for (uint32_t c = 0; c < KT / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_ld_32cols(lanes + 32 * c, r);
-                    tmem_wait_ld();
-                    if (edge) {
-#pragma unroll
-                        for (uint32_t i = 0; i < 32; ++i) {
-                            const int32_t key = k0 + static_cast<int32_t>(32 * c + i);
-                            if (key > kmax || key < kmin) r[i] = 0xff800000u;
+                    for (uint32_t i = 0; i < KT / 2; ++i)
+                        if (zeros >> (i / 8) & 1u) {
+                            h[i] = 0;
+                            if constexpr (kSplit) lo[i] = 0;
                         }
-                    }
-                    uint32_t h[16], lo[16];
+                }
 #pragma unroll
-                    for (uint32_t g = 0; g < 2; ++g) {
-                        // a zero factor keeps a masked key masked: -infinity * 0 is none
-                        const float fg = fmaxf(f * __shfl_sync(0xffffffffu, g_k, 2 * c + g), 1e-38f);
-                        const float b = __shfl_sync(0xffffffffu, g_lv, 2 * c + g) - off;
-                        float sum = 0.0f;
-#pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i) {
-                            const float x = ex2(fmaf(__uint_as_float(r[16 * g + 2 * i]), fg, b));
-                            const float y = ex2(fmaf(__uint_as_float(r[16 * g + 2 * i + 1]), fg, b));
-                            sum += x + y;
-                            h[8 * g + i] = pack_half2(x, y);
-                            if constexpr (kSplit) {
-                                const float2 u = unpack_half2(h[8 * g + i]);
-                                lo[8 * g + i] = pack_half2(x - u.x, y - u.y);
-                            }
-                        }
-                        l = fmaf(sum, __shfl_sync(0xffffffffu, g_iv, 2 * c + g), l);
-                        if (zeros >> (2 * c + g) & 1u) {
-#pragma unroll
-                            for (uint32_t i = 0; i < 8; ++i) h[8 * g + i] = lo[8 * g + i] = 0;
-                        }
-                    }
-                    tmem_st_16cols(lanes + Shape::kPCol + 16 * c, h);
-                    if constexpr (kSplit) tmem_st_16cols(lanes + Shape::kPCol + 32 + 16 * c, lo);
+                for (uint32_t c = 0; c < KT / 64; ++c) {
+                    tmem_st_32cols(lanes + Shape::kPCol + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(h + 32 * c));
+                    if constexpr (kSplit)
+                        tmem_st_32cols(lanes + Shape::kPCol + 32, *reinterpret_cast<uint32_t(*)[32]>(lo));
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&bar_p);
+                mbar_arrive(full_p);
             }
             if (!ok) break;
             // All scores of this block are computed: the next block's queries may take its place.
-            more = w.next();
-            if (more) {
-                load_q(w);
-                fetch_scales(w, w.tile);
-            }
-            if (!wait_warp(&bar_o, seg++)) break;
+            if (more && takes(w)) load_q(w);
+            if (!wait_warp(&bar_o[half], seg++)) break;
             tc_fence_after();
             const uint32_t r = cur.x.rb * kRows + row, token = r / p.group;
-            const bool live = r < static_cast<uint32_t>(cur.s.n) * p.group;
-            const bool started = cur.tile == cur.x.lo;
-            const bool whole = started && cur.count == cur.x.nt;
+            const bool live = r < rows;
             const uint32_t part = 2 * cta + (started ? 1 : 0);
-            if (started && !whole)
-                parts = 1 + static_cast<uint32_t>((cur.x.nt - cur.count + run - 1) / run);
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             E *out = static_cast<E *>(p.O) +
                      static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldo +
@@ -520,48 +570,25 @@ __global__ void __launch_bounds__(kManyThreads, 2)
                 }
             }
             if (live && !whole) p.ws_ml[part * kRows + row] = make_float2(m, l);
-            if (tid == 0 && !more) {
-                p.ws_meta[2 * cta] = make_uint4(parts, static_cast<uint32_t>(cur.s.row0), cur.x.rb * kRows, cur.h);
-                p.ws_meta[2 * cta + 1] = make_uint4(
-                    min(kRows, static_cast<uint32_t>(cur.s.n) * p.group - cur.x.rb * kRows), 0, 0, 0);
-            }
             tc_fence_before();
         }
-    } else if (busy && warp < 8) {
+    } else if (busy && warp < 12) {
         // =============================== conversion ===============================
         constexpr uint32_t NC = DP / 16, RP = 128 / NC, NI = KT / RP;   // chunks a row, rows a step, steps
-        const uint32_t ct = tid - 128, chunk = ct % NC, row0 = ct / NC;
-        uint4 raw_k[NI], raw_v[NI];
-        const uint32_t ps_mask = (1u << p.c.page_shift) - 1u;
-        // A tile's codes of this thread; what is not there is zero.
-        const auto fetch = [&](const Walk &k, int32_t tile, const int8_t *pool, uint4 (&raw)[NI]) {
-#pragma unroll
-            for (uint32_t i = 0; i < NI; ++i) {
-                const int32_t key = tile * static_cast<int32_t>(KT) + static_cast<int32_t>(i * RP + row0);
-                raw[i] = make_uint4(0, 0, 0, 0);
-                if (key >= k.s.len || chunk * 16u >= D) continue;
-                const int32_t page = __ldg(p.pb.table + static_cast<uint64_t>(k.x.b) * p.pb.table_stride +
-                                           (static_cast<uint32_t>(key) >> p.c.page_shift));
-                if (page < 0 || static_cast<uint32_t>(page) >= p.c.num_pages) {
-                    record_error(p.err, kErrBadIndex);
-                    continue;
-                }
-                const uint64_t at = static_cast<uint64_t>(page) * p.c.heads + k.h;
-                raw[i] = __ldg(reinterpret_cast<const uint4 *>(
-                    pool + ((at << p.c.page_shift) + (static_cast<uint32_t>(key) & ps_mask)) * D + chunk * 16u));
-            }
-        };
+        const uint32_t ct = tid - 256, chunk = ct % NC, row0 = ct / NC;
+        const bool there = chunk * 16u < D;      // columns past head_dim are zeros
         // 16 codes to two 16-byte pieces of a 128-byte swizzled row; the columns' upper half
         // writes its pieces in the other order, so that 8 lanes of a row meet 8 banks
-        const auto put = [&](const uint4 (&raw)[NI], uint8_t *dst) {
+        const auto convert = [&](const uint8_t *raw, uint8_t *dst) {
 #pragma unroll
             for (uint32_t i = 0; i < NI; ++i) {
                 const uint32_t row = i * RP + row0;
-                uint4 a, b;
-                codes_to_half4(raw[i].x, a.x, a.y);
-                codes_to_half4(raw[i].y, a.z, a.w);
-                codes_to_half4(raw[i].z, b.x, b.y);
-                codes_to_half4(raw[i].w, b.z, b.w);
+                uint4 w4 = make_uint4(0, 0, 0, 0), a, b;
+                if (there) w4 = *reinterpret_cast<const uint4 *>(raw + row * D + chunk * 16u);
+                codes_to_half4(w4.x, a.x, a.y);
+                codes_to_half4(w4.y, a.z, a.w);
+                codes_to_half4(w4.z, b.x, b.y);
+                codes_to_half4(w4.w, b.z, b.w);
                 uint8_t *at = dst + (chunk / 4u) * (KT * 128u) + row * 128u;
                 const uint32_t piece = (chunk & 3u) * 2u, odd = chunk / 4u;
                 *reinterpret_cast<uint4 *>(at + (((piece + odd) ^ (row & 7u)) * 16u)) = odd ? b : a;
@@ -569,69 +596,157 @@ __global__ void __launch_bounds__(kManyThreads, 2)
             }
             fence_proxy_async_smem();
         };
-        uint32_t it = 0;
-        bool ok = true, more = true;
-        fetch(w, w.tile, p.c.K, raw_k);
-        fetch(w, w.tile, p.c.V, raw_v);
-        while (more && ok) {
-            const Walk cur = w;
-            for (int32_t j = 0; j < cur.count; ++j, ++it) {
-                const bool last = j + 1 == cur.count;
-                if (last) more = w.next();
-                const int32_t tile = last ? w.tile : cur.tile + j + 1;   // the tile to fetch next
-                if (it && !(ok = wait(&bar_k_free, it - 1))) break;
-                put(raw_k, sk);
-                mbar_arrive(&bar_k);
-                if (!last || more) fetch(w, tile, p.c.K, raw_k);
-                if (it && !(ok = wait(&bar_v_free, it - 1))) break;
-                put(raw_v, sv);
-                mbar_arrive(&bar_v);
-                if (!last || more) fetch(w, tile, p.c.V, raw_v);
-            }
+        for (uint32_t it = 0; it < w.left; ++it) {
+            const uint32_t st = it & 1u, round = it >> 1;
+            if (!wait_warp(&bar_rk[st], round) || (it && !wait_warp(&bar_k_free, it - 1))) break;
+            convert(raw_k + st * Shape::kRawBytes, sk);
+            mbar_arrive(&bar_k);
+            mbar_arrive(&bar_rk_free[st]);
+            if (!wait_warp(&bar_rv[st], round) || (round && !wait_warp(&bar_v_free[st], round - 1))) break;
+            convert(raw_v + st * Shape::kRawBytes, sv + st * Shape::kKvBytes);
+            mbar_arrive(&bar_v[st]);
+            mbar_arrive(&bar_rv_free[st]);
         }
-    } else if (busy && lane == 0) {
+    } else if (busy && warp == 12) {
         // =============================== tensor products ===============================
-        constexpr uint32_t idesc_s = umma_idesc_f16(kRows, KT, false);
-        constexpr uint32_t idesc_o = umma_idesc_f16(kRows, DP, true);
-        const uint32_t aq = smem_addr(sq), ak = smem_addr(sk), av = smem_addr(sv);
-        uint32_t it = 0, seg = 0;
-        bool ok = true, more = true;
-        while (more && ok) {
-            if (!(ok = wait(&bar_q, seg++))) break;
-            for (int32_t j = 0; j < w.count; ++j, ++it) {
-                if (!(ok = wait(&bar_k, it))) break;
-                tc_fence_after();
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = umma_idesc_f16(kHalf, KT, false);
+            constexpr uint32_t idesc_o = umma_idesc_f16(kHalf, DP, true);
+            const uint32_t aq = smem_addr(sq), ak = smem_addr(sk), av = smem_addr(sv);
+            const auto scores = [&](uint32_t half) {
 #pragma unroll
-                for (uint32_t half = 0; half < (kSplit ? 2u : 1u); ++half)
+                for (uint32_t x = 0; x < (kSplit ? 2u : 1u); ++x)
 #pragma unroll
                     for (uint32_t k = 0; k < DP / 16; ++k) {
-                        const uint32_t q_off = half * (kRows * DP * 2) + (k / 4) * (kRows * 128) + (k % 4) * 32;
+                        const uint32_t q_off = half * Shape::kQHalf + x * (kHalf * DP * 2) + (k / 4) * (kHalf * 128) + (k % 4) * 32;
                         const uint32_t k_off = (k / 4) * (KT * 128) + (k % 4) * 32;
-                        umma_f16_ss(tmem, umma_desc_k_sw128(aq + q_off), umma_desc_k_sw128(ak + k_off), idesc_s,
-                                    half | k);
+                        umma_f16_ss(tmem + half * Shape::kHalfCols, umma_desc_k_sw128(aq + q_off),
+                                    umma_desc_k_sw128(ak + k_off), idesc_s, x | k);
                     }
-                umma_commit(&bar_k_free);
-                umma_commit(&bar_s);
-                if (!(ok = wait(&bar_p, it)) || !(ok = wait(&bar_v, it))) break;
-                tc_fence_after();
+                umma_commit(&bar_s[half]);
+            };
+            const auto values = [&](uint32_t half, uint32_t st, bool add) {
+                const uint32_t d = tmem + half * Shape::kHalfCols;
 #pragma unroll
-                for (uint32_t half = 0; half < (kSplit ? 2u : 1u); ++half)
+                for (uint32_t x = 0; x < (kSplit ? 2u : 1u); ++x)
 #pragma unroll
                     for (uint32_t k = 0; k < KT / 16; ++k)
-                        umma_f16_ts(tmem + Shape::kOCol, tmem + Shape::kPCol + 32 * half + 8 * k,
-                                    umma_desc_mn_sw128(av + k * 2048, KT * 128), idesc_o,
-                                    (j != 0) | half | k);
-                umma_commit(&bar_v_free);
-                if (j + 1 == w.count) umma_commit(&bar_o);
+                        umma_f16_ts(d + Shape::kOCol, d + Shape::kPCol + 32 * x + 8 * k,
+                                    umma_desc_mn_sw128(av + st * Shape::kKvBytes + k * 2048, KT * 128), idesc_o,
+                                    (add ? 1u : 0u) | x | k);
+            };
+            uint32_t it = 0, done[2] = {0, 0}, seg[2] = {0, 0};
+            bool ok = true, more = true;
+            while (more && ok) {
+                const uint32_t count = static_cast<uint32_t>(w.count);
+                const bool two = static_cast<uint32_t>(w.s.n) * p.group > w.x.rb * kRows + kHalf;
+                more = w.next();
+                if (!(ok = wait(&bar_q[0], seg[0]++) && wait(&bar_k, it))) break;
+                tc_fence_after();
+                scores(0);
+                if (two) {
+                    if (!(ok = wait(&bar_q[1], seg[1]++))) break;
+                    tc_fence_after();
+                    scores(1);
+                }
+                umma_commit(&bar_k_free);
+                for (uint32_t j = 0; j < count && ok; ++j, ++it) {
+                    const uint32_t st = it & 1u;
+                    const bool last = j + 1 == count;
+                    if (!(ok = wait(&bar_v[st], it >> 1) && wait(&bar_p[0], done[0]++))) break;
+                    tc_fence_after();
+                    values(0, st, j != 0);
+                    if (last) {
+                        umma_commit(&bar_o[0]);
+                    } else {
+                        if (!(ok = wait(&bar_k, it + 1))) break;
+                        tc_fence_after();
+                        scores(0);
+                    }
+                    if (two) {
+                        if (!(ok = wait(&bar_p[1], done[1]++))) break;
+                        tc_fence_after();
+                        values(1, st, j != 0);
+                    }
+                    umma_commit(&bar_v_free[st]);
+                    if (last) {
+                        if (two) umma_commit(&bar_o[1]);
+                    } else {
+                        if (two) scores(1);
+                        umma_commit(&bar_k_free);
+                    }
+                }
             }
-            if (ok) more = w.next();
         }
+    } else if (busy && warp == 13) {
+        // =============================== copies ===============================
+        uint32_t it = 0;
+        bool ok = true, more = true;
+        while (more && ok) {
+            const Walk cur = w;
+            more = w.next();
+            for (int32_t j = 0; j < cur.count; ++j, ++it) {
+                const uint32_t st = it & 1u, round = it >> 1, ring = it % kScaleRing;
+                // lane g: group g of 16 keys.  One that is not there stays as it is in shared
+                // memory (whole numbers all the same); its keys are masked or count as zeros.
+                const int32_t key = (cur.tile + j) * static_cast<int32_t>(KT) + static_cast<int32_t>(lane * 16u);
+                const bool wanted = lane < kGroups && key < cur.s.len;
+                int32_t page = -1;
+                if (wanted) {
+                    page = __ldg(p.pb.table + static_cast<uint64_t>(cur.x.b) * p.pb.table_stride +
+                                 (static_cast<uint32_t>(key) >> p.c.page_shift));
+                    if (page < 0 || static_cast<uint32_t>(page) >= p.c.num_pages) {
+                        record_error(p.err, kErrBadIndex);
+                        page = -1;
+                    }
+                }
+                const uint64_t at = page >= 0 ? static_cast<uint64_t>(page) * p.c.heads + cur.h : 0;
+                float ks = 0.0f, vs = 0.0f;
+                if (page >= 0) {
+                    ks = __ldg(p.c.K_scale + at);
+                    vs = __ldg(p.c.V_scale + at);
+                }
+                // Tile it - 2 of K is converted, so the scores of tile it - 3 are there, and so the
+                // weights of tile it - 4: its place in the ring of scales is free, too.
+                if (round && !(ok = wait_warp(&bar_rk_free[st], round - 1))) break;
+                if (lane < kGroups) {
+                    const float lv = vs > 0.0f ? __log2f(vs) : 0.0f;   // a page of zeros has the scale 0
+                    sh_k[ring][lane] = ks;
+                    sh_lv[ring][lane] = lv;
+                    sh_iv[ring][lane] = vs > 0.0f ? ex2(-lv) : 1.0f;
+                }
+                const uint32_t zeros = __ballot_sync(0xffffffffu, lane < kGroups && !(vs > 0.0f));
+                const uint32_t bytes = 16u * D * __popc(__ballot_sync(0xffffffffu, page >= 0));
+                if (lane == 0) sh_zeros[ring] = zeros;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_sc[ring]);
+                const uint64_t src = ((at << p.c.page_shift) + (static_cast<uint32_t>(key) & ((1u << p.c.page_shift) - 1u))) * D;
+                if (lane == 0) mbar_arrive_expect_tx(&bar_rk[st], bytes);
+                __syncwarp();
+                if (page >= 0)
+                    bulk_load_1d(raw_k + st * Shape::kRawBytes + lane * 16u * D, p.c.K + src, 16u * D, &bar_rk[st]);
+                if (round && !(ok = wait_warp(&bar_rv_free[st], round - 1))) break;
+                if (lane == 0) mbar_arrive_expect_tx(&bar_rv[st], bytes);
+                __syncwarp();
+                if (page >= 0)
+                    bulk_load_1d(raw_v + st * Shape::kRawBytes + lane * 16u * D, p.c.V + src, 16u * D, &bar_rv[st]);
+            }
+        }
+        // a run that was given up may leave copies in flight: they end before the block does
+        if (!ok)
+            for (uint32_t i = 0; i < 2; ++i) {
+                const uint32_t n = (it + 1 - i) / 2;   // tiles of this slot that were begun
+                if (n) {
+                    mbar_wait(&bar_rk[i], (n - 1) & 1u, p.limit_ns, nullptr, nullptr);
+                    mbar_wait(&bar_rv[i], (n - 1) & 1u, p.limit_ns, nullptr, nullptr);
+                }
+            }
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 12) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, Shape::kCols);
+        tmem_dealloc(tmem, 2 * Shape::kHalfCols);
     }
 }
 
@@ -702,7 +817,7 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem));
         ready_device = device;
     }
-    const uint32_t grid = static_cast<uint32_t>(ctx.num_sms) * 2;
+    const uint32_t grid = static_cast<uint32_t>(ctx.num_sms);
     const uint64_t blocks = static_cast<uint64_t>(a.batch.tokens) * p.group / kRows + a.batch.batch;
     const auto pad = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
     const size_t o_bytes = pad(2ull * grid * kRows * DP * sizeof(float));
@@ -733,7 +848,7 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     if (e == cudaSuccess)
         e = launch_pdl(ctx.stream, &paged_prefill_kernel<T, DP>, dim3(grid), dim3(kManyThreads), Shape::kSmem, p, plan);
     if (e == cudaSuccess)
-        e = launch_pdl(ctx.stream, &paged_prefill_join_kernel<T, DP>, dim3(grid, 4), dim3(256), 0, p);
+        e = launch_pdl(ctx.stream, &paged_prefill_join_kernel<T, DP>, dim3(grid, 8), dim3(256), 0, p);
     const cudaError_t f = cudaFreeAsync(ws, ctx.stream);
     return e == cudaSuccess ? f : e;
 }

@@ -185,6 +185,19 @@ def test_attention_ragged_rows_of_many(gpu, torch, dtype, d):
     check_attention(o, *attention64(s, q64, 4, True, 0), dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("spans", [[(40, 60000)], [(300, 20000), (5, 9000), (1, 30000)]])
+def test_attention_long_runs_of_key_tiles(gpu, torch, dtype, spans):
+    """Tens of thousands of keys under a few hundred rows: every CTA walks many tiles of one
+    block, and blocks are joined from many CTAs."""
+    s = Setup(torch, spans, 1, 128, 64)
+    q, q64 = rows(torch, np.random.default_rng(6), s.tokens, 2 * 128, dtype)
+    o = torch.full((s.tokens, 2, 128), float("nan"), dtype=q.dtype, device="cuda")
+    torch.cuda.synchronize()
+    gpu.paged_attention(s.cache, s.batch, q.view(s.tokens, 2, 128), o)
+    check_attention(o, *attention64(s, q64, 2, True, 0), dtype)
+
+
 @pytest.mark.parametrize("dtype,extra", [("f32", 3), ("f32", 4), ("bf16", 1), ("f16", 8), ("f16", 4)])
 def test_attention_strided_rows_and_in_place(gpu, torch, dtype, extra):
     """Rows with gaps of odd and even sizes, unaligned bases, and the output over the queries."""
