@@ -13,8 +13,6 @@
 //           memory, the weights go back over it as f16 (the second product takes
 //           its A operand from there), and O is rescaled there when a row's
 //           maximum grew.  One half's softmax runs under the other's products.
-// The weights of a tile are first computed with the maximum so far; only when
-// some row exceeds it by 2^6 are they computed again, so a tile is read once.
 //
 // f32 rows: Q = hi + lo in f16 (22 bits), P likewise; each product is two
 // tensor instructions on the same accumulator, with tiles of 64 keys so that S
@@ -183,12 +181,11 @@ __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-
 template <RowType T, uint32_t DP>
 struct ManyShape {
     static constexpr bool kSplit = T == RowType::kF32;
@@ -204,32 +201,30 @@ struct ManyShape {
 
 // Where a CTA stands in the units: head, block, tile; the roles walk alike.
 struct Walk {
-    const AttnParams *p;
-    const Plan *plan;
     uint32_t left, h, e, blocks;    // tiles left; current head and block
     int32_t tile, count;            // first tile and tiles of this segment
     RowBlock x;
     PagedSeq s;
 
     // Takes the segment that begins `off` tiles into block e.
-    __device__ __forceinline__ void take(uint32_t off) {
-        const int4 v = __ldcg(reinterpret_cast<const int4 *>(plan->blocks) + e);
+    __device__ __forceinline__ void take(const AttnParams &p, const Plan &plan, uint32_t off) {
+        const int4 v = __ldcg(reinterpret_cast<const int4 *>(plan.blocks) + e);
         x.b = static_cast<uint32_t>(v.x);
         x.rb = static_cast<uint32_t>(v.y);
         x.lo = v.z;
         x.nt = v.w;
         tile = x.lo + static_cast<int32_t>(off);
         count = min(x.nt - static_cast<int32_t>(off), static_cast<int32_t>(left));
-        load_seq(p->pb, p->c.page_shift, x.b, s);
+        load_seq(p.pb, p.c.page_shift, x.b, s);
     }
-    __device__ __forceinline__ bool next() {
+    __device__ __forceinline__ bool next(const AttnParams &p, const Plan &plan) {
         left -= static_cast<uint32_t>(count);
         if (!left) return false;
         if (++e == blocks) {
             e = 0;
             ++h;
         }
-        take(0);
+        take(p, plan, 0);
         return true;
     }
 };
@@ -298,8 +293,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
     // ---- this CTA's run
     Walk w;
-    w.p = &p;
-    w.plan = &plan;
     w.blocks = __ldcg(plan.head);
     const uint32_t per_head = __ldcg(plan.head + 1);
     const uint64_t total = static_cast<uint64_t>(per_head) * p.c.heads;
@@ -319,7 +312,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             hi = min(hi, lo + step);
         }
         w.e = lo;
-        w.take(off - __ldcg(plan.before + lo));
+        w.take(p, plan, off - __ldcg(plan.before + lo));
     }
 
     // The block's 65536 registers go where they are needed: 256 x 168 + 256 x 88.  (The spare
@@ -336,46 +329,56 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         uint64_t *const full_s = &bar_s[half], *const full_p = &bar_p[half];
         float f_next = 0.0f;
         // Query rows to shared memory as f16, scaled by a power of two.  DP / 8 lanes take a
-        // row, so a warp reads whole rows, 64 registers of them in flight.
+        // row, so a warp reads whole rows, 4 steps in work and 4 in flight.
         const auto load_q = [&](const Walk &k) {
-            constexpr uint32_t LR = DP / 8, RI = 32 / LR;            // lanes a row, rows a step
-            constexpr uint32_t NS = kSplit ? (LR < 8 ? LR : 8) : LR; // steps in flight
+            constexpr uint32_t LR = DP / 8, RI = 32 / LR, NS = 4;    // lanes a row, rows a step, steps at once
             const uint32_t d = (lane % LR) * 8, rows = static_cast<uint32_t>(k.s.n) * p.group;
             const bool vec = p.vec & 1u;
             int ex_mine = 0;
             const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-#pragma unroll 1
-            for (uint32_t i0 = 0; i0 < LR; i0 += NS) {
-                alignas(16) E x[NS][8];
+            constexpr uint32_t NW = sizeof(E) / 2;
+            uint4 next[NS][NW];
+            const auto read = [&](uint32_t i0) {
 #pragma unroll
                 for (uint32_t i = 0; i < NS; ++i) {
                     const uint32_t r = k.x.rb * kRows + (row & ~31u) + (i0 + i) * RI + lane / LR;
                     const uint32_t token = r / p.group;
-                    uint4 *v = reinterpret_cast<uint4 *>(x[i]);
 #pragma unroll
-                    for (uint32_t e = 0; e < sizeof(E) / 2; ++e) v[e] = make_uint4(0, 0, 0, 0);
-                    if (r < rows && d < D) {
-                        const E *src = static_cast<const E *>(p.Q) +
-                                       static_cast<uint64_t>(k.s.row0 + static_cast<int32_t>(token)) * p.ldq +
-                                       (k.h * p.group + (r - token * p.group)) * D + d;
-                        if (vec) {
+                    for (uint32_t e = 0; e < NW; ++e) next[i][e] = make_uint4(0, 0, 0, 0);
+                    if (r >= rows || d >= D) continue;
+                    const E *src = static_cast<const E *>(p.Q) +
+                                   static_cast<uint64_t>(k.s.row0 + static_cast<int32_t>(token)) * p.ldq +
+                                   (k.h * p.group + (r - token * p.group)) * D + d;
+                    if (vec) {
 #pragma unroll
-                            for (uint32_t e = 0; e < sizeof(E) / 2; ++e)
-                                v[e] = __ldg(reinterpret_cast<const uint4 *>(src) + e);
-                        } else {
+                        for (uint32_t e = 0; e < NW; ++e) next[i][e] = __ldg(reinterpret_cast<const uint4 *>(src) + e);
+                    } else {
+                        alignas(16) E x[8];
 #pragma unroll
-                            for (uint32_t e = 0; e < 8; ++e) x[i][e] = src[e];
-                        }
+                        for (uint32_t e = 0; e < 8; ++e) x[e] = src[e];
+#pragma unroll
+                        for (uint32_t e = 0; e < NW; ++e) next[i][e] = reinterpret_cast<const uint4 *>(x)[e];
                     }
                 }
+            };
+            read(0);
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < LR; i0 += NS) {
+                float y[NS][8];
 #pragma unroll
                 for (uint32_t i = 0; i < NS; ++i) {
-                    float y[8], most = 0.0f;
+                    alignas(16) E x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        y[e] = to_f32(x[i][e]);
-                        most = fmaxf(most, fabsf(y[e]));
-                    }
+                    for (uint32_t e = 0; e < NW; ++e) reinterpret_cast<uint4 *>(x)[e] = next[i][e];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[i][e] = to_f32(x[e]);
+                }
+                if (i0 + NS < LR) read(i0 + NS);
+#pragma unroll
+                for (uint32_t i = 0; i < NS; ++i) {
+                    float most = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(y[i][e]));
 #pragma unroll
                     for (uint32_t o = 1; o < LR; o <<= 1)
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     uint32_t *h = reinterpret_cast<uint32_t *>(&hi), *l = reinterpret_cast<uint32_t *>(&lo);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float a = y[2 * e] * up, b = y[2 * e + 1] * up;
+                        const float a = y[i][2 * e] * up, b = y[i][2 * e + 1] * up;
                         h[e] = pack_half2(a, b);
                         if constexpr (kSplit) {
                             const float2 g = unpack_half2(h[e]);
@@ -410,34 +413,74 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             return half == 0 || static_cast<uint32_t>(k.s.n) * p.group > k.x.rb * kRows + kHalf;
         };
         uint32_t tile_no = 0, done = 0, seg = 0;  // tiles of the run; tiles and segments of this half
-        bool more = true;
-        if (takes(w)) load_q(w);
-        while (more) {
+        float m = 0.0f, l = 0.0f;
+        bool more = true, ok = true, write = false;
+        Walk cur = w;                             // the segment in work, whose output comes last
+        for (;;) {
+            // The scores of the segment before are all computed: these queries may take the place
+            // of its own, and their first scores be computed while its output is written.
+            if (more && takes(w)) load_q(w);
             const float f = f_next;
-            const Walk cur = w;
-            more = w.next();
-            const bool started = cur.tile == cur.x.lo;
-            const bool whole = started && cur.count == cur.x.nt;
-            const uint32_t rows = static_cast<uint32_t>(cur.s.n) * p.group;
+            if (write) {
+                if (!wait_warp(&bar_o[half], seg++)) break;
+                tc_fence_after();
+                const bool started = cur.tile == cur.x.lo, whole = started && cur.count == cur.x.nt;
+                const uint32_t r = cur.x.rb * kRows + row, token = r / p.group;
+                const bool live = r < static_cast<uint32_t>(cur.s.n) * p.group;
+                const uint32_t part = 2 * cta + (started ? 1 : 0);
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                E *out = static_cast<E *>(p.O) +
+                         static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldo +
+                         (cur.h * p.group + (r - token * p.group)) * D;
+                float *po = p.ws_o + (static_cast<uint64_t>(part) * kRows + row) * DP;
+#pragma unroll
+                for (uint32_t c = 0; c < DP / 32; ++c) {
+                    uint32_t v[32];
+                    __syncwarp();
+                    tmem_ld_32cols(lanes + Shape::kOCol + 32 * c, v);
+                    tmem_wait_ld();
+                    if (!live) continue;
+                    if (whole) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; i += 8)
+                            if (32 * c + i < D) {
+                                float x[8];
+#pragma unroll
+                                for (uint32_t k = 0; k < 8; ++k) x[k] = __uint_as_float(v[i + k]) * inv;
+                                store8(out + 32 * c + i, p.vec & 4u, x);
+                            }
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4 *>(po + 32 * c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    }
+                }
+                if (live && !whole) p.ws_ml[part * kRows + row] = make_float2(m, l);
+                tc_fence_before();
+            }
+            if (!more) break;
+            cur = w;
+            more = w.next(p, plan);
             if (tid == 0 && !more) {
                 // joined with the CTAs that go on with the block, when it begins here
-                const uint32_t parts = started && !whole
+                const uint32_t parts = cur.tile == cur.x.lo && cur.count != cur.x.nt
                                            ? 1 + static_cast<uint32_t>((cur.x.nt - cur.count + run - 1) / run)
                                            : 0;
                 p.ws_meta[2 * cta] = make_uint4(parts, static_cast<uint32_t>(cur.s.row0), cur.x.rb * kRows, cur.h);
-                p.ws_meta[2 * cta + 1] = make_uint4(min(kRows, rows - cur.x.rb * kRows), 0, 0, 0);
+                p.ws_meta[2 * cta + 1] = make_uint4(
+                    min(kRows, static_cast<uint32_t>(cur.s.n) * p.group - cur.x.rb * kRows), 0, 0, 0);
             }
-            if (!takes(cur)) {
+            write = takes(cur);
+            if (!write) {
                 tile_no += static_cast<uint32_t>(cur.count);
-                if (more && takes(w)) load_q(w);
                 continue;
             }
             int32_t kmin, kmax, kmin_last, kmax_first, unused;
             row_limits(p, cur.s, cur.x.rb * kRows + row, kmin, kmax);
             row_limits(p, cur.s, cur.x.rb * kRows + half * kHalf, unused, kmax_first);
             row_limits(p, cur.s, cur.x.rb * kRows + half * kHalf + kHalf - 1, kmin_last, unused);
-            float m = -INFINITY, l = 0.0f;
-            bool ok = true;
+            m = -INFINITY;
+            l = 0.0f;
             for (int32_t j = 0; j < cur.count; ++j, ++tile_no, ++done) {
                 const int32_t k0 = (cur.tile + j) * static_cast<int32_t>(KT);
                 const uint32_t ring = tile_no % kScaleRing;
@@ -445,59 +488,41 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 if (!(ok = wait_warp(&bar_sc[ring], tile_no / kScaleRing) && wait_warp(full_s, done))) break;
                 tc_fence_after();
                 const uint32_t zeros = sh_zeros[ring];
-                uint32_t h[KT / 2], lo[kSplit ? KT / 2 : 1];
-                float sum;
-#pragma unroll 1
-                for (;;) {
-                    const float off = m == -INFINITY ? 0.0f : m - kLift;
-                    float top = -INFINITY;
-                    sum = 0.0f;
+                // Loops over 64 keys are not unrolled: the code of all roles has to stay in the
+                // instruction caches (unrolled, a fifth of the stalls were for instructions).
+                const auto read = [&](uint32_t c, uint32_t (&x)[64]) {
+                    tmem_ld_32cols(lanes + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(x));
+                    tmem_ld_32cols(lanes + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+                    tmem_wait_ld();
+                    if (edge) {   // bits of the keys that the row sees
+                        const int64_t lo = max(0, min(64, kmin - k0 - static_cast<int32_t>(64 * c)));
+                        const int64_t hi = max(0, min(64, kmax + 1 - k0 - static_cast<int32_t>(64 * c)));
+                        const uint64_t seen = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
 #pragma unroll
-                    for (uint32_t c = 0; c < KT / 32; ++c) {
-                        uint32_t r[32];
-                        tmem_ld_32cols(lanes + 32 * c, r);
-                        tmem_wait_ld();
-                        if (edge) {
-#pragma unroll
-                            for (uint32_t i = 0; i < 32; ++i) {
-                                const int32_t key = k0 + static_cast<int32_t>(32 * c + i);
-                                if (key > kmax || key < kmin) r[i] = 0xff800000u;  // -infinity
-                            }
-                        }
-#pragma unroll
-                        for (uint32_t g = 0; g < 2; ++g) {
-                            const uint32_t gg = 2 * c + g;
-                            // a factor of zero would make masked scores NaN
-                            const float fg = fmaxf(f * sh_k[ring][gg], 1e-38f);
-                            const float b = sh_lv[ring][gg] - off;
-                            float x[4];
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i)
-                                x[i] = fmaxf(fmaxf(__uint_as_float(r[16 * g + i]), __uint_as_float(r[16 * g + 4 + i])),
-                                             fmaxf(__uint_as_float(r[16 * g + 8 + i]), __uint_as_float(r[16 * g + 12 + i])));
-                            // scales are not negative: the largest product is the largest score
-                            top = fmaxf(top, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fg, b));
-                            const uint64_t f2 = pack_f32x2(fg, fg), b2 = pack_f32x2(b, b);
-                            uint64_t s2 = 0;
-#pragma unroll
-                            for (uint32_t i = 0; i < 8; ++i) {
-                                const uint64_t t = fma_f32x2(
-                                    pack_f32x2(__uint_as_float(r[16 * g + 2 * i]), __uint_as_float(r[16 * g + 2 * i + 1])),
-                                    f2, b2);
-                                const float u = ex2(half_f32x2(t, 0)), v = ex2(half_f32x2(t, 1));
-                                s2 = add_f32x2(s2, pack_f32x2(u, v));
-                                h[8 * gg + i] = pack_half2(u, v);
-                                if constexpr (kSplit) {
-                                    const float2 y = unpack_half2(h[8 * gg + i]);
-                                    lo[8 * gg + i] = pack_half2(u - y.x, v - y.y);
-                                }
-                            }
-                            sum = fmaf(half_f32x2(s2, 0) + half_f32x2(s2, 1), sh_iv[ring][gg], sum);
-                        }
+                        for (uint32_t i = 0; i < 64; ++i)
+                            if (!(seen >> i & 1u)) x[i] = 0xff800000u;  // -infinity
                     }
-                    top += off;
-                    if (!__any_sync(0xffffffffu, top > m + kSlack)) break;
-                    // some row's maximum grew by more than the slack: rescale, and again
+                };
+                // a factor of zero would make masked scores NaN
+                const auto factor = [&](uint32_t g) { return fmaxf(f * sh_k[ring][g], 1e-38f); };
+                float top = -INFINITY;
+#pragma unroll 1
+                for (uint32_t c = 0; c < KT / 64; ++c) {
+                    uint32_t x[64];
+                    read(c, x);
+#pragma unroll
+                    for (uint32_t g = 0; g < 4; ++g) {
+                        const auto score = [&](uint32_t i) { return __uint_as_float(x[16 * g + i]); };
+                        const float y0 = max3(score(0), score(1), score(2)), y1 = max3(score(3), score(4), score(5));
+                        const float y2 = max3(score(6), score(7), score(8)), y3 = max3(score(9), score(10), score(11));
+                        const float y4 = max3(score(12), score(13), score(14));
+                        // scales are not negative: the largest product is the largest score
+                        top = fmaxf(top, fmaf(fmaxf(max3(y0, y1, y2), max3(y3, y4, score(15))),
+                                              factor(4 * c + g), sh_lv[ring][4 * c + g]));
+                    }
+                }
+                if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                    // some row's maximum grew by more than the slack
                     const float to = fmaxf(m, top);
                     const float a = to > m ? ex2(m - to) : 1.0f;
                     l *= a;
@@ -515,62 +540,46 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         }
                     }
                 }
-                l += sum;
-                if (zeros) {   // pages of zeros count in the sum alone
-#pragma unroll
-                    for (uint32_t i = 0; i < KT / 2; ++i)
-                        if (zeros >> (i / 8) & 1u) {
-                            h[i] = 0;
-                            if constexpr (kSplit) lo[i] = 0;
-                        }
-                }
-#pragma unroll
+                const float off = m == -INFINITY ? 0.0f : m - kLift;
+#pragma unroll 1
                 for (uint32_t c = 0; c < KT / 64; ++c) {
-                    tmem_st_32cols(lanes + Shape::kPCol + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(h + 32 * c));
-                    if constexpr (kSplit)
-                        tmem_st_32cols(lanes + Shape::kPCol + 32, *reinterpret_cast<uint32_t(*)[32]>(lo));
+                    uint32_t x[64], h[32], lo[kSplit ? 32 : 1];
+                    read(c, x);
+#pragma unroll
+                    for (uint32_t g = 0; g < 4; ++g) {
+                        const float fg = factor(4 * c + g), b = sh_lv[ring][4 * c + g] - off;
+                        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; ++i) {
+                            const float u = ex2(fmaf(__uint_as_float(x[16 * g + 2 * i]), fg, b));
+                            const float v = ex2(fmaf(__uint_as_float(x[16 * g + 2 * i + 1]), fg, b));
+                            s0 += u;
+                            s1 += v;
+                            h[8 * g + i] = pack_half2(u, v);
+                            if constexpr (kSplit) {
+                                const float2 y = unpack_half2(h[8 * g + i]);
+                                lo[8 * g + i] = pack_half2(u - y.x, v - y.y);
+                            }
+                        }
+                        l = fmaf(s0 + s1, sh_iv[ring][4 * c + g], l);
+                    }
+                    const uint32_t zero4 = zeros >> (4 * c) & 15u;
+                    if (zero4) {   // pages of zeros count in the sum alone
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i)
+                            if (zero4 >> (i / 8) & 1u) {
+                                h[i] = 0;
+                                if constexpr (kSplit) lo[i] = 0;
+                            }
+                    }
+                    tmem_st_32cols(lanes + Shape::kPCol + 32 * c, h);
+                    if constexpr (kSplit) tmem_st_32cols(lanes + Shape::kPCol + 32, lo);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(full_p);
             }
             if (!ok) break;
-            // All scores of this block are computed: the next block's queries may take its place.
-            if (more && takes(w)) load_q(w);
-            if (!wait_warp(&bar_o[half], seg++)) break;
-            tc_fence_after();
-            const uint32_t r = cur.x.rb * kRows + row, token = r / p.group;
-            const bool live = r < rows;
-            const uint32_t part = 2 * cta + (started ? 1 : 0);
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            E *out = static_cast<E *>(p.O) +
-                     static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldo +
-                     (cur.h * p.group + (r - token * p.group)) * D;
-            float *po = p.ws_o + (static_cast<uint64_t>(part) * kRows + row) * DP;
-#pragma unroll
-            for (uint32_t c = 0; c < DP / 32; ++c) {
-                uint32_t v[32];
-                __syncwarp();
-                tmem_ld_32cols(lanes + Shape::kOCol + 32 * c, v);
-                tmem_wait_ld();
-                if (!live) continue;
-                if (whole) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 32; i += 8)
-                        if (32 * c + i < D) {
-                            float x[8];
-#pragma unroll
-                            for (uint32_t k = 0; k < 8; ++k) x[k] = __uint_as_float(v[i + k]) * inv;
-                            store8(out + 32 * c + i, p.vec & 4u, x);
-                        }
-                } else {
-#pragma unroll
-                    for (uint32_t i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4 *>(po + 32 * c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                }
-            }
-            if (live && !whole) p.ws_ml[part * kRows + row] = make_float2(m, l);
-            tc_fence_before();
         }
     } else if (busy && warp < 12) {
         // =============================== conversion ===============================
@@ -580,7 +589,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         // 16 codes to two 16-byte pieces of a 128-byte swizzled row; the columns' upper half
         // writes its pieces in the other order, so that 8 lanes of a row meet 8 banks
         const auto convert = [&](const uint8_t *raw, uint8_t *dst) {
-#pragma unroll
+#pragma unroll 4
             for (uint32_t i = 0; i < NI; ++i) {
                 const uint32_t row = i * RP + row0;
                 uint4 w4 = make_uint4(0, 0, 0, 0), a, b;
@@ -596,16 +605,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
             fence_proxy_async_smem();
         };
-        for (uint32_t it = 0; it < w.left; ++it) {
-            const uint32_t st = it & 1u, round = it >> 1;
-            if (!wait_warp(&bar_rk[st], round) || (it && !wait_warp(&bar_k_free, it - 1))) break;
-            convert(raw_k + st * Shape::kRawBytes, sk);
-            mbar_arrive(&bar_k);
-            mbar_arrive(&bar_rk_free[st]);
-            if (!wait_warp(&bar_rv[st], round) || (round && !wait_warp(&bar_v_free[st], round - 1))) break;
-            convert(raw_v + st * Shape::kRawBytes, sv + st * Shape::kKvBytes);
-            mbar_arrive(&bar_v[st]);
-            mbar_arrive(&bar_rv_free[st]);
+        // K of the run's tile, then V, and so on
+#pragma unroll 1
+        for (uint32_t x = 0; x < 2 * w.left; ++x) {
+            const uint32_t it = x >> 1, st = it & 1u, round = it >> 1;
+            const bool v = x & 1u;
+            if (!wait_warp(v ? &bar_rv[st] : &bar_rk[st], round)) break;
+            if (v ? round != 0 && !wait_warp(&bar_v_free[st], round - 1) : it != 0 && !wait_warp(&bar_k_free, it - 1)) break;
+            convert((v ? raw_v : raw_k) + st * Shape::kRawBytes, v ? sv + st * Shape::kKvBytes : sk);
+            mbar_arrive(v ? &bar_v[st] : &bar_k);
+            mbar_arrive(v ? &bar_rv_free[st] : &bar_rk_free[st]);
         }
     } else if (busy && warp == 12) {
         // =============================== tensor products ===============================
@@ -638,42 +647,37 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             uint32_t it = 0, done[2] = {0, 0}, seg[2] = {0, 0};
             bool ok = true, more = true;
             while (more && ok) {
-                const uint32_t count = static_cast<uint32_t>(w.count);
-                const bool two = static_cast<uint32_t>(w.s.n) * p.group > w.x.rb * kRows + kHalf;
-                more = w.next();
-                if (!(ok = wait(&bar_q[0], seg[0]++) && wait(&bar_k, it))) break;
-                tc_fence_after();
-                scores(0);
-                if (two) {
-                    if (!(ok = wait(&bar_q[1], seg[1]++))) break;
-                    tc_fence_after();
-                    scores(1);
-                }
-                umma_commit(&bar_k_free);
-                for (uint32_t j = 0; j < count && ok; ++j, ++it) {
-                    const uint32_t st = it & 1u;
+                const int32_t count = w.count;
+                const uint32_t halves = static_cast<uint32_t>(w.s.n) * p.group > w.x.rb * kRows + kHalf ? 2 : 1;
+                more = w.next(p, plan);
+                // step -1 only computes the first tile's scores; a half's values of a tile and its
+                // scores of the next one follow each other, while the other half has its softmax
+#pragma unroll 1
+                for (int32_t j = -1; j < count && ok; ++j) {
                     const bool last = j + 1 == count;
-                    if (!(ok = wait(&bar_v[st], it >> 1) && wait(&bar_p[0], done[0]++))) break;
-                    tc_fence_after();
-                    values(0, st, j != 0);
-                    if (last) {
-                        umma_commit(&bar_o[0]);
-                    } else {
-                        if (!(ok = wait(&bar_k, it + 1))) break;
-                        tc_fence_after();
-                        scores(0);
+                    const uint32_t st = it & 1u;
+                    if (j >= 0 && !(ok = wait(&bar_v[st], it >> 1))) break;
+#pragma unroll 1
+                    for (uint32_t half = 0; half < halves; ++half) {
+                        if (j >= 0) {
+                            if (!(ok = wait(&bar_p[half], done[half]++))) break;
+                            tc_fence_after();
+                            values(half, st, j != 0);
+                        } else if (!(ok = wait(&bar_q[half], seg[half]++))) {
+                            break;
+                        }
+                        if (last) {
+                            umma_commit(&bar_o[half]);
+                        } else {
+                            if (half == 0 && !(ok = wait(&bar_k, j < 0 ? it : it + 1))) break;
+                            tc_fence_after();
+                            scores(half);
+                        }
                     }
-                    if (two) {
-                        if (!(ok = wait(&bar_p[1], done[1]++))) break;
-                        tc_fence_after();
-                        values(1, st, j != 0);
-                    }
-                    umma_commit(&bar_v_free[st]);
-                    if (last) {
-                        if (two) umma_commit(&bar_o[1]);
-                    } else {
-                        if (two) scores(1);
-                        umma_commit(&bar_k_free);
+                    if (!last) umma_commit(&bar_k_free);
+                    if (j >= 0) {
+                        umma_commit(&bar_v_free[st]);
+                        ++it;
                     }
                 }
             }
@@ -684,7 +688,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         bool ok = true, more = true;
         while (more && ok) {
             const Walk cur = w;
-            more = w.next();
+            more = w.next(p, plan);
             for (int32_t j = 0; j < cur.count; ++j, ++it) {
                 const uint32_t st = it & 1u, round = it >> 1, ring = it % kScaleRing;
                 // lane g: group g of 16 keys.  One that is not there stays as it is in shared
