@@ -4,11 +4,12 @@
 // The mathematics is paged_attention.cu's.  A CTA, one an SM, works on 256 query
 // rows of one key/value head (tokens x grouped heads, packed) and walks their
 // keys in tiles of KT.  Its warps:
-//   13      copies a tile's codes to shared memory (bulk copies of 16 keys, two
-//           tiles ahead) and its page scales beside them;
-//   8-11    turn the codes into f16 (exact), in the swizzled layout of the
-//           tensor core's operands;
-//   12      one thread issues S = Q K^T and O += P V for both halves of the rows;
+//   17      copies a tile's codes to shared memory (bulk copies, half a tile at a
+//           time) and its page scales beside them, ahead of their use;
+//   8-15    turn the codes into f16 (exact), in the swizzled layout of the
+//           tensor core's operands, four warps the first halves of the tiles
+//           and four the second;
+//   16      issues S = Q K^T and O += P V for both halves of the rows;
 //   0-3, 4-7  softmax of 128 rows each, one row a thread: S is read from tensor
 //           memory, the weights go back over it as f16 (the second product takes
 //           its A operand from there), and O is rescaled there when a row's
@@ -35,8 +36,9 @@ namespace {
 
 constexpr uint32_t kHalf = 128;              // rows of one accumulator (UMMA M)
 constexpr uint32_t kRows = 2 * kHalf;        // query rows of a block
-constexpr uint32_t kManyThreads = 512;       // 8 softmax, 4 converter, tensor-issue, copy and 2 spare warps
+constexpr uint32_t kManyThreads = 640;       // 8 softmax, 8 converter, tensor-issue, copy and 2 spare warps
 constexpr uint32_t kScaleRing = 4;           // tiles whose scales are kept
+constexpr uint32_t kRawRing = 4;             // half tiles of codes on their way or in conversion
 constexpr uint32_t kPlanThreads = 1024;
 
 // A block of rows and the key tiles that any of its rows sees.
@@ -138,21 +140,45 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const AttnPara
 }
 
 // ---- tensor core wrappers -------------------------------------------------------
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The whole warp runs the issuing code and one elected lane's instructions take
+// effect: descriptors then stay in uniform registers (issued from a branch of
+// one lane, an instruction of 64 clocks took 75 to 97 to issue).
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t is;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(is));
+    return is;
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
         : "memory");
 }
 // A from tensor memory: f16 pairs, 8 columns for 16 elements of K.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void umma_f16_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                            uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint32_t lead, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(lead)
         : "memory");
 }
 // f16 x f16 -> f32, A K-major; B K-major or, transposed, MN-major.
@@ -181,6 +207,32 @@ __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// mbar_wait that lets the warp sleep for up to 50 us at a time: the waiting
+// roles' polls would take issue slots from the working ones.
+__device__ __forceinline__ bool wait_asleep(uint64_t *bar, uint32_t parity, uint64_t limit_ns,
+                                            uint32_t *err, volatile int *abort) {
+    const uint32_t a = smem_addr(bar);
+    uint64_t start = 0;
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (*abort) return false;
+        const uint64_t now = global_timer_ns();
+        if (!start) start = now;
+        if (now - start > limit_ns) {
+            record_error(err, kErrWaitTimeout);
+            *abort = 1;
+            return false;
+        }
+    }
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -192,9 +244,9 @@ struct ManyShape {
     static constexpr uint32_t KT = kSplit ? 64 : 128;          // keys of a tile
     static constexpr uint32_t kQHalf = kHalf * DP * 2 * (kSplit ? 2 : 1);
     static constexpr uint32_t kKvBytes = KT * DP * 2;           // a tile of K or V in f16
-    static constexpr uint32_t kRawBytes = KT * DP;              // its codes
-    // queries, K, two of V, two tiles' codes of each
-    static constexpr uint32_t kSmem = 2 * kQHalf + 3 * kKvBytes + 4 * kRawBytes + 1024;
+    static constexpr uint32_t kRawBytes = KT * DP / 2;          // the codes of half of it
+    // queries, two tiles of K and of V, four half tiles of codes
+    static constexpr uint32_t kSmem = 2 * kQHalf + 4 * kKvBytes + kRawRing * kRawBytes + 1024;
     // tensor memory of a half: S (KT columns; P over it, or for f32 hi and lo after it), O
     static constexpr uint32_t kPCol = kSplit ? 64 : 0, kOCol = 128, kHalfCols = 256;
 };
@@ -238,11 +290,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     constexpr uint32_t KT = Shape::KT, kGroups = KT / 16;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *const sq = smem, *const sk = smem + 2 * Shape::kQHalf, *const sv = sk + Shape::kKvBytes;
-    uint8_t *const raw_k = sv + 2 * Shape::kKvBytes, *const raw_v = raw_k + 2 * Shape::kRawBytes;
+    uint8_t *const sq = smem, *const sk = smem + 2 * Shape::kQHalf, *const sv = sk + 2 * Shape::kKvBytes;
+    uint8_t *const raw = sv + 2 * Shape::kKvBytes;
     __shared__ uint64_t bar_q[2], bar_o[2], bar_s[2], bar_p[2];          // of a half
-    __shared__ uint64_t bar_k, bar_k_free, bar_v[2], bar_v_free[2];      // f16 tiles
-    __shared__ uint64_t bar_rk[2], bar_rk_free[2], bar_rv[2], bar_rv_free[2];  // codes
+    __shared__ uint64_t bar_k[2], bar_k_free[2], bar_v[2], bar_v_free[2];   // f16 tiles
+    __shared__ uint64_t bar_r[kRawRing], bar_r_free[kRawRing];              // codes
     __shared__ uint64_t bar_sc[kScaleRing];
     // a tile's 16-key groups: K scale, log2 of the V scale, 1 / V scale; pages of zeros as bits
     __shared__ __align__(16) float sh_k[kScaleRing][8], sh_lv[kScaleRing][8], sh_iv[kScaleRing][8];
@@ -256,24 +308,25 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         sh_abort = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(&bar_q[i], 128);
-            mbar_init(&bar_p[i], 128);
+            mbar_init(&bar_q[i], 4);
+            mbar_init(&bar_p[i], 4);
             mbar_init(&bar_s[i], 1);
             mbar_init(&bar_o[i], 1);
-            mbar_init(&bar_v[i], 128);
+            mbar_init(&bar_k[i], 8);
+            mbar_init(&bar_v[i], 8);
+            mbar_init(&bar_k_free[i], 1);
             mbar_init(&bar_v_free[i], 1);
-            mbar_init(&bar_rk[i], 1);
-            mbar_init(&bar_rv[i], 1);
-            mbar_init(&bar_rk_free[i], 128);
-            mbar_init(&bar_rv_free[i], 128);
         }
-        mbar_init(&bar_k, 128);
-        mbar_init(&bar_k_free, 1);
+#pragma unroll
+        for (uint32_t i = 0; i < kRawRing; ++i) {
+            mbar_init(&bar_r[i], 1);
+            mbar_init(&bar_r_free[i], 4);
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kScaleRing; ++i) mbar_init(&bar_sc[i], 1);
         fence_barrier_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         tmem_alloc(&sh_tmem, 2 * Shape::kHalfCols);
         tmem_relinquish();
     }
@@ -283,11 +336,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const uint32_t tmem = sh_tmem;
     pdl_enter();
     const auto wait = [&](uint64_t *bar, uint32_t parity) {
-        return mbar_wait(bar, parity & 1u, p.limit_ns, p.err, &sh_abort);
+        return wait_asleep(bar, parity & 1u, p.limit_ns, p.err, &sh_abort);
     };
     // the same for a whole warp, which goes on together (tensor memory loads need that)
     const auto wait_warp = [&](uint64_t *bar, uint32_t parity) {
         return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+    };
+    // one arrival a warp, for all that its lanes did (32 arrivals would queue up)
+    const auto arrive_warp = [&](uint64_t *bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
     };
     if (tid == 0) p.ws_meta[2 * cta].x = 0;   // nothing to join, unless the run says so at its end
 
@@ -315,10 +373,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         w.take(p, plan, off - __ldcg(plan.before + lo));
     }
 
-    // The block's 65536 registers go where they are needed: 256 x 168 + 256 x 88.  (The spare
-    // warps make up the fourth warpgroup, so that every scheduler's share adds up, too.)
-    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // The block's 640 x 96 registers go where they are needed: 256 x 152 + 384 x 56.  (The spare
+    // warps make up the fifth warpgroup, so that every scheduler's share adds up, too.)
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
 
     if (busy && warp < 8) {
         // =============================== softmax ===============================
@@ -407,7 +465,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
             f_next = fabsf(p.scale_log2) * pow2(-ex_mine);
             fence_proxy_async_smem();
-            mbar_arrive(&bar_q[half]);
+            arrive_warp(&bar_q[half]);
         };
         const auto takes = [&](const Walk &k) {   // this half has rows of the block
             return half == 0 || static_cast<uint32_t>(k.s.n) * p.group > k.x.rb * kRows + kHalf;
@@ -577,177 +635,214 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(full_p);
+                arrive_warp(full_p);
             }
             if (!ok) break;
         }
-    } else if (busy && warp < 12) {
+    } else if (busy && warp < 16) {
         // =============================== conversion ===============================
-        constexpr uint32_t NC = DP / 16, RP = 128 / NC, NI = KT / RP;   // chunks a row, rows a step, steps
-        const uint32_t ct = tid - 256, chunk = ct % NC, row0 = ct / NC;
+        constexpr uint32_t NC = DP / 16, RP = 128 / NC, NI = KT / 2 / RP;  // chunks a row, rows a step, steps
+        const uint32_t ct = tid & 127u, chunk = ct % NC, row0 = ct / NC, second = warp >= 12 ? 1u : 0u;
         const bool there = chunk * 16u < D;      // columns past head_dim are zeros
-        // 16 codes to two 16-byte pieces of a 128-byte swizzled row; the columns' upper half
-        // writes its pieces in the other order, so that 8 lanes of a row meet 8 banks
-        const auto convert = [&](const uint8_t *raw, uint8_t *dst) {
+        // 16 codes to two 16-byte pieces of a 128-byte swizzled row.  The columns' upper half
+        // takes its second 8 codes first, so that 8 lanes of a row meet 8 banks.  (RP is a
+        // multiple of 8: a thread's rows share their place in the swizzle.)
+        const bool odd = chunk >= 4u;
+        const uint32_t piece = (chunk & 3u) * 2u, turn = row0 & 7u;
+        const uint32_t to = (chunk / 4u) * (KT * 128u) + row0 * 128u;
+        const uint32_t at0 = to + (((piece + odd) ^ turn) * 16u), at1 = to + (((piece + !odd) ^ turn) * 16u);
+        const auto convert = [&](const uint8_t *codes, uint8_t *dst) {
+            codes += row0 * D + chunk * 16u;
 #pragma unroll 4
             for (uint32_t i = 0; i < NI; ++i) {
-                const uint32_t row = i * RP + row0;
-                uint4 w4 = make_uint4(0, 0, 0, 0), a, b;
-                if (there) w4 = *reinterpret_cast<const uint4 *>(raw + row * D + chunk * 16u);
-                codes_to_half4(w4.x, a.x, a.y);
-                codes_to_half4(w4.y, a.z, a.w);
-                codes_to_half4(w4.z, b.x, b.y);
-                codes_to_half4(w4.w, b.z, b.w);
-                uint8_t *at = dst + (chunk / 4u) * (KT * 128u) + row * 128u;
-                const uint32_t piece = (chunk & 3u) * 2u, odd = chunk / 4u;
-                *reinterpret_cast<uint4 *>(at + (((piece + odd) ^ (row & 7u)) * 16u)) = odd ? b : a;
-                *reinterpret_cast<uint4 *>(at + (((piece + 1u - odd) ^ (row & 7u)) * 16u)) = odd ? a : b;
+                uint4 c = make_uint4(0, 0, 0, 0), h;
+                if (there) c = *reinterpret_cast<const uint4 *>(codes + i * RP * D);
+                if (odd) c = make_uint4(c.z, c.w, c.x, c.y);
+                codes_to_half4(c.x, h.x, h.y);
+                codes_to_half4(c.y, h.z, h.w);
+                *reinterpret_cast<uint4 *>(dst + at0 + i * RP * 128u) = h;
+                codes_to_half4(c.z, h.x, h.y);
+                codes_to_half4(c.w, h.z, h.w);
+                *reinterpret_cast<uint4 *>(dst + at1 + i * RP * 128u) = h;
             }
             fence_proxy_async_smem();
         };
-        // K of the run's tile, then V, and so on
+        // this warp's half of a tile's K, then of its V, and on to the next tile
 #pragma unroll 1
-        for (uint32_t x = 0; x < 2 * w.left; ++x) {
-            const uint32_t it = x >> 1, st = it & 1u, round = it >> 1;
-            const bool v = x & 1u;
-            if (!wait_warp(v ? &bar_rv[st] : &bar_rk[st], round)) break;
-            if (v ? round != 0 && !wait_warp(&bar_v_free[st], round - 1) : it != 0 && !wait_warp(&bar_k_free, it - 1)) break;
-            convert((v ? raw_v : raw_k) + st * Shape::kRawBytes, v ? sv + st * Shape::kKvBytes : sk);
-            mbar_arrive(v ? &bar_v[st] : &bar_k);
-            mbar_arrive(v ? &bar_rv_free[st] : &bar_rk_free[st]);
+        for (uint32_t x = second; x < 4 * w.left; x += 2) {
+            const uint32_t it = x >> 2, st = it & 1u, slot = x % kRawRing;
+            const bool v = x & 2u;
+            if (!wait_warp(&bar_r[slot], x / kRawRing)) break;
+            if (it >= 2 && !wait_warp(v ? &bar_v_free[st] : &bar_k_free[st], (it >> 1) - 1)) break;
+            convert(raw + slot * Shape::kRawBytes, (v ? sv : sk) + st * Shape::kKvBytes + second * (KT / 2 * 128u));
+            arrive_warp(v ? &bar_v[st] : &bar_k[st]);
+            arrive_warp(&bar_r_free[slot]);
         }
-    } else if (busy && warp == 12) {
+    } else if (busy && warp == 16) {
         // =============================== tensor products ===============================
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = umma_idesc_f16(kHalf, KT, false);
-            constexpr uint32_t idesc_o = umma_idesc_f16(kHalf, DP, true);
-            const uint32_t aq = smem_addr(sq), ak = smem_addr(sk), av = smem_addr(sv);
-            const auto scores = [&](uint32_t half) {
+        const uint32_t lead = elect_lane();
+        constexpr uint32_t idesc_s = umma_idesc_f16(kHalf, KT, false);
+        constexpr uint32_t idesc_o = umma_idesc_f16(kHalf, DP, true);
+        const uint32_t aq = smem_addr(sq), ak = smem_addr(sk), av = smem_addr(sv);
+        const auto scores = [&](uint32_t half, uint32_t st) {
 #pragma unroll
-                for (uint32_t x = 0; x < (kSplit ? 2u : 1u); ++x)
+            for (uint32_t x = 0; x < (kSplit ? 2u : 1u); ++x)
 #pragma unroll
-                    for (uint32_t k = 0; k < DP / 16; ++k) {
-                        const uint32_t q_off = half * Shape::kQHalf + x * (kHalf * DP * 2) + (k / 4) * (kHalf * 128) + (k % 4) * 32;
-                        const uint32_t k_off = (k / 4) * (KT * 128) + (k % 4) * 32;
-                        umma_f16_ss(tmem + half * Shape::kHalfCols, umma_desc_k_sw128(aq + q_off),
-                                    umma_desc_k_sw128(ak + k_off), idesc_s, x | k);
-                    }
-                umma_commit(&bar_s[half]);
-            };
-            const auto values = [&](uint32_t half, uint32_t st, bool add) {
-                const uint32_t d = tmem + half * Shape::kHalfCols;
-#pragma unroll
-                for (uint32_t x = 0; x < (kSplit ? 2u : 1u); ++x)
-#pragma unroll
-                    for (uint32_t k = 0; k < KT / 16; ++k)
-                        umma_f16_ts(d + Shape::kOCol, d + Shape::kPCol + 32 * x + 8 * k,
-                                    umma_desc_mn_sw128(av + st * Shape::kKvBytes + k * 2048, KT * 128), idesc_o,
-                                    (add ? 1u : 0u) | x | k);
-            };
-            uint32_t it = 0, done[2] = {0, 0}, seg[2] = {0, 0};
-            bool ok = true, more = true;
-            while (more && ok) {
-                const int32_t count = w.count;
-                const uint32_t halves = static_cast<uint32_t>(w.s.n) * p.group > w.x.rb * kRows + kHalf ? 2 : 1;
-                more = w.next(p, plan);
-                // step -1 only computes the first tile's scores; a half's values of a tile and its
-                // scores of the next one follow each other, while the other half has its softmax
-#pragma unroll 1
-                for (int32_t j = -1; j < count && ok; ++j) {
-                    const bool last = j + 1 == count;
-                    const uint32_t st = it & 1u;
-                    if (j >= 0 && !(ok = wait(&bar_v[st], it >> 1))) break;
-#pragma unroll 1
-                    for (uint32_t half = 0; half < halves; ++half) {
-                        if (j >= 0) {
-                            if (!(ok = wait(&bar_p[half], done[half]++))) break;
-                            tc_fence_after();
-                            values(half, st, j != 0);
-                        } else if (!(ok = wait(&bar_q[half], seg[half]++))) {
-                            break;
-                        }
-                        if (last) {
-                            umma_commit(&bar_o[half]);
-                        } else {
-                            if (half == 0 && !(ok = wait(&bar_k, j < 0 ? it : it + 1))) break;
-                            tc_fence_after();
-                            scores(half);
-                        }
-                    }
-                    if (!last) umma_commit(&bar_k_free);
-                    if (j >= 0) {
-                        umma_commit(&bar_v_free[st]);
-                        ++it;
-                    }
+                for (uint32_t k = 0; k < DP / 16; ++k) {
+                    const uint32_t q_off = half * Shape::kQHalf + x * (kHalf * DP * 2) + (k / 4) * (kHalf * 128) + (k % 4) * 32;
+                    const uint32_t k_off = (k / 4) * (KT * 128) + (k % 4) * 32;
+                    umma_f16_ss(lead, tmem + half * Shape::kHalfCols, umma_desc_k_sw128(aq + q_off),
+                                umma_desc_k_sw128(ak + st * Shape::kKvBytes + k_off), idesc_s, x | k);
                 }
-            }
-        }
-    } else if (busy && warp == 13) {
-        // =============================== copies ===============================
-        uint32_t it = 0;
+            umma_commit_by(lead, &bar_s[half]);
+        };
+        const auto values = [&](uint32_t half, uint32_t st, bool add) {
+            const uint32_t d = tmem + half * Shape::kHalfCols;
+#pragma unroll
+            for (uint32_t x = 0; x < (kSplit ? 2u : 1u); ++x)
+#pragma unroll
+                for (uint32_t k = 0; k < KT / 16; ++k)
+                    umma_f16_ts(lead, d + Shape::kOCol, d + Shape::kPCol + 32 * x + 8 * k,
+                                umma_desc_mn_sw128(av + st * Shape::kKvBytes + k * 2048, KT * 128), idesc_o,
+                                (add ? 1u : 0u) | x | k);
+        };
+        uint32_t it = 0, done[2] = {0, 0}, seg[2] = {0, 0};
         bool ok = true, more = true;
         while (more && ok) {
-            const Walk cur = w;
+            const int32_t count = w.count;
+            const uint32_t halves = static_cast<uint32_t>(w.s.n) * p.group > w.x.rb * kRows + kHalf ? 2 : 1;
             more = w.next(p, plan);
-            for (int32_t j = 0; j < cur.count; ++j, ++it) {
-                const uint32_t st = it & 1u, round = it >> 1, ring = it % kScaleRing;
-                // lane g: group g of 16 keys.  One that is not there stays as it is in shared
-                // memory (whole numbers all the same); its keys are masked or count as zeros.
-                const int32_t key = (cur.tile + j) * static_cast<int32_t>(KT) + static_cast<int32_t>(lane * 16u);
-                const bool wanted = lane < kGroups && key < cur.s.len;
-                int32_t page = -1;
-                if (wanted) {
-                    page = __ldg(p.pb.table + static_cast<uint64_t>(cur.x.b) * p.pb.table_stride +
-                                 (static_cast<uint32_t>(key) >> p.c.page_shift));
-                    if (page < 0 || static_cast<uint32_t>(page) >= p.c.num_pages) {
-                        record_error(p.err, kErrBadIndex);
-                        page = -1;
+            // step -1 only computes the first tile's scores; a half's values of a tile and its
+            // scores of the next one follow each other, while the other half has its softmax
+#pragma unroll 1
+            for (int32_t j = -1; j < count && ok; ++j) {
+                const bool last = j + 1 == count;
+                const uint32_t st = it & 1u;
+                const uint32_t next = j < 0 ? it : it + 1;     // the tile of the scores
+                if (j >= 0 && !(ok = wait_warp(&bar_v[st], it >> 1))) break;
+#pragma unroll 1
+                for (uint32_t half = 0; half < halves; ++half) {
+                    if (j >= 0) {
+                        if (!(ok = wait_warp(&bar_p[half], done[half]++))) break;
+                        tc_fence_after();
+                        values(half, st, j != 0);
+                    } else if (!(ok = wait_warp(&bar_q[half], seg[half]++))) {
+                        break;
+                    }
+                    if (last) {
+                        umma_commit_by(lead, &bar_o[half]);
+                    } else {
+                        if (half == 0 && !(ok = wait_warp(&bar_k[next & 1u], next >> 1))) break;
+                        tc_fence_after();
+                        scores(half, next & 1u);
                     }
                 }
-                const uint64_t at = page >= 0 ? static_cast<uint64_t>(page) * p.c.heads + cur.h : 0;
-                float ks = 0.0f, vs = 0.0f;
-                if (page >= 0) {
-                    ks = __ldg(p.c.K_scale + at);
-                    vs = __ldg(p.c.V_scale + at);
+                if (!last) umma_commit_by(lead, &bar_k_free[next & 1u]);
+                if (j >= 0) {
+                    umma_commit_by(lead, &bar_v_free[st]);
+                    ++it;
                 }
-                // Tile it - 2 of K is converted, so the scores of tile it - 3 are there, and so the
-                // weights of tile it - 4: its place in the ring of scales is free, too.
-                if (round && !(ok = wait_warp(&bar_rk_free[st], round - 1))) break;
-                if (lane < kGroups) {
-                    const float lv = vs > 0.0f ? __log2f(vs) : 0.0f;   // a page of zeros has the scale 0
-                    sh_k[ring][lane] = ks;
-                    sh_lv[ring][lane] = lv;
-                    sh_iv[ring][lane] = vs > 0.0f ? ex2(-lv) : 1.0f;
-                }
-                const uint32_t zeros = __ballot_sync(0xffffffffu, lane < kGroups && !(vs > 0.0f));
-                const uint32_t bytes = 16u * D * __popc(__ballot_sync(0xffffffffu, page >= 0));
-                if (lane == 0) sh_zeros[ring] = zeros;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_sc[ring]);
-                const uint64_t src = ((at << p.c.page_shift) + (static_cast<uint32_t>(key) & ((1u << p.c.page_shift) - 1u))) * D;
-                if (lane == 0) mbar_arrive_expect_tx(&bar_rk[st], bytes);
-                __syncwarp();
-                if (page >= 0)
-                    bulk_load_1d(raw_k + st * Shape::kRawBytes + lane * 16u * D, p.c.K + src, 16u * D, &bar_rk[st]);
-                if (round && !(ok = wait_warp(&bar_rv_free[st], round - 1))) break;
-                if (lane == 0) mbar_arrive_expect_tx(&bar_rv[st], bytes);
-                __syncwarp();
-                if (page >= 0)
-                    bulk_load_1d(raw_v + st * Shape::kRawBytes + lane * 16u * D, p.c.V + src, 16u * D, &bar_rv[st]);
             }
+        }
+    } else if (busy && warp == 17) {
+        // =============================== copies ===============================
+        // Lane g takes group g of 16 keys.  A tile's pages are looked up two tiles before its
+        // codes are copied, and its scales read one tile before, so that neither is waited for.
+        struct Group {
+            int32_t page;       // -1: not there
+            uint32_t h, slot;   // head; slot of its first key in the page
+            float ks, vs;
+        };
+        int32_t j = 0;          // tiles of the segment looked up
+        bool more = true;
+        const auto look_up = [&](Group &g) {
+            g.page = -1;
+            g.ks = g.vs = 0.0f;
+            if (!more) return;
+            const int32_t key = (w.tile + j) * static_cast<int32_t>(KT) + static_cast<int32_t>(lane * 16u);
+            g.h = w.h;
+            g.slot = static_cast<uint32_t>(key) & ((1u << p.c.page_shift) - 1u);
+            if (lane < kGroups && key < w.s.len)
+                g.page = __ldg(p.pb.table + static_cast<uint64_t>(w.x.b) * p.pb.table_stride +
+                               (static_cast<uint32_t>(key) >> p.c.page_shift));
+            else
+                g.slot = 0xffffffffu;
+            if (++j == w.count) {
+                j = 0;
+                more = w.next(p, plan);
+            }
+        };
+        const auto read_scales = [&](Group &g) {
+            if (g.slot == 0xffffffffu) return;
+            if (g.page < 0 || static_cast<uint32_t>(g.page) >= p.c.num_pages) {
+                record_error(p.err, kErrBadIndex);
+                g.page = -1;
+                return;
+            }
+            const uint64_t at = static_cast<uint64_t>(g.page) * p.c.heads + g.h;
+            g.ks = __ldg(p.c.K_scale + at);
+            g.vs = __ldg(p.c.V_scale + at);
+        };
+        const uint32_t tiles = w.left;
+        const uint32_t per_copy = min(1u << (p.c.page_shift - 4u), kGroups / 2);   // groups of a page in half a tile
+        Group now, next, later;
+        now.slot = next.slot = later.slot = 0xffffffffu;
+        now.h = next.h = later.h = 0;
+        look_up(next);
+        look_up(later);
+        read_scales(next);
+        uint32_t begun = 0;     // half tiles whose copies were begun
+        bool ok = true;
+        for (uint32_t it = 0; it < tiles; ++it) {
+            now = next;
+            next = later;
+            later.slot = 0xffffffffu;
+            look_up(later);
+            if (it + 1 < tiles) read_scales(next);
+            const uint32_t ring = it % kScaleRing;
+            // A group that is not there stays as it is in shared memory (whole numbers all the
+            // same); its keys are masked or count as zeros.
+            const uint64_t at = now.page >= 0 ? static_cast<uint64_t>(now.page) * p.c.heads + now.h : 0;
+            const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);
+            const uint64_t src = ((at << p.c.page_shift) + now.slot) * D;
+            const uint32_t zeros = __ballot_sync(0xffffffffu, lane < kGroups && !(now.vs > 0.0f));
+#pragma unroll 1
+            for (uint32_t part = 0; part < 4; ++part) {      // K in two halves, V in two
+                constexpr uint32_t kPart = kGroups / 2;      // groups of a half
+                const uint32_t x = 4 * it + part, slot = x % kRawRing, first = (part & 1u) * kPart;
+                // A half tile is copied when its place's last one is converted.  K's first half:
+                // K of tile it - 1 is then, so the scores of tile it - 3 are there (two tiles of K
+                // are kept), and so the weights of tile it - 4: its scales' place is free, too.
+                if (x >= kRawRing && !(ok = wait_warp(&bar_r_free[slot], x / kRawRing - 1))) break;
+                if (lane == first)
+                    mbar_arrive_expect_tx(&bar_r[slot], 16u * D * __popc(there >> first & ((1u << kPart) - 1u)));
+                // one copy for the groups of a page: by the lane of its first one in this half
+                if (now.page >= 0 && lane >= first && lane < first + kPart && (lane - first) % per_copy == 0)
+                    bulk_load_1d(raw + slot * Shape::kRawBytes + (lane - first) * 16u * D,
+                                 (part < 2 ? p.c.K : p.c.V) + src,
+                                 16u * D * __popc(there >> lane & ((1u << per_copy) - 1u)), &bar_r[slot]);
+                if (part == 0) {
+                    if (lane < kGroups) {
+                        const float lv = now.vs > 0.0f ? __log2f(now.vs) : 0.0f;   // a page of zeros has the scale 0
+                        sh_k[ring][lane] = now.ks;
+                        sh_lv[ring][lane] = lv;
+                        sh_iv[ring][lane] = now.vs > 0.0f ? ex2(-lv) : 1.0f;
+                    }
+                    if (lane == 0) sh_zeros[ring] = zeros;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar_sc[ring]);
+                }
+                begun = x + 1;
+            }
+            if (!ok) break;
         }
         // a run that was given up may leave copies in flight: they end before the block does
         if (!ok)
-            for (uint32_t i = 0; i < 2; ++i) {
-                const uint32_t n = (it + 1 - i) / 2;   // tiles of this slot that were begun
-                if (n) {
-                    mbar_wait(&bar_rk[i], (n - 1) & 1u, p.limit_ns, nullptr, nullptr);
-                    mbar_wait(&bar_rv[i], (n - 1) & 1u, p.limit_ns, nullptr, nullptr);
-                }
-            }
+            for (uint32_t x = begun > kRawRing ? begun - kRawRing : 0; x < begun; ++x)
+                mbar_wait(&bar_r[x % kRawRing], (x / kRawRing) & 1u, p.limit_ns, nullptr, nullptr);
     }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 2 * Shape::kHalfCols);
