@@ -81,28 +81,26 @@ __device__ __forceinline__ void seq_units(const AttnParams &p, uint32_t b, Curso
     k.nt = max(1, hi - k.lo);
 }
 
-// The next unit; loads the next sequence that has rows where one ends (the
-// caller stops before the last unit's successor is asked for).
+// The next unit; true where it belongs to another row tile.  Loads the next
+// sequence that has rows where one ends (the caller stops before the last
+// unit's successor is asked for).
 template <uint32_t MR>
-__device__ __forceinline__ void next_unit(const AttnParams &p, Cursor &k) {
-    if (++k.tile < k.lo + k.nt) return;
-    if (++k.rt < k.rts) {
-        k.tile = k.lo;
-        return;
+__device__ __forceinline__ bool next_unit(const AttnParams &p, Cursor &k) {
+    if (++k.tile < k.lo + k.nt) return false;
+    if (++k.rt == k.rts) {
+        k.rt = 0;
+        if (++k.h == p.c.heads) {
+            k.h = 0;
+            bool bad;
+            uint32_t b = k.b;
+            do {
+                if (++b >= p.pb.batch) break;
+                seq_units<MR>(p, b, k, &bad);
+            } while (k.rts == 0);
+        }
     }
-    k.rt = 0;
-    if (++k.h < p.c.heads) {
-        k.tile = k.lo;
-        return;
-    }
-    k.h = 0;
-    bool bad;
-    uint32_t b = k.b;
-    do {
-        if (++b >= p.pb.batch) break;
-        seq_units<MR>(p, b, k, &bad);
-    } while (k.rts == 0);
     k.tile = k.lo;
+    return true;
 }
 
 // Persistent CTAs, each with an equal run of units: sequences of any lengths
@@ -110,13 +108,17 @@ __device__ __forceinline__ void next_unit(const AttnParams &p, Cursor &k) {
 // CTAs only where runs meet.  A warp keeps kStages - 1 units in flight through
 // its own ring of cp.async copies (no CTA-wide waits within a run), across
 // the ends of sequences too.
-template <RowType T, uint32_t DP>
+//
+// MR, the query rows of a tile: 16 for 16-bit rows; 8 where no sequence has
+// more (the upper half of the tile is then zeros that cost no softmax); 8 for
+// f32, whose low halves are the upper rows.
+template <RowType T, uint32_t DP, uint32_t MR>
 __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
-    paged_attention_kernel(const AttnParams p, const uint32_t min_units) {
+    paged_attention_kernel(const __grid_constant__ AttnParams p, const uint32_t min_units) {
     using E = typename RowOf<T>::type;
     using Shape = AttnShape<DP>;
     constexpr bool kSplit = T == RowType::kF32;
-    constexpr uint32_t MR = kSplit ? 8 : 16;       // query rows of a tile
+    static_assert(MR == 8 || (MR == 16 && !kSplit), "rows of a tile");
     constexpr uint32_t S = Shape::kStages, NC = DP / 16, NG = DP / 64, NJ = DP / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float sh_scale[kWarps][S][4];       // K_scale and V_scale of a unit's 16-key groups
@@ -205,20 +207,31 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
                                : -1;
         }
     };
+    // What the row tile to copy for sees at most, and the place of this lane's 16 bytes.
+    int32_t ahead_min = 0, ahead_max = 0;
+    const auto ahead_limits = [&]() {
+        int32_t unused;
+        row_limits(p, ahead.s, ahead.rt * MR, ahead_min, unused);
+        row_limits(p, ahead.s, ahead.rt * MR + MR - 1, unused, ahead_max);
+    };
+    const uint32_t my_row = lane / NC, my_ch = lane % NC, lane_src = my_row * D + my_ch * 16u;
+    const bool my_ch_there = my_ch * 16u < D;
+    constexpr uint32_t kStep = 32 / NC;                          // rows of a warp's copy
+    const auto place = [&](uint32_t q) {                         // of its row q * kStep + my_row
+        const uint32_t row = q * kStep + my_row;
+        return row * DP + (DP == 64 ? my_ch ^ ((row >> 1) & 3u) : my_ch ^ (row & 7u)) * 16u;
+    };
     const auto issue = [&]() {
         if (ahead_left) {
             const int32_t k0 = ahead.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
             uint8_t *const dst = ring + slot_in * Shape::kSlot;
-            int32_t kmin0, kmax1, unused;
-            row_limits(p, ahead.s, ahead.rt * MR, kmin0, unused);
-            row_limits(p, ahead.s, ahead.rt * MR + MR - 1, unused, kmax1);
             uint64_t base[2];
             bool ok[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int32_t key = k0 + 16 * i;
                 // a group with nothing to see is left as it is
-                const bool live = key < ahead.s.len && key <= kmax1 && key + 16 > kmin0;
+                const bool live = key < ahead.s.len && key <= ahead_max && key + 16 > ahead_min;
                 ok[i] = live && page_next[i] >= 0 && static_cast<uint32_t>(page_next[i]) < p.c.num_pages;
                 if (live && !ok[i] && lane == 0) record_error(p.err, kErrBadIndex);
                 const uint64_t at = ok[i] ? static_cast<uint64_t>(page_next[i]) * p.c.heads + ahead.h : 0;
@@ -228,23 +241,34 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
                 if (lane == 2 + i)
                     cp_async_4_zfill(&sh_scale[warp][slot_in][2 + i], p.c.V_scale + at, ok[i]);
             }
+            constexpr uint32_t kCopies = kWarpKeys / kStep;      // of K, and of V
+            if (ok[0] && ok[1] && k0 + static_cast<int32_t>(kWarpKeys) <= ahead.s.len) {
+                if (my_ch_there) {
 #pragma unroll
-            for (uint32_t q = 0; q < kWarpKeys * NC / 32; ++q) {
-                const uint32_t idx = lane + 32 * q, row = idx / NC, ch = idx % NC;
-                const uint32_t i = q / (16 * NC / 32);       // the row's 16-key group
-                const uint32_t sw = DP == 64 ? ch ^ ((row >> 1) & 3u) : ch ^ (row & 7u);
-                const bool in = ok[i] && k0 + static_cast<int32_t>(row) < ahead.s.len;
-                if (ch * 16u < D) {
-                    const uint64_t src = base[i] + (row & 15u) * D + ch * 16u;
-                    cp_async_16_zfill(dst + row * DP + sw * 16u, p.c.K + (in ? src : 0), in);
-                    cp_async_16_zfill(dst + kWarpKeys * DP + row * DP + sw * 16u, p.c.V + (in ? src : 0), in);
+                    for (uint32_t q = 0; q < kCopies; ++q) {
+                        const uint64_t src = base[q / (kCopies / 2)] + lane_src + (q % (kCopies / 2)) * kStep * D;
+                        cp_async_16(dst + place(q), p.c.K + src);
+                        cp_async_16(dst + kWarpKeys * DP + place(q), p.c.V + src);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (uint32_t q = 0; q < kCopies; ++q) {         // a sequence's last keys
+                    const uint32_t i = q / (kCopies / 2);
+                    const bool in = ok[i] && k0 + static_cast<int32_t>(q * kStep + my_row) < ahead.s.len;
+                    const uint64_t src = in ? base[i] + lane_src + (q % (kCopies / 2)) * kStep * D : 0;
+                    if (my_ch_there) {
+                        cp_async_16_zfill(dst + place(q), p.c.K + src, in);
+                        cp_async_16_zfill(dst + kWarpKeys * DP + place(q), p.c.V + src, in);
+                    }
                 }
             }
-            if (--ahead_left) next_unit<MR>(p, ahead);
+            if (--ahead_left && next_unit<MR>(p, ahead)) ahead_limits();
         }
         cp_async_commit();
         slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
     };
+    ahead_limits();
 
     fetch_pages();
 #pragma unroll
@@ -266,7 +290,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
         row_limits(p, cur.s, cur.rt * MR + MR - 1, kmin_last, kmax_last);
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
-            if (kSplit && i == 1) break;
+            if (MR == 8 && i == 1) break;
             const uint32_t r = cur.rt * MR + n + 8 * i;
             row_limits(p, cur.s, r, kmin[i], kmax[i]);
             m[i] = -INFINITY;
@@ -310,6 +334,8 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
                         const float2 h0 = unpack_half2(aq[g][s][0]), h1 = unpack_half2(aq[g][s][2]);
                         aq[g][s][1] = pack_half2(x0 - h0.x, x1 - h0.y);
                         aq[g][s][3] = pack_half2(x2 - h1.x, x3 - h1.y);
+                    } else if constexpr (MR == 8) {
+                        aq[g][s][1] = aq[g][s][3] = 0;
                     }
                 }
         }
@@ -319,7 +345,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
             for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
     };
 
-    constexpr uint32_t NR = kSplit ? 1 : 2;      // rows of a thread
+    constexpr uint32_t NR = MR / 8;              // rows of a thread
     const auto compute = [&](uint32_t slot) {
         const int32_t k0 = cur.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
         if (k0 > kmax_last || k0 + static_cast<int32_t>(kWarpKeys) <= kmin_first) return;  // warp-uniform
@@ -389,13 +415,14 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
                 l[r] *= f[r];
                 m[r] = to;
             }
-            const float f1 = kSplit ? f[0] : f[1];
 #pragma unroll
             for (uint32_t j = 0; j < NJ; ++j) {
                 acc[j][0] *= f[0];
                 acc[j][1] *= f[0];
-                acc[j][2] *= f1;
-                acc[j][3] *= f1;
+                if constexpr (kSplit || MR == 16) {
+                    acc[j][2] *= f[NR - 1];
+                    acc[j][3] *= f[NR - 1];
+                }
             }
         }
         float off[2];
@@ -418,6 +445,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
                 } else {
                     if (!on[t >> 1]) h = 0;
                     pa[t >> 1][2 * (t & 1) + r] = h;
+                    if constexpr (MR == 8) pa[t >> 1][2 * (t & 1) + 1] = 0;
                 }
             }
         // values: a thread's rows kq, +4, +8, +12 of a 16-key group and the dims of lane group n
@@ -579,10 +607,9 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
 // Joins a row tile's parts: block (c, y) those of the tile that begins in CTA
 // c and goes on in the next ones, 32 groups of 4 values of it; 8 lanes share
 // the parts, added in a fixed order.
-template <RowType T, uint32_t DP>
+template <RowType T, uint32_t DP, uint32_t MR>
 __global__ void __launch_bounds__(256) paged_attention_join_kernel(const AttnParams p) {
     using E = typename RowOf<T>::type;
-    constexpr uint32_t MR = T == RowType::kF32 ? 8 : 16;
     __shared__ float4 sh_o[8][32];
     __shared__ float2 sh_ml[8][32];
     pdl_enter();
@@ -639,10 +666,9 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const AttnPar
     from_f32(o.w * inv, out[3]);
 }
 
-template <RowType T, uint32_t DP>
+template <RowType T, uint32_t DP, uint32_t MR>
 cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
     using Shape = AttnShape<DP>;
-    constexpr uint32_t MR = T == RowType::kF32 ? 8 : 16;
     const uint32_t elem = T == RowType::kF32 ? 4 : 2;
     AttnParams p{};
     p.c = a.cache;
@@ -662,7 +688,7 @@ cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
     int device = 0;
     VNPU_LAUNCH(cudaGetDevice(&device));
     if (ready_device != device) {
-        VNPU_LAUNCH(cudaFuncSetAttribute(paged_attention_kernel<T, DP>,
+        VNPU_LAUNCH(cudaFuncSetAttribute(paged_attention_kernel<T, DP, MR>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem));
         ready_device = device;
     }
@@ -679,24 +705,32 @@ cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
         p.ws_meta = reinterpret_cast<uint4 *>(static_cast<char *>(ws) + o_bytes + ml_bytes);
     }
     if (ctx.launch_counter) *ctx.launch_counter += split ? 2 : 1;
-    cudaError_t e = launch_pdl(ctx.stream, &paged_attention_kernel<T, DP>, dim3(grid), dim3(kThreadsA),
+    cudaError_t e = launch_pdl(ctx.stream, &paged_attention_kernel<T, DP, MR>, dim3(grid), dim3(kThreadsA),
                                Shape::kSmem, p, 1u);
     if (split) {
         const uint64_t rows = std::min<uint64_t>(MR, 1ull * a.batch.max_tokens * p.group);
         const uint32_t y = static_cast<uint32_t>((rows * (DP / 4) + 31) / 32);
         if (e == cudaSuccess)
-            e = launch_pdl(ctx.stream, &paged_attention_join_kernel<T, DP>, dim3(grid, y), dim3(256), 0, p);
+            e = launch_pdl(ctx.stream, &paged_attention_join_kernel<T, DP, MR>, dim3(grid, y), dim3(256), 0, p);
         const cudaError_t f = cudaFreeAsync(ws, ctx.stream);
         if (e == cudaSuccess) e = f;
     }
     return e;
 }
 
-template <RowType T>
+template <RowType T, uint32_t MR>
 cudaError_t launch_by_dim(const LaunchCtx &ctx, const PagedAttention &a) {
-    if (a.cache.head_dim <= 64) return launch_attention<T, 64>(ctx, a);
-    if (a.cache.head_dim <= 128) return launch_attention<T, 128>(ctx, a);
-    return launch_attention<T, 256>(ctx, a);
+    if (a.cache.head_dim <= 64) return launch_attention<T, 64, MR>(ctx, a);
+    if (a.cache.head_dim <= 128) return launch_attention<T, 128, MR>(ctx, a);
+    return launch_attention<T, 256, MR>(ctx, a);
+}
+
+template <RowType T>
+cudaError_t launch_few(const LaunchCtx &ctx, const PagedAttention &a) {
+    if constexpr (T != RowType::kF32) {
+        if (1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > 8) return launch_by_dim<T, 16>(ctx, a);
+    }
+    return launch_by_dim<T, 8>(ctx, a);
 }
 
 }  // namespace
@@ -707,9 +741,9 @@ cudaError_t paged_attention(const LaunchCtx &ctx, const PagedAttention &a) {
         if (e != cudaErrorNotSupported) return e;
     }
     switch (a.type) {
-    case RowType::kF32: return launch_by_dim<RowType::kF32>(ctx, a);
-    case RowType::kF16: return launch_by_dim<RowType::kF16>(ctx, a);
-    default: return launch_by_dim<RowType::kBF16>(ctx, a);
+    case RowType::kF32: return launch_few<RowType::kF32>(ctx, a);
+    case RowType::kF16: return launch_few<RowType::kF16>(ctx, a);
+    default: return launch_few<RowType::kBF16>(ctx, a);
     }
 }
 
