@@ -12,9 +12,8 @@
 // bits, so both products run on f16 tensor instructions with nothing lost on
 // the cache's side.  A query row is scaled by a power of two to a largest
 // element in [2^13, 2^14): f16 and bf16 queries are then exact too (down to
-// 2^-27 of the row's largest), and f32 ones become hi + lo, 22 bits, as two
-// rows of the 16-row tile whose products are added; their weights p are split
-// the same way.  Sums, maxima and accumulators are f32.
+// 2^-27 of the row's largest), and f32 ones become hi + lo, 22 bits, two
+// products on one accumulator; their weights p are split the same way.  Sums, maxima and accumulators are f32.
 //
 // m follows the running maximum only when that has grown by more than 2^6, so
 // the accumulators are rescaled a few times a row instead of at every step.
@@ -29,23 +28,29 @@ constexpr uint32_t kWarps = 4, kThreadsA = kWarps * 32;
 constexpr uint32_t kTile = 128;      // keys of a work unit, 32 for each warp
 constexpr uint32_t kWarpKeys = kTile / kWarps;
 
-template <uint32_t DP>
+// As many CTAs an SM as the registers allow (the kernel is bound by the latency
+// of its own instructions before it is by memory), rings as deep as that allows.
+template <uint32_t DP, uint32_t MR>
 struct AttnShape {
-    static constexpr uint32_t kStages = DP == 64 ? 6 : 3;
+    static constexpr uint32_t kCtasPerSm = DP == 256 ? 1 : MR == 8 ? 3 : 2;
     static constexpr uint32_t kSlot = kWarpKeys * DP * 2;   // a warp's K and V codes of a unit
+    static constexpr uint32_t kStages = (DP == 256 ? 200u : 208u / kCtasPerSm) * 1024 / (kWarps * kSlot);
     static constexpr uint32_t kSmem = kWarps * kStages * kSlot;
-    static constexpr uint32_t kCtasPerSm = DP == 256 ? 1 : 2;
+    static_assert(kStages >= 2 && kSlot >= 16 * DP * 4, "a slot also takes a warp's accumulators");
 };
-// A slot also takes a warp's 16 x DP f32 accumulators when warps are joined.
-static_assert(AttnShape<128>::kSlot == 16 * 128 * 4, "a slot holds a warp's accumulators");
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of 16-bit elements held as a product's fragment.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ float quad_max(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
@@ -109,17 +114,22 @@ __device__ __forceinline__ bool next_unit(const AttnParams &p, Cursor &k) {
 // its own ring of cp.async copies (no CTA-wide waits within a run), across
 // the ends of sequences too.
 //
-// MR, the query rows of a tile: 16 for 16-bit rows; 8 where no sequence has
-// more (the upper half of the tile is then zeros that cost no softmax); 8 for
-// f32, whose low halves are the upper rows.
+// The products are transposed: S^T = K Q^T and O^T += V^T P^T, so that the 16-row
+// side of the tensor instruction is keys, then head_dim, and the query rows are
+// its 8 columns.  For the few rows of a decode step that is half the products
+// and half the accumulators of S = Q K^T.  P^T's fragment is S^T's transposed
+// 8 x 8 by 8 x 8, one instruction each.  MR, the query rows of a tile, is 8, or
+// 16 (two column tiles under one conversion of the codes) where a sequence has
+// more.
 template <RowType T, uint32_t DP, uint32_t MR>
-__global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
+__global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     paged_attention_kernel(const __grid_constant__ AttnParams p, const uint32_t min_units) {
     using E = typename RowOf<T>::type;
-    using Shape = AttnShape<DP>;
+    using Shape = AttnShape<DP, MR>;
     constexpr bool kSplit = T == RowType::kF32;
-    static_assert(MR == 8 || (MR == 16 && !kSplit), "rows of a tile");
-    constexpr uint32_t S = Shape::kStages, NC = DP / 16, NG = DP / 64, NJ = DP / 8;
+    static_assert(MR == 8 || MR == 16, "rows of a tile");
+    constexpr uint32_t NT = MR / 8;                // column tiles
+    constexpr uint32_t S = Shape::kStages, NC = DP / 16, NG = DP / 64, NJ = DP / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float sh_scale[kWarps][S][4];       // K_scale and V_scale of a unit's 16-key groups
     __shared__ float2 sh_ml[kWarps][16];
@@ -214,12 +224,17 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
         row_limits(p, ahead.s, ahead.rt * MR, ahead_min, unused);
         row_limits(p, ahead.s, ahead.rt * MR + MR - 1, unused, ahead_max);
     };
+    // 16-byte pieces of a row of codes change places by this: the readers below take pieces kq
+    // of two rows next to each other (K), and pieces m, m + 4 of every second row (V)
+    const auto swizzle = [](uint32_t row) {
+        return DP == 64 ? (row >> 1) & 3u : (row & 1u) << 2 | ((row >> 1) & 3u);
+    };
     const uint32_t my_row = lane / NC, my_ch = lane % NC, lane_src = my_row * D + my_ch * 16u;
     const bool my_ch_there = my_ch * 16u < D;
     constexpr uint32_t kStep = 32 / NC;                          // rows of a warp's copy
     const auto place = [&](uint32_t q) {                         // of its row q * kStep + my_row
         const uint32_t row = q * kStep + my_row;
-        return row * DP + (DP == 64 ? my_ch ^ ((row >> 1) & 3u) : my_ch ^ (row & 7u)) * 16u;
+        return row * DP + (my_ch ^ swizzle(row)) * 16u;
     };
     const auto issue = [&]() {
         if (ahead_left) {
@@ -255,8 +270,8 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
 #pragma unroll 1
                 for (uint32_t q = 0; q < kCopies; ++q) {         // a sequence's last keys
                     const uint32_t i = q / (kCopies / 2);
-                    const bool in = ok[i] && k0 + static_cast<int32_t>(q * kStep + my_row) < ahead.s.len;
-                    const uint64_t src = in ? base[i] + lane_src + (q % (kCopies / 2)) * kStep * D : 0;
+                    const bool in = (i ? ok[1] : ok[0]) && k0 + static_cast<int32_t>(q * kStep + my_row) < ahead.s.len;
+                    const uint64_t src = in ? (i ? base[1] : base[0]) + lane_src + (q % (kCopies / 2)) * kStep * D : 0;
                     if (my_ch_there) {
                         cp_async_16_zfill(dst + place(q), p.c.K + src, in);
                         cp_async_16_zfill(dst + kWarpKeys * DP + place(q), p.c.V + src, in);
@@ -278,10 +293,13 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
     }
 
     // ---- state of the current (sequence, head, row tile)
-    uint32_t aq[NG][4][4];       // query fragments
-    float acc[NJ][4];
-    float m[2], l[2], qf[2];     // running maximum, sum, and score factor of rows n, n + 8
-    int32_t kmin[2], kmax[2], kmin_last = 0, kmax_first = 0, kmin_first = 0, kmax_last = 0;
+    uint32_t bq[NT][NG][4][2];             // query fragments
+    uint32_t bl[kSplit ? NT : 1][NG][4][2];  // f32: their low halves
+    float acc[NT][NJ][4];
+    // of rows 8 t + 2 kq and + 1: running maximum, sum, score factor, and what the scores have too
+    // much (codes_to_half4_biased)
+    float m[NT][2], l[NT][2], qf[NT][2], q_bias[NT][2];
+    int32_t kmin[NT][2], kmax[NT][2], kmin_last = 0, kmax_first = 0, kmin_first = 0, kmax_last = 0;
     int32_t first_tile = 0;
     const auto begin_rows = [&]() {
         first_tile = cur.tile;
@@ -289,12 +307,8 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
         row_limits(p, cur.s, cur.rt * MR, kmin_first, kmax_first);
         row_limits(p, cur.s, cur.rt * MR + MR - 1, kmin_last, kmax_last);
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) {
-            if (MR == 8 && i == 1) break;
-            const uint32_t r = cur.rt * MR + n + 8 * i;
-            row_limits(p, cur.s, r, kmin[i], kmax[i]);
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
+        for (uint32_t t = 0; t < NT; ++t) {
+            const uint32_t r = cur.rt * MR + 8 * t + n;     // the row of this lane's fragment
             float v[NG][16];
             float most = 0.0f;
             const uint32_t token = r / p.group;
@@ -321,56 +335,77 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
             most = quad_max(most);
             const int ex = row_exponent(most);
             const float up = pow2(ex);
-            qf[i] = p.scale_log2 * pow2(-ex);
+            float total = 0.0f;
 #pragma unroll
             for (uint32_t g = 0; g < NG; ++g)
 #pragma unroll
-                for (uint32_t s = 0; s < 4; ++s) {
-                    const float x0 = v[g][4 * s] * up, x1 = v[g][4 * s + 1] * up;
-                    const float x2 = v[g][4 * s + 2] * up, x3 = v[g][4 * s + 3] * up;
-                    aq[g][s][i] = pack_half2(x0, x1);
-                    aq[g][s][2 + i] = pack_half2(x2, x3);
-                    if constexpr (kSplit) {
-                        const float2 h0 = unpack_half2(aq[g][s][0]), h1 = unpack_half2(aq[g][s][2]);
-                        aq[g][s][1] = pack_half2(x0 - h0.x, x1 - h0.y);
-                        aq[g][s][3] = pack_half2(x2 - h1.x, x3 - h1.y);
-                    } else if constexpr (MR == 8) {
-                        aq[g][s][1] = aq[g][s][3] = 0;
+                for (uint32_t s = 0; s < 4; ++s)
+#pragma unroll
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        const float x0 = v[g][4 * s + 2 * k] * up, x1 = v[g][4 * s + 2 * k + 1] * up;
+                        bq[t][g][s][k] = pack_half2(x0, x1);
+                        const float2 y = unpack_half2(bq[t][g][s][k]);
+                        if constexpr (kSplit) bl[t][g][s][k] = pack_half2(x0 - y.x, x1 - y.y);
+                        else total += y.x + y.y;
                     }
-                }
+            total += __shfl_xor_sync(0xffffffffu, total, 1);
+            total += __shfl_xor_sync(0xffffffffu, total, 2);
+            const float factor = p.scale_log2 * pow2(-ex);
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) {
+                qf[t][e] = __shfl_sync(0xffffffffu, factor, 8 * kq + 4 * e);
+                q_bias[t][e] = kCodeBias * __shfl_sync(0xffffffffu, total, 8 * kq + 4 * e);
+                row_limits(p, cur.s, cur.rt * MR + 8 * t + 2 * kq + e, kmin[t][e], kmax[t][e]);
+                m[t][e] = -INFINITY;
+                l[t][e] = 0.0f;
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.0f;
         }
-#pragma unroll
-        for (uint32_t j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
     };
 
-    constexpr uint32_t NR = MR / 8;              // rows of a thread
     const auto compute = [&](uint32_t slot) {
         const int32_t k0 = cur.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
         if (k0 > kmax_last || k0 + static_cast<int32_t>(kWarpKeys) <= kmin_first) return;  // warp-uniform
         const uint8_t *kb = ring + slot * Shape::kSlot, *vb = kb + kWarpKeys * DP;
         const float *sc = sh_scale[warp][slot];
-        // scores of 4 x 8 keys: column c of tile 2i + tt is key 16i + 8tt + (c >> 1) + 4 (c & 1),
-        // so a thread's two columns are keys kq and kq + 4, the rows of V it reads below
-        float s[4][4];
+        // scores of two groups of 16 keys: element e of a fragment is key n + 8 (e >> 1) of the
+        // group and row 2 kq + (e & 1).  The head_dim index is permuted, the same way in K and Q:
+        // a lane's 16 codes are the elements of four products
+        float s[2][NT][4];
 #pragma unroll
-        for (uint32_t t = 0; t < 4; ++t) {
-            s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.0f;
-            const uint32_t row = 8u * t + (n >> 1) + 4u * (n & 1u);
+        for (uint32_t i = 0; i < 2; ++i)
 #pragma unroll
-            for (uint32_t g = 0; g < NG; ++g) {
-                const uint32_t ch = kq + 4u * g;
-                const uint32_t sw = DP == 64 ? ch ^ ((row >> 1) & 3u) : ch ^ (row & 7u);
-                const uint4 w = *reinterpret_cast<const uint4 *>(kb + row * DP + sw * 16u);
-                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+            for (uint32_t t = 0; t < NT; ++t) s[i][t][0] = s[i][t][1] = s[i][t][2] = s[i][t][3] = 0.0f;
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    uint32_t b0, b1;
-                    codes_to_half4(word[e], b0, b1);
-                    mma_f16(s[t], aq[g][e][0], aq[g][e][1], aq[g][e][2], aq[g][e][3], b0, b1);
-                }
+        for (uint32_t g = 0; g < NG; ++g) {
+            uint4 w[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t row = 8u * i + n;
+                w[i] = *reinterpret_cast<const uint4 *>(kb + row * DP + ((kq + 4u * g) ^ swizzle(row)) * 16u);
             }
+            const auto word = [&](uint32_t i, uint32_t e) { return e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w; };
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    uint32_t a0, a1, a2, a3;
+                    if constexpr (kSplit) {
+                        codes_to_half4(word(2 * i, e), a0, a2);
+                        codes_to_half4(word(2 * i + 1, e), a1, a3);
+                    } else {
+                        codes_to_half4_biased(word(2 * i, e), a0, a2);
+                        codes_to_half4_biased(word(2 * i + 1, e), a1, a3);
+                    }
+#pragma unroll
+                    for (uint32_t t = 0; t < NT; ++t) {
+                        mma_f16(s[i][t], a0, a1, a2, a3, bq[t][g][e][0], bq[t][g][e][1]);
+                        if constexpr (kSplit) mma_f16(s[i][t], a0, a1, a2, a3, bl[t][g][e][0], bl[t][g][e][1]);
+                    }
+                }
         }
         float lv[2], iv[2];
         bool on[2];
@@ -382,89 +417,87 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
             iv[i] = on[i] ? ex2(-lv[i]) : 1.0f;
         }
         const bool edge = k0 + static_cast<int32_t>(kWarpKeys) - 1 > kmax_first || k0 < kmin_last;
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (uint32_t t = 0; t < 4; ++t)
-#pragma unroll
-            for (uint32_t r = 0; r < NR; ++r) {
-                const float f = qf[r] * sc[t >> 1];
-#pragma unroll
-                for (uint32_t e = 0; e < 2; ++e) {
-                    float x = kSplit ? s[t][e] + s[t][2 + e] : s[t][2 * r + e];
-                    x = fmaf(x, f, lv[t >> 1]);
-                    if (edge) {
-                        const int32_t key = k0 + static_cast<int32_t>(8 * t + kq + 4 * e);
-                        if (key > kmax[r] || key < kmin[r]) x = -INFINITY;
-                    }
-                    s[t][2 * r + e] = x;
-                    top[r] = fmaxf(top[r], x);
-                }
-            }
+        float top[NT][2];
         bool grown = false;
 #pragma unroll
-        for (uint32_t r = 0; r < NR; ++r) {
-            top[r] = quad_max(top[r]);
-            grown |= top[r] > m[r] + kSlack;
-        }
+        for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+            for (uint32_t r = 0; r < 2; ++r) {
+                top[t][r] = -INFINITY;
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    const float f = qf[t][r] * sc[i];
+                    const float b = kSplit ? lv[i] : fmaf(-q_bias[t][r], f, lv[i]);
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        float x = fmaf(s[i][t][2 * e + r], f, b);
+                        if (edge) {
+                            const int32_t key = k0 + static_cast<int32_t>(16 * i + 8 * e + n);
+                            if (key > kmax[t][r] || key < kmin[t][r]) x = -INFINITY;
+                        }
+                        s[i][t][2 * e + r] = x;
+                        top[t][r] = fmaxf(top[t][r], x);
+                    }
+                }
+#pragma unroll
+                for (uint32_t o = 4; o < 32; o <<= 1)
+                    top[t][r] = fmaxf(top[t][r], __shfl_xor_sync(0xffffffffu, top[t][r], o));
+                grown |= top[t][r] > m[t][r] + kSlack;
+            }
         if (__any_sync(0xffffffffu, grown)) {
-            float f[2];
 #pragma unroll
-            for (uint32_t r = 0; r < NR; ++r) {
-                const float to = fmaxf(m[r], top[r]);
-                f[r] = to > m[r] ? ex2(m[r] - to) : 1.0f;
-                l[r] *= f[r];
-                m[r] = to;
-            }
+            for (uint32_t t = 0; t < NT; ++t) {
+                float f[2];
 #pragma unroll
-            for (uint32_t j = 0; j < NJ; ++j) {
-                acc[j][0] *= f[0];
-                acc[j][1] *= f[0];
-                if constexpr (kSplit || MR == 16) {
-                    acc[j][2] *= f[NR - 1];
-                    acc[j][3] *= f[NR - 1];
+                for (uint32_t r = 0; r < 2; ++r) {
+                    const float to = fmaxf(m[t][r], top[t][r]);
+                    f[r] = to > m[t][r] ? ex2(m[t][r] - to) : 1.0f;
+                    l[t][r] *= f[r];
+                    m[t][r] = to;
                 }
+#pragma unroll
+                for (uint32_t j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) acc[t][j][e] *= f[e & 1];
             }
         }
-        float off[2];
+        uint32_t pb[2][NT][2], pl[2][kSplit ? NT : 1][2];
 #pragma unroll
-        for (uint32_t r = 0; r < NR; ++r) off[r] = m[r] == -INFINITY ? 0.0f : m[r] - kLift;
-        uint32_t pa[2][4];
+        for (uint32_t t = 0; t < NT; ++t) {
+            float off[2];
 #pragma unroll
-        for (uint32_t t = 0; t < 4; ++t)
+            for (uint32_t r = 0; r < 2; ++r) off[r] = m[t][r] == -INFINITY ? 0.0f : m[t][r] - kLift;
 #pragma unroll
-            for (uint32_t r = 0; r < NR; ++r) {
-                const float x = ex2(s[t][2 * r] - off[r]), y = ex2(s[t][2 * r + 1] - off[r]);
-                l[r] = fmaf(x + y, iv[t >> 1], l[r]);
-                uint32_t h = pack_half2(x, y);
-                if constexpr (kSplit) {
-                    const float2 f = unpack_half2(h);
-                    uint32_t lo = pack_half2(x - f.x, y - f.y);
-                    if (!on[t >> 1]) h = lo = 0;
-                    pa[t >> 1][2 * (t & 1)] = h;
-                    pa[t >> 1][2 * (t & 1) + 1] = lo;
-                } else {
-                    if (!on[t >> 1]) h = 0;
-                    pa[t >> 1][2 * (t & 1) + r] = h;
-                    if constexpr (MR == 8) pa[t >> 1][2 * (t & 1) + 1] = 0;
+            for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    const float x = ex2(s[i][t][2 * e] - off[0]), y = ex2(s[i][t][2 * e + 1] - off[1]);
+                    l[t][0] = fmaf(x, iv[i], l[t][0]);
+                    l[t][1] = fmaf(y, iv[i], l[t][1]);
+                    const uint32_t h = on[i] ? pack_half2(x, y) : 0u;
+                    pb[i][t][e] = transpose8x8(h);
+                    if constexpr (kSplit) {
+                        const float2 u = unpack_half2(h);
+                        pl[i][t][e] = transpose8x8(on[i] ? pack_half2(x - u.x, y - u.y) : 0u);
+                    }
                 }
-            }
-        // values: a thread's rows kq, +4, +8, +12 of a 16-key group and the dims of lane group n
+        }
+        // values: a lane's keys 2 kq, 2 kq + 1, + 8, + 9 of a group, and the dims of lane group n
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
             constexpr uint32_t NW = DP / 32;       // words of a row for a thread
             uint32_t w[4][NW];
 #pragma unroll
             for (uint32_t q = 0; q < 4; ++q) {
-                const uint32_t row = 16u * i + kq + 4u * q;
+                const uint32_t row = 16u * i + 2u * kq + (q & 1u) + 8u * (q >> 1);
                 if constexpr (DP == 64) {
-                    const uint32_t sw = (n >> 1) ^ ((row >> 1) & 3u);
-                    const uint2 x = *reinterpret_cast<const uint2 *>(vb + row * DP + sw * 16u + (n & 1u) * 8u);
+                    const uint2 x = *reinterpret_cast<const uint2 *>(vb + row * DP + ((n >> 1) ^ swizzle(row)) * 16u + (n & 1u) * 8u);
                     w[q][0] = x.x;
                     w[q][1] = x.y;
                 } else {
 #pragma unroll
                     for (uint32_t g = 0; g < DP / 128; ++g) {
-                        const uint32_t ch = 8u * g + (((n >> 1) + 4u * (n & 1u)) ^ (row & 7u));
+                        const uint32_t ch = 8u * g + (((n >> 1) + 4u * (n & 1u)) ^ swizzle(row));
                         const uint4 x = *reinterpret_cast<const uint4 *>(vb + row * DP + ch * 16u);
                         w[q][4 * g] = x.x;
                         w[q][4 * g + 1] = x.y;
@@ -474,16 +507,18 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
                 }
             }
 #pragma unroll
-            for (uint32_t k = 0; k < NW; ++k) {
-                uint32_t b0[4], b1[4];
-                codes_to_half4(__byte_perm(w[0][k], w[1][k], 0x5140), b0[0], b0[1]);
-                codes_to_half4(__byte_perm(w[0][k], w[1][k], 0x7362), b0[2], b0[3]);
-                codes_to_half4(__byte_perm(w[2][k], w[3][k], 0x5140), b1[0], b1[1]);
-                codes_to_half4(__byte_perm(w[2][k], w[3][k], 0x7362), b1[2], b1[3]);
+            for (uint32_t k = 0; k < NW; ++k)
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j)
-                    mma_f16(acc[4 * k + j], pa[i][0], pa[i][1], pa[i][2], pa[i][3], b0[j], b1[j]);
-            }
+                for (uint32_t half = 0; half < 2; ++half) {
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_half4(__byte_perm(w[0][k], w[1][k], half ? 0x7362 : 0x5140), a0, a1);
+                    codes_to_half4(__byte_perm(w[2][k], w[3][k], half ? 0x7362 : 0x5140), a2, a3);
+#pragma unroll
+                    for (uint32_t t = 0; t < NT; ++t) {
+                        mma_f16(acc[t][2 * k + half], a0, a1, a2, a3, pb[i][t][0], pb[i][t][1]);
+                        if constexpr (kSplit) mma_f16(acc[t][2 * k + half], a0, a1, a2, a3, pl[i][t][0], pl[i][t][1]);
+                    }
+                }
         }
     };
 
@@ -493,35 +528,30 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP>::kCtasPerSm)
         const uint32_t rows = min(MR, static_cast<uint32_t>(cur.s.n) * p.group - cur.rt * MR);
         float *const mine_o = reinterpret_cast<float *>(ring + slot * Shape::kSlot);
 #pragma unroll
-        for (uint32_t r = 0; r < NR; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (kq == 0) sh_ml[warp][n + 8 * r] = make_float2(m[r], l[r]);
-        }
+        for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+            for (uint32_t r = 0; r < 2; ++r) {
+#pragma unroll
+                for (uint32_t o = 4; o < 32; o <<= 1) l[t][r] += __shfl_xor_sync(0xffffffffu, l[t][r], o);
+                if (n == 0) sh_ml[warp][8 * t + 2 * kq + r] = make_float2(m[t][r], l[t][r]);
+            }
         __syncwarp();  // all lanes are done with the slot's codes
 #pragma unroll
-        for (uint32_t r = 0; r < NR; ++r) {
-            const uint32_t row = n + 8 * r;
-            if (row >= rows) continue;
+        for (uint32_t t = 0; t < NT; ++t)
 #pragma unroll
-            for (uint32_t e = 0; e < 2; ++e) {
-                // column 2 kq + e of tile j is dim j of the chunk that lane group 2 kq + e reads
+            for (uint32_t r = 0; r < 2; ++r) {
+                const uint32_t row = 8 * t + 2 * kq + r;
+                if (row >= rows) continue;
+                // a lane's sums of a row are the DP / 8 dims of the codes that it read
 #pragma unroll
-                for (uint32_t j = 0; j < NJ; j += 4) {
+                for (uint32_t j = 0; j < NJ; j += 2) {
                     uint32_t d;
-                    if constexpr (DP == 64) d = 8u * (2u * kq + e) + j;
-                    else d = 128u * (j / 16u) + 16u * (kq + 4u * e) + j % 16u;
-                    float4 x;
-                    if constexpr (kSplit)
-                        x = make_float4(acc[j][e] + acc[j][2 + e], acc[j + 1][e] + acc[j + 1][2 + e],
-                                        acc[j + 2][e] + acc[j + 2][2 + e], acc[j + 3][e] + acc[j + 3][2 + e]);
-                    else
-                        x = make_float4(acc[j][2 * r + e], acc[j + 1][2 * r + e], acc[j + 2][2 * r + e],
-                                        acc[j + 3][2 * r + e]);
-                    reinterpret_cast<float4 *>(mine_o)[row * (DP / 4) + ((d / 4) ^ (row & 7u))] = x;
+                    if constexpr (DP == 64) d = 8u * n + 2u * j;
+                    else d = 128u * (j / 8u) + 16u * ((n >> 1) + 4u * (n & 1u)) + 2u * (j % 8u);
+                    reinterpret_cast<float4 *>(mine_o)[row * (DP / 4) + ((d / 4) ^ (row & 7u))] =
+                        make_float4(acc[t][j][r], acc[t][j][2 + r], acc[t][j + 1][r], acc[t][j + 1][2 + r]);
                 }
             }
-        }
         __syncthreads();
         const bool started = first_tile == cur.lo;
         const uint32_t part = 2 * cta + (started ? 1 : 0);
@@ -668,7 +698,7 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const AttnPar
 
 template <RowType T, uint32_t DP, uint32_t MR>
 cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
-    using Shape = AttnShape<DP>;
+    using Shape = AttnShape<DP, MR>;
     const uint32_t elem = T == RowType::kF32 ? 4 : 2;
     AttnParams p{};
     p.c = a.cache;
@@ -722,15 +752,13 @@ template <RowType T, uint32_t MR>
 cudaError_t launch_by_dim(const LaunchCtx &ctx, const PagedAttention &a) {
     if (a.cache.head_dim <= 64) return launch_attention<T, 64, MR>(ctx, a);
     if (a.cache.head_dim <= 128) return launch_attention<T, 128, MR>(ctx, a);
-    return launch_attention<T, 256, MR>(ctx, a);
+    return launch_attention<T, 256, 8>(ctx, a);   // 16 rows' accumulators do not fit the registers
 }
 
 template <RowType T>
 cudaError_t launch_few(const LaunchCtx &ctx, const PagedAttention &a) {
-    if constexpr (T != RowType::kF32) {
-        if (1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > 8) return launch_by_dim<T, 16>(ctx, a);
-    }
-    return launch_by_dim<T, 8>(ctx, a);
+    return 1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > 8 ? launch_by_dim<T, 16>(ctx, a)
+                                                                       : launch_by_dim<T, 8>(ctx, a);
 }
 
 }  // namespace
