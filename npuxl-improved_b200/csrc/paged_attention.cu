@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
         if (ahead_left) {
             const int32_t k0 = ahead.tile * static_cast<int32_t>(kTile) + static_cast<int32_t>(warp * kWarpKeys);
             uint8_t *const dst = ring + slot_in * Shape::kSlot;
-            uint64_t base[2];
+            uint64_t base[2], scale_at[2];
             bool ok[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -251,21 +251,27 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
                 if (live && !ok[i] && lane == 0) record_error(p.err, kErrBadIndex);
                 const uint64_t at = ok[i] ? static_cast<uint64_t>(page_next[i]) * p.c.heads + ahead.h : 0;
                 base[i] = ((at << p.c.page_shift) + (static_cast<uint32_t>(key) & ((1u << p.c.page_shift) - 1u))) * D;
-                if (lane == i)
-                    cp_async_4_zfill(&sh_scale[warp][slot_in][i], p.c.K_scale + at, ok[i]);
-                if (lane == 2 + i)
-                    cp_async_4_zfill(&sh_scale[warp][slot_in][2 + i], p.c.V_scale + at, ok[i]);
+                scale_at[i] = at;
             }
+            if (lane < 4)   // K's of the two groups, then V's
+                cp_async_4_zfill(&sh_scale[warp][slot_in][lane],
+                                 (lane < 2 ? p.c.K_scale : p.c.V_scale) + (lane & 1u ? scale_at[1] : scale_at[0]),
+                                 lane & 1u ? ok[1] : ok[0]);
             constexpr uint32_t kCopies = kWarpKeys / kStep;      // of K, and of V
             if (ok[0] && ok[1] && k0 + static_cast<int32_t>(kWarpKeys) <= ahead.s.len) {
-                if (my_ch_there) {
+                const auto copy = [&](uint32_t row_bytes) {
 #pragma unroll
-                    for (uint32_t q = 0; q < kCopies; ++q) {
-                        const uint64_t src = base[q / (kCopies / 2)] + lane_src + (q % (kCopies / 2)) * kStep * D;
-                        cp_async_16(dst + place(q), p.c.K + src);
-                        cp_async_16(dst + kWarpKeys * DP + place(q), p.c.V + src);
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        const int8_t *const ks = p.c.K + base[i] + lane_src, *const vs = p.c.V + base[i] + lane_src;
+#pragma unroll
+                        for (uint32_t q = 0; q < kCopies / 2; ++q) {
+                            cp_async_16(dst + place(i * (kCopies / 2) + q), ks + q * kStep * row_bytes);
+                            cp_async_16(dst + kWarpKeys * DP + place(i * (kCopies / 2) + q), vs + q * kStep * row_bytes);
+                        }
                     }
-                }
+                };
+                if (D == DP) copy(DP);               // offsets known to the compiler
+                else if (my_ch_there) copy(D);
             } else {
 #pragma unroll 1
                 for (uint32_t q = 0; q < kCopies; ++q) {         // a sequence's last keys
