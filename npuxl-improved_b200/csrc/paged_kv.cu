@@ -9,6 +9,8 @@
 // a run of n rows touches at most floor(n / page_size) + 2 pages, so sequence
 // b's segments can start at floor(cu[b] / page_size) + 2 b, which any CTA can
 // search for; the numbers left over are CTAs that leave at once.
+#include <algorithm>
+
 #include "paged_common.cuh"
 
 namespace vnpu_b200 {
@@ -72,13 +74,24 @@ inline uint64_t segment_items(const PagedCache &c, const PagedBatch &b) {
     return b.max_tokens == 1 ? b.batch : (static_cast<uint64_t>(b.tokens) >> c.page_shift) + 2ull * b.batch;
 }
 
-// cos and sin of `pos` times t 2^-64 turns.  The product is taken modulo one
-// turn (the 64-bit wrap), then rounded to 32 bits: off by 2^-24 of the angle
-// in (-pi, pi] at every position, where a 32-bit position * frequency is off
-// by 2^-24 of the whole angle, 1e-2 at position 1e5.
+// `pos` times t 2^-64 turns in half turns, in [-1, 1).  The product is taken
+// modulo one turn (the 64-bit wrap) and rounded to 32 bits: off by 2^-24 of the
+// angle at every position, where a 32-bit position * frequency is off by 2^-24
+// of the whole angle, 1e-2 at position 1e5.
+__device__ __forceinline__ float half_turns(int32_t pos, uint64_t t) {
+    const uint32_t p = static_cast<uint32_t>(pos);
+    const uint32_t top = p * static_cast<uint32_t>(t >> 32) + __umulhi(p, static_cast<uint32_t>(t));
+    return static_cast<float>(static_cast<int32_t>(top)) * 0x1p-31f;
+}
+// Queries' angles, shared by their heads: sine and cosine to the last places.
 __device__ __forceinline__ void turn_sincos(int32_t pos, uint64_t t, float *sn, float *cs) {
-    const int64_t a = static_cast<int64_t>(static_cast<uint64_t>(static_cast<int64_t>(pos)) * t);
-    sincospif(static_cast<float>(a) * 0x1p-63f, sn, cs);
+    sincospif(half_turns(pos, t), sn, cs);
+}
+// Keys' angles, one for each pair and head: the fast sine and cosine, 2^-21 off
+// at most in (-pi, pi], a ten-thousandth of a code (with the exact ones the
+// prompts' append took 80 us instead of 40).
+__device__ __forceinline__ void turn_sincos_fast(int32_t pos, uint64_t t, float *sn, float *cs) {
+    __sincosf(half_turns(pos, t) * 3.14159265358979f, sn, cs);
 }
 
 // A head's 16 elements of unit u as two groups of 8 and their pairs' first
@@ -145,22 +158,27 @@ __device__ __forceinline__ uint32_t rescaled4(uint32_t w, float ratio) {
     return r;
 }
 
-constexpr uint32_t kQueryRows(uint32_t nt) { return nt / 64; }  // query rows of a CTA
+constexpr uint32_t kQueryRows(uint32_t nt) { return nt / 128; }  // query rows of a CTA
 
-// Grid: segments x heads x {K, V}, then the query rows.  A thread holds up to
-// U units (16 elements each) of its segment in registers between the maximum
-// and the rounding; a segment with more is read again, from L2.
-template <RowType T, uint32_t NT, uint32_t U>
-__global__ void __launch_bounds__(NT) paged_append_kernel(
+// Grid: segments x heads x {K, V}, then the query rows.  A segment of one head
+// is a CTA's work, or, where every sequence has one token, a warp's (kWarp).  A
+// thread holds up to U units (16 elements each) of its segment in registers
+// between the maximum and the rounding; a segment with more is read again,
+// from L2.
+template <RowType T, uint32_t NT, uint32_t U, bool kWarp>
+__global__ void __launch_bounds__(NT, kWarp ? 8 : U == 2 ? 4 : 2) paged_append_kernel(
     const PagedCache c, const PagedBatch pb, const void *Qv, const void *Kv, const void *Vv,
     void *Qov, uint32_t ldq, uint32_t ldk, uint32_t ldv, uint32_t ldqo, uint32_t q_heads,
-    uint32_t rotary, bool interleaved, uint32_t vec, uint32_t kv_ctas, const PagedTurns turns,
-    uint32_t *err) {
+    uint32_t rotary, bool interleaved, uint32_t vec, uint32_t kv_ctas, uint32_t kv_items,
+    const PagedTurns turns, uint32_t *err) {
     using E = typename RowOf<T>::type;
-    pdl_enter();
+    constexpr uint32_t GT = kWarp ? 32 : NT;         // threads of a segment
     __shared__ float2 sh_turn[kQueryRows(NT)][128];
+    __shared__ __align__(16) uint64_t sh_rate[128];  // turns: lanes read different ones
     __shared__ float sh_max[NT / 32];
-    const uint32_t tid = threadIdx.x, D = c.head_dim;
+    const uint32_t tid = threadIdx.x, D = c.head_dim, lane = kWarp ? tid & 31u : tid;
+    if (tid < rotary / 2u) sh_rate[tid] = turns.t[tid];
+    pdl_enter();
 
     if (blockIdx.x >= kv_ctas) {
         // ---- queries: rotate rows r0 .. r0 + kQueryRows - 1, angles shared by the heads
@@ -189,11 +207,12 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(
             }
             pos[i] = s.start + static_cast<int32_t>(r) - s.row0;
         }
+        __syncthreads();
         const uint32_t pairs = rotary / 2u;
 #pragma unroll
         for (uint32_t i = 0; i < kQueryRows(NT); ++i)
             for (uint32_t j = tid; j < pairs; j += NT)
-                turn_sincos(pos[i], turns.t[j], &sh_turn[i][j].y, &sh_turn[i][j].x);
+                turn_sincos(pos[i], sh_rate[j], &sh_turn[i][j].y, &sh_turn[i][j].x);
         __syncthreads();
         const uint32_t per_row = q_heads * (D / 16u);
         const bool vin = vec & 1u, vout = vec & 8u;
@@ -222,12 +241,16 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(
         return;
     }
 
-    const uint32_t item = blockIdx.x / (2u * c.heads);
-    const uint32_t which = blockIdx.x - item * 2u * c.heads;
+    if constexpr (kWarp) __syncthreads();
+    const uint32_t index = kWarp ? blockIdx.x * (NT / 32u) + (tid >> 5) : blockIdx.x;
+    if (index >= kv_items) return;
+    const uint32_t item = index / (2u * c.heads);
+    const uint32_t which = index - item * 2u * c.heads;
     const bool value = which >= c.heads;
     const uint32_t h = value ? which - c.heads : which;
     Segment g;
     if (!find_segment<NT>(c, pb, item, err, g)) return;
+    if constexpr (!kWarp) __syncthreads();           // sh_rate
     const uint32_t ld = value ? ldv : ldk;
     const bool vin = vec & (value ? 4u : 2u);
     const E *in = static_cast<const E *>(value ? Vv : Kv) + static_cast<uint64_t>(g.row0) * ld + h * D;
@@ -250,7 +273,7 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(
         const Unit x = unit_of(k - r * per_row, rot, interleaved);
         if (x.pair >= 0)
             rotate_unit(a, b, interleaved, [&](int e, float *sn, float *cs) {
-                turn_sincos(g.pos0 + static_cast<int32_t>(r), turns.t[x.pair + e], sn, cs);
+                turn_sincos_fast(g.pos0 + static_cast<int32_t>(r), sh_rate[x.pair + e], sn, cs);
             });
     };
     float most = 0.0f;
@@ -265,30 +288,32 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(
     float a[U][8], b[U][8];
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)  // all loads in flight before the first is used
-        if (tid + u * NT < units) fetch(tid + u * NT, a[u], b[u]);
+        if (lane + u * GT < units) fetch(lane + u * GT, a[u], b[u]);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
-        if (tid + u * NT < units) {
-            turn(tid + u * NT, a[u], b[u]);
+        if (lane + u * GT < units) {
+            turn(lane + u * GT, a[u], b[u]);
             widen(a[u], b[u]);
         }
-    for (uint32_t k = tid + U * NT; k < units; k += NT) {
+    for (uint32_t k = lane + U * GT; k < units; k += GT) {
         float x[8], y[8];
         fetch(k, x, y);
         turn(k, x, y);
         widen(x, y);
     }
     most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));  // >= 0
-    if ((tid & 31u) == 0) sh_max[tid >> 5] = most;
-    __syncthreads();
+    if constexpr (!kWarp) {
+        if ((tid & 31u) == 0) sh_max[tid >> 5] = most;
+        __syncthreads();
 #pragma unroll
-    for (uint32_t i = 0; i < NT / 32u; ++i) most = fmaxf(most, sh_max[i]);
+        for (uint32_t i = 0; i < NT / 32u; ++i) most = fmaxf(most, sh_max[i]);
+    }
 
     // A scale below the smallest normal number has no finite reciprocal: such a page is zero.
     const float fresh = __fdiv_rn(most, 127.0f);
     const float now = fmaxf(held, fresh < 1.17549435e-38f ? 0.0f : fresh);
     const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
-    if (tid == 0) *scale = now;
+    if (lane == 0) *scale = now;
     const auto put = [&](uint32_t k, const float (&a)[8], const float (&b)[8]) {
         const uint32_t r = k / per_row;
         const Unit x = unit_of(k - r * per_row, rot, interleaved);
@@ -298,8 +323,8 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(
     };
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
-        if (tid + u * NT < units) put(tid + u * NT, a[u], b[u]);
-    for (uint32_t k = tid + U * NT; k < units; k += NT) {
+        if (lane + u * GT < units) put(lane + u * GT, a[u], b[u]);
+    for (uint32_t k = lane + U * GT; k < units; k += GT) {
         float x[8], y[8];
         fetch(k, x, y);
         turn(k, x, y);
@@ -308,7 +333,7 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(
     if (g.slot0 && now > held) {  // the scale grew: round the page's older codes to it
         const float ratio = __fdiv_rn(held, now);
         uint4 *old = reinterpret_cast<uint4 *>(page);
-        for (uint32_t k = tid; k < static_cast<uint32_t>(g.slot0) * per_row; k += NT) {
+        for (uint32_t k = lane; k < static_cast<uint32_t>(g.slot0) * per_row; k += GT) {
             uint4 w = old[k];
             w.x = rescaled4(w.x, ratio);
             w.y = rescaled4(w.y, ratio);
@@ -319,41 +344,67 @@ __global__ void __launch_bounds__(NT) paged_append_kernel(
     }
 }
 
-// A CTA reads one segment of one head, K and V.
+// A CTA reads one segment of `span` heads, K and V; a thread has 4 units of
+// each in flight.
 template <RowType T, uint32_t NT>
 __global__ void __launch_bounds__(NT) paged_read_kernel(
     const PagedCache c, const PagedBatch pb, void *Kv, void *Vv, uint64_t ld_row, uint64_t ld_head,
-    bool vec, uint32_t *err) {
+    uint32_t span, uint32_t spans, bool vec, uint32_t *err) {
     using E = typename RowOf<T>::type;
     pdl_enter();
-    const uint32_t item = blockIdx.x / c.heads, h = blockIdx.x - item * c.heads;
+    const uint32_t item = blockIdx.x / spans, h0 = (blockIdx.x - item * spans) * span;
     Segment g;
     if (!find_segment<NT>(c, pb, item, err, g)) return;
-    const uint32_t D = c.head_dim, per_row = D / 16u, units = g.n * per_row;
-    const uint64_t at = static_cast<uint64_t>(g.page) * c.heads + h;
-    const uint64_t first = (at << c.page_shift) * D + static_cast<uint32_t>(g.slot0) * D;
-    const uint64_t out0 = static_cast<uint64_t>(g.row0) * ld_row + h * ld_head;
-    const float ks = Kv ? __ldg(c.K_scale + at) : 0.0f, vs = Vv ? __ldg(c.V_scale + at) : 0.0f;
+    const uint32_t D = c.head_dim, per_row = D / 16u, per_head = g.n * per_row;
+    const uint32_t units = min(span, c.heads - h0) * per_head;
+    const uint64_t at0 = static_cast<uint64_t>(g.page) * c.heads + h0;
     const auto put = [&](const uint4 &w, float s, E *out) {
         const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = static_cast<float>(static_cast<int8_t>(word[2 * half + (i >> 2)] >> (8 * (i & 3)))) * s;
+            for (int i = 0; i < 2; ++i) {
+                uint32_t x, y;          // by way of exact 16-bit floats
+                codes_to_half4(word[2 * half + i], x, y);
+                const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+                const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&y));
+                v[4 * i] = lo.x * s;
+                v[4 * i + 1] = lo.y * s;
+                v[4 * i + 2] = hi.x * s;
+                v[4 * i + 3] = hi.y * s;
+            }
             store8(out + 8 * half, vec, v);
         }
     };
-#pragma unroll 2
-    for (uint32_t k = threadIdx.x; k < units; k += NT) {
-        const uint32_t r = k / per_row, d = (k - r * per_row) * 16u;
-        const uint64_t o = out0 + r * ld_row + d;
-        uint4 kw, vw;
-        if (Kv) kw = __ldg(reinterpret_cast<const uint4 *>(c.K + first) + k);
-        if (Vv) vw = __ldg(reinterpret_cast<const uint4 *>(c.V + first) + k);
-        if (Kv) put(kw, ks, static_cast<E *>(Kv) + o);
-        if (Vv) put(vw, vs, static_cast<E *>(Vv) + o);
+    constexpr uint32_t B = 4;
+    for (uint32_t k0 = threadIdx.x; k0 < units; k0 += B * NT) {
+        uint4 kw[B], vw[B];
+        float ks[B], vs[B];
+        uint64_t o[B];
+#pragma unroll
+        for (uint32_t i = 0; i < B; ++i) {
+            const uint32_t k = k0 + i * NT;
+            if (k >= units) continue;
+            const uint32_t h = k / per_head, in_head = k - h * per_head, r = in_head / per_row;
+            const uint64_t at = at0 + h;
+            const uint64_t from = ((at << c.page_shift) + static_cast<uint32_t>(g.slot0)) * D + in_head * 16u;
+            o[i] = (g.row0 + static_cast<uint64_t>(r)) * ld_row + (h0 + h) * ld_head + (in_head - r * per_row) * 16u;
+            if (Kv) {
+                kw[i] = __ldg(reinterpret_cast<const uint4 *>(c.K + from));
+                ks[i] = __ldg(c.K_scale + at);
+            }
+            if (Vv) {
+                vw[i] = __ldg(reinterpret_cast<const uint4 *>(c.V + from));
+                vs[i] = __ldg(c.V_scale + at);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < B; ++i) {
+            if (k0 + i * NT >= units) continue;
+            if (Kv) put(kw[i], ks[i], static_cast<E *>(Kv) + o[i]);
+            if (Vv) put(vw[i], vs[i], static_cast<E *>(Vv) + o[i]);
+        }
     }
 }
 
@@ -380,36 +431,44 @@ cudaError_t paged_kv_append(const LaunchCtx &ctx, const PagedAppend &p) {
                          (aligned16(p.Q_out, 1ull * p.ldqo * elem) ? 8u : 0u);
     PagedTurns turns{};
     for (uint32_t j = 0; j < p.rotary / 2; ++j) turns.t[j] = p.turns[j];
-    const uint64_t kv = segment_items(p.cache, p.batch) * 2 * p.cache.heads;
+    const uint64_t items = segment_items(p.cache, p.batch) * 2 * p.cache.heads;
+    // One token a sequence: a segment is one row, a warp's work (as a CTA's, 64 sequences of 8
+    // heads took 13 us instead of 6).
     const bool single = p.batch.max_tokens == 1;
     const uint32_t nt = single ? 128 : 256, rows = kQueryRows(nt);
+    const uint64_t kv = single ? (items + 3) / 4 : items;
     const uint64_t grid = kv + (p.Q ? (p.batch.tokens + rows - 1) / rows : 0);
-    if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+    if (items > 0x7fffffffull || grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
     // Units a thread holds: a page's worth, at most 4 (64 registers).
     const uint64_t units = (static_cast<uint64_t>(p.cache.head_dim) << p.cache.page_shift) / 16 / 256;
     if (ctx.launch_counter) ++*ctx.launch_counter;
     return by_type(p.type, [&](auto t) -> cudaError_t {
         constexpr RowType T = decltype(t)::value;
-        auto kernel = single ? &paged_append_kernel<T, 128, 1>
-                      : units <= 2 ? &paged_append_kernel<T, 256, 2>
-                                   : &paged_append_kernel<T, 256, 4>;
+        auto kernel = single ? &paged_append_kernel<T, 128, 1, true>
+                      : units <= 2 ? &paged_append_kernel<T, 256, 2, false>
+                                   : &paged_append_kernel<T, 256, 4, false>;
         return launch_pdl(ctx.stream, kernel, dim3(static_cast<uint32_t>(grid)), dim3(nt), 0, p.cache,
                           p.batch, p.Q, p.K, p.V, p.Q_out, p.ldq, p.ldk, p.ldv, p.ldqo, p.q_heads,
-                          p.rotary, p.interleaved, vec, static_cast<uint32_t>(kv), turns, ctx.err);
+                          p.rotary, p.interleaved, vec, static_cast<uint32_t>(kv),
+                          static_cast<uint32_t>(items), turns, ctx.err);
     });
 }
 
 cudaError_t paged_kv_read(const LaunchCtx &ctx, const PagedRead &p) {
     const uint32_t elem = p.type == RowType::kF32 ? 4 : 2;
     const bool vec = aligned16(p.K_out, p.ld_row * elem) && aligned16(p.V_out, p.ld_head * elem);
-    const uint64_t grid = segment_items(p.cache, p.batch) * p.cache.heads;
+    // Heads of a CTA: enough for 4 units of K and of V a thread, where pages are small.
+    const uint32_t in_head = (p.cache.head_dim << p.cache.page_shift) / 16u;
+    const uint32_t span = std::max(1u, std::min(p.cache.heads, 512u / in_head));
+    const uint32_t spans = (p.cache.heads + span - 1) / span;
+    const uint64_t grid = segment_items(p.cache, p.batch) * spans;
     if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
     if (ctx.launch_counter) ++*ctx.launch_counter;
     return by_type(p.type, [&](auto t) -> cudaError_t {
         constexpr RowType T = decltype(t)::value;
         return launch_pdl(ctx.stream, &paged_read_kernel<T, 128>, dim3(static_cast<uint32_t>(grid)),
                           dim3(128), 0, p.cache, p.batch, p.K_out, p.V_out, p.ld_row, p.ld_head,
-                          vec, ctx.err);
+                          span, spans, vec, ctx.err);
     });
 }
 
