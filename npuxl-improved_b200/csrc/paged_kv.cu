@@ -16,6 +16,10 @@
 namespace vnpu_b200 {
 namespace {
 
+// Tables are read 8 entries a lane, from places 8 apart: one entry of room after
+// each 8 keeps lanes off each other's banks.
+__host__ __device__ constexpr uint32_t pad8(uint32_t j) { return j + j / 8u; }
+
 struct PagedTurns {
     uint64_t t[128];
 };
@@ -28,29 +32,62 @@ struct Segment {
     int64_t page;
 };
 
+// The sequence of a rising numbering: the first b with base_after(b) > w, by the
+// whole block, with its numbers.  While batch <= NT the lookup and the numbers
+// are one trip to memory.  False: none, or one with bad numbers (reported).
+template <uint32_t NT, typename F>
+__device__ __forceinline__ bool find_numbers(const PagedCache &c, const PagedBatch &pb, const F &base_after,
+                                             uint64_t w, uint32_t *err, uint32_t &b, PagedSeq &s) {
+    __shared__ PagedSeq sh_seq;
+    __shared__ bool sh_good;
+    bool good = false;
+    if (pb.batch <= NT) {
+        const uint32_t t = threadIdx.x;
+        uint64_t base = ~0ull;
+        if (t < pb.batch) {
+            good = load_seq(pb, c.page_shift, t, s);
+            base = base_after(t);
+        }
+        b = __syncthreads_count(base <= w);
+        if (t == b) {
+            sh_seq = s;
+            sh_good = good;
+        }
+        __syncthreads();
+        if (b >= pb.batch) return false;
+        s = sh_seq;
+        good = sh_good;
+    } else {
+        b = find_seq<NT>(pb.batch, base_after, w);
+        if (b >= pb.batch) return false;
+        good = load_seq(pb, c.page_shift, b, s);
+    }
+    if (!good && threadIdx.x == 0) record_error(err, kErrBadIndex);
+    return good;
+}
+
 // Segment number `item` of the batch; false: no such segment, or a bad one.
+// Its page is as the table gives it: page_there() looks at it.
 template <uint32_t NT>
 __device__ __forceinline__ bool find_segment(const PagedCache &c, const PagedBatch &pb,
                                              uint32_t item, uint32_t *err, Segment &g) {
     uint32_t b, seg = 0;
+    PagedSeq s;
     if (pb.max_tokens == 1) {
         b = item;  // one segment a sequence: item b is sequence b's
+        if (!load_seq(pb, c.page_shift, b, s)) {
+            if (threadIdx.x == 0) record_error(err, kErrBadIndex);
+            return false;
+        }
     } else {
         const auto after = [&](uint32_t i) -> uint64_t {
             const int32_t cu = __ldg(pb.cu + i + 1);
             return (static_cast<uint64_t>(cu < 0 ? 0 : cu) >> c.page_shift) + 2ull * (i + 1);
         };
-        b = find_seq<NT>(pb.batch, after, item);
-        if (b >= pb.batch) return false;
-        const int32_t c0 = __ldg(pb.cu + b);
-        const uint64_t base = (static_cast<uint64_t>(c0 < 0 ? 0 : c0) >> c.page_shift) + 2ull * b;
+        if (!find_numbers<NT>(c, pb, after, item, err, b, s)) return false;
+        const uint64_t base = (static_cast<uint64_t>(s.row0) >> c.page_shift) + 2ull * b;
         if (item < base) return false;  // only where cu falls
         seg = static_cast<uint32_t>(item - base);
-    }
-    PagedSeq s;
-    if (!load_seq(pb, c.page_shift, b, s)) {
-        if (threadIdx.x == 0) record_error(err, kErrBadIndex);
-        return false;
     }
     if (s.n == 0) return false;
     const uint64_t index = (static_cast<uint32_t>(s.start) >> c.page_shift) + static_cast<uint64_t>(seg);
@@ -59,15 +96,16 @@ __device__ __forceinline__ bool find_segment(const PagedCache &c, const PagedBat
     const int64_t lo = max(static_cast<int64_t>(s.start), p0);
     const int64_t hi = min(static_cast<int64_t>(s.len), p0 + (static_cast<int64_t>(1) << c.page_shift));
     g.page = __ldg(pb.table + static_cast<uint64_t>(b) * pb.table_stride + index);
-    if (g.page < 0 || g.page >= c.num_pages) {
-        if (threadIdx.x == 0) record_error(err, kErrBadIndex);
-        return false;
-    }
     g.row0 = s.row0 + static_cast<int32_t>(lo - s.start);
     g.n = static_cast<int32_t>(hi - lo);
     g.slot0 = static_cast<int32_t>(lo - p0);
     g.pos0 = static_cast<int32_t>(lo);
     return true;
+}
+__device__ __forceinline__ bool page_there(const PagedCache &c, const Segment &g, uint32_t *err) {
+    const bool there = g.page >= 0 && g.page < c.num_pages;
+    if (!there && threadIdx.x == 0) record_error(err, kErrBadIndex);
+    return there;
 }
 
 inline uint64_t segment_items(const PagedCache &c, const PagedBatch &b) {
@@ -146,6 +184,19 @@ __device__ __forceinline__ uint32_t code_of(float x, float inv) {
     const int q = __float2int_rn(__fmul_rn(x, inv));
     return static_cast<uint32_t>(max(-127, min(127, q))) & 0xffu;
 }
+// Codes of 4 finite values: adding 1.5 * 2^23 leaves the nearest whole number
+// (ties to even) in the low bits, two's complement, in one instruction a value.
+__device__ __forceinline__ uint32_t codes4_finite(const float *v, float inv) {
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fmaf_rn(v[i], inv, 12582912.0f));
+    return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 __device__ __forceinline__ uint32_t codes4(const float *v, float inv) {
     return code_of(v[0], inv) | (code_of(v[1], inv) << 8) | (code_of(v[2], inv) << 16) |
            (code_of(v[3], inv) << 24);
@@ -158,7 +209,7 @@ __device__ __forceinline__ uint32_t rescaled4(uint32_t w, float ratio) {
     return r;
 }
 
-constexpr uint32_t kQueryRows(uint32_t nt) { return nt / 128; }  // query rows of a CTA
+constexpr uint32_t kQueryRows(uint32_t nt) { return nt == 128 ? 1 : 4; }  // query rows of a CTA
 
 // Grid: segments x heads x {K, V}, then the query rows.  A segment of one head
 // is a CTA's work, or, where every sequence has one token, a warp's (kWarp).  A
@@ -166,76 +217,85 @@ constexpr uint32_t kQueryRows(uint32_t nt) { return nt / 128; }  // query rows o
 // between the maximum and the rounding; a segment with more is read again,
 // from L2.
 template <RowType T, uint32_t NT, uint32_t U, bool kWarp>
-__global__ void __launch_bounds__(NT, kWarp ? 8 : U == 2 ? 4 : 2) paged_append_kernel(
+__global__ void __launch_bounds__(NT, kWarp ? 6 : U == 2 ? 3 : 2) paged_append_kernel(
     const PagedCache c, const PagedBatch pb, const void *Qv, const void *Kv, const void *Vv,
     void *Qov, uint32_t ldq, uint32_t ldk, uint32_t ldv, uint32_t ldqo, uint32_t q_heads,
     uint32_t rotary, bool interleaved, uint32_t vec, uint32_t kv_ctas, uint32_t kv_items,
     const PagedTurns turns, uint32_t *err) {
     using E = typename RowOf<T>::type;
     constexpr uint32_t GT = kWarp ? 32 : NT;         // threads of a segment
-    __shared__ float2 sh_turn[kQueryRows(NT)][128];
-    __shared__ __align__(16) uint64_t sh_rate[128];  // turns: lanes read different ones
-    __shared__ float sh_max[NT / 32];
+    __shared__ float2 sh_turn[kQueryRows(NT)][pad8(128)];
+    __shared__ uint64_t sh_rate[pad8(128)];          // turns: lanes read different ones
+    __shared__ uint32_t sh_max[NT / 32];
     const uint32_t tid = threadIdx.x, D = c.head_dim, lane = kWarp ? tid & 31u : tid;
-    if (tid < rotary / 2u) sh_rate[tid] = turns.t[tid];
+    if (tid < rotary / 2u) sh_rate[pad8(tid)] = turns.t[tid];
     pdl_enter();
 
     if (blockIdx.x >= kv_ctas) {
         // ---- queries: rotate rows r0 .. r0 + kQueryRows - 1, angles shared by the heads
         const uint32_t r0 = (blockIdx.x - kv_ctas) * kQueryRows(NT);
         int32_t pos[kQueryRows(NT)];
+        PagedSeq s;                 // of the row before, mostly this one's too
+        s.n = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kQueryRows(NT); ++i) {
-            const uint32_t r = r0 + i;
+        for (uint32_t i = 0; i < kQueryRows(NT); ++i) {   // block-uniform
+            const int32_t r = static_cast<int32_t>(r0 + i);
             pos[i] = -1;
-            if (r >= pb.tokens) continue;
-            // the row's sequence: row b itself when every sequence has one
-            uint32_t b = r;
-            const bool own = r < pb.batch && __ldg(pb.cu + r) == static_cast<int32_t>(r) &&
-                             __ldg(pb.cu + r + 1) == static_cast<int32_t>(r) + 1;
-            if (!own)  // block-uniform
-                b = find_seq<NT>(pb.batch, [&](uint32_t j) -> uint64_t {
+            if (r0 + i >= pb.tokens) continue;
+            bool good = s.n != 0 && r < s.row0 + s.n;
+            if (!good && kWarp) {   // row b is sequence b's when every sequence has one
+                good = r0 + i < pb.batch && load_seq(pb, c.page_shift, r0 + i, s) && s.row0 == r && s.n == 1;
+            }
+            if (!good) {
+                uint32_t b;
+                const auto after = [&](uint32_t j) -> uint64_t {
                     const int32_t cu = __ldg(pb.cu + j + 1);
                     return cu < 0 ? 0u : static_cast<uint64_t>(cu);
-                }, r);
-            if (b >= pb.batch) continue;  // a row of no sequence
-            PagedSeq s;
-            if (!load_seq(pb, c.page_shift, b, s) || static_cast<int32_t>(r) < s.row0 ||
-                static_cast<int32_t>(r) >= s.row0 + s.n) {
-                if (tid == 0) record_error(err, kErrBadIndex);
-                continue;
+                };
+                good = find_numbers<NT>(c, pb, after, r0 + i, err, b, s);
+                if (!good || r < s.row0 || r >= s.row0 + s.n) {   // a row of no sequence, or of a bad one
+                    s.n = 0;
+                    continue;
+                }
             }
-            pos[i] = s.start + static_cast<int32_t>(r) - s.row0;
+            pos[i] = s.start + r - s.row0;
         }
         __syncthreads();
         const uint32_t pairs = rotary / 2u;
 #pragma unroll
         for (uint32_t i = 0; i < kQueryRows(NT); ++i)
             for (uint32_t j = tid; j < pairs; j += NT)
-                turn_sincos(pos[i], sh_rate[j], &sh_turn[i][j].y, &sh_turn[i][j].x);
+                turn_sincos(pos[i], sh_rate[pad8(j)], &sh_turn[i][pad8(j)].y, &sh_turn[i][pad8(j)].x);
         __syncthreads();
         const uint32_t per_row = q_heads * (D / 16u);
         const bool vin = vec & 1u, vout = vec & 8u;
+        for (uint32_t k = tid; k < per_row; k += NT) {
+            const uint32_t h = k / (D / 16u);
+            const Unit x = unit_of(k - h * (D / 16u), rotary, interleaved);
+            constexpr uint32_t F = kQueryRows(NT) < 2 ? 1 : 2;    // rows in flight
 #pragma unroll
-        for (uint32_t i = 0; i < kQueryRows(NT); ++i) {
-            if (pos[i] < 0) continue;
-            const E *in = static_cast<const E *>(Qv) + static_cast<uint64_t>(r0 + i) * ldq;
-            E *out = static_cast<E *>(Qov) + static_cast<uint64_t>(r0 + i) * ldqo;
-#pragma unroll 2
-            for (uint32_t k = tid; k < per_row; k += NT) {
-                const uint32_t h = k / (D / 16u);
-                const Unit x = unit_of(k - h * (D / 16u), rotary, interleaved);
-                float a[8], b[8];
-                load8(in + h * D + x.o0, vin, a);
-                load8(in + h * D + x.o1, vin, b);
-                if (x.pair >= 0)
-                    rotate_unit(a, b, interleaved, [&](int e, float *sn, float *cs) {
-                        const float2 t = sh_turn[i][x.pair + e];
-                        *cs = t.x;
-                        *sn = t.y;
-                    });
-                store8(out + h * D + x.o0, vout, a);
-                store8(out + h * D + x.o1, vout, b);
+            for (uint32_t i0 = 0; i0 < kQueryRows(NT); i0 += F) {
+                float a[F][8], b[F][8];
+#pragma unroll
+                for (uint32_t i = 0; i < F; ++i) {
+                    if (pos[i0 + i] < 0) continue;
+                    const E *in = static_cast<const E *>(Qv) + static_cast<uint64_t>(r0 + i0 + i) * ldq + h * D;
+                    load8(in + x.o0, vin, a[i]);
+                    load8(in + x.o1, vin, b[i]);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < F; ++i) {
+                    if (pos[i0 + i] < 0) continue;
+                    E *out = static_cast<E *>(Qov) + static_cast<uint64_t>(r0 + i0 + i) * ldqo + h * D;
+                    if (x.pair >= 0)
+                        rotate_unit(a[i], b[i], interleaved, [&](int e, float *sn, float *cs) {
+                            const float2 t = sh_turn[i0 + i][pad8(x.pair) + e];
+                            *cs = t.x;
+                            *sn = t.y;
+                        });
+                    store8(out + x.o0, vout, a[i]);
+                    store8(out + x.o1, vout, b[i]);
+                }
             }
         }
         return;
@@ -254,77 +314,119 @@ __global__ void __launch_bounds__(NT, kWarp ? 8 : U == 2 ? 4 : 2) paged_append_k
     const uint32_t ld = value ? ldv : ldk;
     const bool vin = vec & (value ? 4u : 2u);
     const E *in = static_cast<const E *>(value ? Vv : Kv) + static_cast<uint64_t>(g.row0) * ld + h * D;
-    const uint64_t at = static_cast<uint64_t>(g.page) * c.heads + h;
-    int8_t *page = (value ? c.V : c.K) + ((at << c.page_shift) * D);
-    float *scale = (value ? c.V_scale : c.K_scale) + at;
-    const float held = g.slot0 ? *scale : 0.0f;
     const uint32_t rot = value ? 0u : rotary;
-    const uint32_t per_row = D / 16u, units = g.n * per_row;
-
-    const auto fetch = [&](uint32_t k, float (&a)[8], float (&b)[8]) {
-        const uint32_t r = k / per_row;
-        const Unit x = unit_of(k - r * per_row, rot, interleaved);
-        const E *row = in + static_cast<uint64_t>(r) * ld;
+    // This thread's units: row and place in the row, GT units on from one to the next.
+    const uint32_t per_row = D / 16u, rows = static_cast<uint32_t>(g.n);
+    struct Place {
+        uint32_t r, u;
+    };
+    Place p0;
+    p0.r = lane / per_row;
+    p0.u = lane - p0.r * per_row;
+    const uint32_t dr = GT / per_row, du = GT - dr * per_row;
+    const auto next = [&](Place x) {
+        x.r += dr;
+        x.u += du;
+        if (x.u >= per_row) {
+            x.u -= per_row;
+            ++x.r;
+        }
+        return x;
+    };
+    const auto fetch = [&](const Place &at, float (&a)[8], float (&b)[8]) {
+        const Unit x = unit_of(at.u, rot, interleaved);
+        const E *row = in + static_cast<uint64_t>(at.r) * ld;
         load8(row + x.o0, vin, a);
         load8(row + x.o1, vin, b);
     };
-    const auto turn = [&](uint32_t k, float (&a)[8], float (&b)[8]) {
-        const uint32_t r = k / per_row;
-        const Unit x = unit_of(k - r * per_row, rot, interleaved);
+    const auto turn = [&](const Place &at, float (&a)[8], float (&b)[8]) {
+        const Unit x = unit_of(at.u, rot, interleaved);
         if (x.pair >= 0)
             rotate_unit(a, b, interleaved, [&](int e, float *sn, float *cs) {
-                turn_sincos_fast(g.pos0 + static_cast<int32_t>(r), sh_rate[x.pair + e], sn, cs);
+                turn_sincos_fast(g.pos0 + static_cast<int32_t>(at.r), sh_rate[pad8(x.pair) + e], sn, cs);
             });
     };
     float most = 0.0f;
     const auto widen = [&](const float (&a)[8], const float (&b)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = fabsf(a[i]), y = fabsf(b[i]);
-            if (x <= 3.402823466e38f) most = fmaxf(most, x);  // NaN and infinity do not count
-            if (y <= 3.402823466e38f) most = fmaxf(most, y);
-        }
+        for (int i = 0; i < 8; ++i) most = max_nan(most, max_nan(fabsf(a[i]), fabsf(b[i])));
     };
+    Place at[U];
     float a[U][8], b[U][8];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u)  // all loads in flight before the first is used
-        if (lane + u * GT < units) fetch(lane + u * GT, a[u], b[u]);
+    for (uint32_t u = 0; u < U; ++u) {  // all loads in flight before the first is used
+        at[u] = u ? next(at[u - 1]) : p0;
+        if (at[u].r < rows) fetch(at[u], a[u], b[u]);
+    }
+    if (!page_there(c, g, err)) return;
+    const uint64_t head = static_cast<uint64_t>(g.page) * c.heads + h;
+    int8_t *page = (value ? c.V : c.K) + ((head << c.page_shift) * D);
+    float *scale = (value ? c.V_scale : c.K_scale) + head;
+    const float held = g.slot0 ? *scale : 0.0f;
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
-        if (lane + u * GT < units) {
-            turn(lane + u * GT, a[u], b[u]);
+        if (at[u].r < rows) {
+            turn(at[u], a[u], b[u]);
             widen(a[u], b[u]);
         }
-    for (uint32_t k = lane + U * GT; k < units; k += GT) {
+    const Place rest = next(at[U - 1]);
+    for (Place k = rest; k.r < rows; k = next(k)) {
         float x[8], y[8];
         fetch(k, x, y);
         turn(k, x, y);
         widen(x, y);
     }
-    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));  // >= 0
+    // the bits of |x| rise with it, infinity and NaN last
+    uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
     if constexpr (!kWarp) {
-        if ((tid & 31u) == 0) sh_max[tid >> 5] = most;
+        if ((tid & 31u) == 0) sh_max[tid >> 5] = bits;
         __syncthreads();
 #pragma unroll
-        for (uint32_t i = 0; i < NT / 32u; ++i) most = fmaxf(most, sh_max[i]);
+        for (uint32_t i = 0; i < NT / 32u; ++i) bits = max(bits, sh_max[i]);
+    }
+    const bool finite = bits < 0x7f800000u;
+    if (!finite) {   // once more, without what is not finite
+        if constexpr (!kWarp) __syncthreads();
+        most = 0.0f;
+        for (Place k = p0; k.r < rows; k = next(k)) {
+            float x[8], y[8];
+            fetch(k, x, y);
+            turn(k, x, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (fabsf(x[i]) <= 3.402823466e38f) most = fmaxf(most, fabsf(x[i]));
+                if (fabsf(y[i]) <= 3.402823466e38f) most = fmaxf(most, fabsf(y[i]));
+            }
+        }
+        bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+        if constexpr (!kWarp) {
+            if ((tid & 31u) == 0) sh_max[tid >> 5] = bits;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < NT / 32u; ++i) bits = max(bits, sh_max[i]);
+        }
     }
 
     // A scale below the smallest normal number has no finite reciprocal: such a page is zero.
-    const float fresh = __fdiv_rn(most, 127.0f);
+    const float fresh = __fdiv_rn(__uint_as_float(bits), 127.0f);
     const float now = fmaxf(held, fresh < 1.17549435e-38f ? 0.0f : fresh);
     const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
     if (lane == 0) *scale = now;
-    const auto put = [&](uint32_t k, const float (&a)[8], const float (&b)[8]) {
-        const uint32_t r = k / per_row;
-        const Unit x = unit_of(k - r * per_row, rot, interleaved);
-        int8_t *row = page + static_cast<uint32_t>(g.slot0 + r) * D;
-        *reinterpret_cast<uint2 *>(row + x.o0) = make_uint2(codes4(a, inv), codes4(a + 4, inv));
-        *reinterpret_cast<uint2 *>(row + x.o1) = make_uint2(codes4(b, inv), codes4(b + 4, inv));
+    const auto put = [&](const Place &k, const float (&a)[8], const float (&b)[8]) {
+        const Unit x = unit_of(k.u, rot, interleaved);
+        int8_t *row = page + static_cast<uint32_t>(g.slot0 + k.r) * D;
+        if (finite) {
+            *reinterpret_cast<uint2 *>(row + x.o0) = make_uint2(codes4_finite(a, inv), codes4_finite(a + 4, inv));
+            *reinterpret_cast<uint2 *>(row + x.o1) = make_uint2(codes4_finite(b, inv), codes4_finite(b + 4, inv));
+        } else {
+            *reinterpret_cast<uint2 *>(row + x.o0) = make_uint2(codes4(a, inv), codes4(a + 4, inv));
+            *reinterpret_cast<uint2 *>(row + x.o1) = make_uint2(codes4(b, inv), codes4(b + 4, inv));
+        }
     };
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
-        if (lane + u * GT < units) put(lane + u * GT, a[u], b[u]);
-    for (uint32_t k = lane + U * GT; k < units; k += GT) {
+        if (at[u].r < rows) put(at[u], a[u], b[u]);
+    for (Place k = rest; k.r < rows; k = next(k)) {
         float x[8], y[8];
         fetch(k, x, y);
         turn(k, x, y);
@@ -344,17 +446,21 @@ __global__ void __launch_bounds__(NT, kWarp ? 8 : U == 2 ? 4 : 2) paged_append_k
     }
 }
 
-// A CTA reads one segment of `span` heads, K and V; a thread has 4 units of
-// each in flight.
+// A CTA reads one segment of `span` heads, of K or of V; a thread has 4 units
+// in flight.
 template <RowType T, uint32_t NT>
-__global__ void __launch_bounds__(NT) paged_read_kernel(
-    const PagedCache c, const PagedBatch pb, void *Kv, void *Vv, uint64_t ld_row, uint64_t ld_head,
-    uint32_t span, uint32_t spans, bool vec, uint32_t *err) {
+__global__ void __launch_bounds__(NT, 10) paged_read_kernel(
+    const PagedCache c, const PagedBatch pb, void *first, void *second, uint64_t ld_row,
+    uint64_t ld_head, uint32_t span, uint32_t spans, bool vec, bool swap, uint32_t *err) {
     using E = typename RowOf<T>::type;
     pdl_enter();
     const uint32_t item = blockIdx.x / spans, h0 = (blockIdx.x - item * spans) * span;
     Segment g;
-    if (!find_segment<NT>(c, pb, item, err, g)) return;
+    if (!find_segment<NT>(c, pb, item, err, g) || !page_there(c, g, err)) return;
+    const bool value = (blockIdx.y != 0) != swap;
+    E *const out0 = static_cast<E *>(blockIdx.y ? second : first);
+    const int8_t *const pool = value ? c.V : c.K;
+    const float *const scales = value ? c.V_scale : c.K_scale;
     const uint32_t D = c.head_dim, per_row = D / 16u, per_head = g.n * per_row;
     const uint32_t units = min(span, c.heads - h0) * per_head;
     const uint64_t at0 = static_cast<uint64_t>(g.page) * c.heads + h0;
@@ -379,32 +485,23 @@ __global__ void __launch_bounds__(NT) paged_read_kernel(
     };
     constexpr uint32_t B = 4;
     for (uint32_t k0 = threadIdx.x; k0 < units; k0 += B * NT) {
-        uint4 kw[B], vw[B];
-        float ks[B], vs[B];
-        uint64_t o[B];
+        uint4 w[B];
+        float sc[B];
+        E *out[B];
 #pragma unroll
         for (uint32_t i = 0; i < B; ++i) {
             const uint32_t k = k0 + i * NT;
             if (k >= units) continue;
             const uint32_t h = k / per_head, in_head = k - h * per_head, r = in_head / per_row;
             const uint64_t at = at0 + h;
-            const uint64_t from = ((at << c.page_shift) + static_cast<uint32_t>(g.slot0)) * D + in_head * 16u;
-            o[i] = (g.row0 + static_cast<uint64_t>(r)) * ld_row + (h0 + h) * ld_head + (in_head - r * per_row) * 16u;
-            if (Kv) {
-                kw[i] = __ldg(reinterpret_cast<const uint4 *>(c.K + from));
-                ks[i] = __ldg(c.K_scale + at);
-            }
-            if (Vv) {
-                vw[i] = __ldg(reinterpret_cast<const uint4 *>(c.V + from));
-                vs[i] = __ldg(c.V_scale + at);
-            }
+            w[i] = __ldg(reinterpret_cast<const uint4 *>(
+                pool + ((at << c.page_shift) + static_cast<uint32_t>(g.slot0)) * D + in_head * 16u));
+            sc[i] = __ldg(scales + at);
+            out[i] = out0 + (g.row0 + static_cast<uint64_t>(r)) * ld_row + (h0 + h) * ld_head + (in_head - r * per_row) * 16u;
         }
 #pragma unroll
-        for (uint32_t i = 0; i < B; ++i) {
-            if (k0 + i * NT >= units) continue;
-            if (Kv) put(kw[i], ks[i], static_cast<E *>(Kv) + o[i]);
-            if (Vv) put(vw[i], vs[i], static_cast<E *>(Vv) + o[i]);
-        }
+        for (uint32_t i = 0; i < B; ++i)
+            if (k0 + i * NT < units) put(w[i], sc[i], out[i]);
     }
 }
 
@@ -457,7 +554,7 @@ cudaError_t paged_kv_append(const LaunchCtx &ctx, const PagedAppend &p) {
 cudaError_t paged_kv_read(const LaunchCtx &ctx, const PagedRead &p) {
     const uint32_t elem = p.type == RowType::kF32 ? 4 : 2;
     const bool vec = aligned16(p.K_out, p.ld_row * elem) && aligned16(p.V_out, p.ld_head * elem);
-    // Heads of a CTA: enough for 4 units of K and of V a thread, where pages are small.
+    // Heads of a CTA: enough for 4 units a thread, where pages are small.
     const uint32_t in_head = (p.cache.head_dim << p.cache.page_shift) / 16u;
     const uint32_t span = std::max(1u, std::min(p.cache.heads, 512u / in_head));
     const uint32_t spans = (p.cache.heads + span - 1) / span;
@@ -466,9 +563,12 @@ cudaError_t paged_kv_read(const LaunchCtx &ctx, const PagedRead &p) {
     if (ctx.launch_counter) ++*ctx.launch_counter;
     return by_type(p.type, [&](auto t) -> cudaError_t {
         constexpr RowType T = decltype(t)::value;
-        return launch_pdl(ctx.stream, &paged_read_kernel<T, 128>, dim3(static_cast<uint32_t>(grid)),
-                          dim3(128), 0, p.cache, p.batch, p.K_out, p.V_out, p.ld_row, p.ld_head,
-                          span, spans, vec, ctx.err);
+        // K, then V; or the one of them that is wanted
+        void *const first = p.K_out ? p.K_out : p.V_out;
+        return launch_pdl(ctx.stream, &paged_read_kernel<T, 128>,
+                          dim3(static_cast<uint32_t>(grid), p.K_out && p.V_out ? 2 : 1), dim3(128), 0, p.cache,
+                          p.batch, first, p.V_out, p.ld_row, p.ld_head, span, spans, vec, p.K_out == nullptr,
+                          ctx.err);
     });
 }
 
