@@ -947,7 +947,7 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     if (e == cudaSuccess)
         e = launch_pdl(ctx.stream, &paged_prefill_kernel<T, DP>, dim3(grid), dim3(kManyThreads), Shape::kSmem, p, plan);
     if (e == cudaSuccess)
-        e = launch_pdl(ctx.stream, &paged_prefill_join_kernel<T, DP>, dim3(grid, 8), dim3(256), 0, p);
+        e = launch_pdl(ctx.stream, &paged_prefill_join_kernel<T, DP>, dim3(grid, kRows * DP / 4 / 256), dim3(256), 0, p);
     const cudaError_t f = cudaFreeAsync(ws, ctx.stream);
     return e == cudaSuccess ? f : e;
 }
