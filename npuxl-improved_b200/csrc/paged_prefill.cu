@@ -4,8 +4,8 @@
 // The mathematics is paged_attention.cu's.  A CTA, one an SM, works on 256 query
 // rows of one key/value head (tokens x grouped heads, packed) and walks their
 // keys in tiles of KT.  Its warps:
-//   17      copies a tile's codes to shared memory (bulk copies, half a tile at a
-//           time) and its page scales beside them, ahead of their use;
+//   17, 18  copy a tile's codes of K and of V to shared memory (bulk copies, half a
+//           tile at a time) and its page scales beside them, ahead of their use;
 //   8-15    turn the codes into f16 (exact), in the swizzled layout of the
 //           tensor core's operands, four warps the first halves of the tiles
 //           and four the second;
@@ -36,7 +36,7 @@ namespace {
 
 constexpr uint32_t kHalf = 128;              // rows of one accumulator (UMMA M)
 constexpr uint32_t kRows = 2 * kHalf;        // query rows of a block
-constexpr uint32_t kManyThreads = 640;       // 8 softmax, 8 converter, tensor-issue, copy and 2 spare warps
+constexpr uint32_t kManyThreads = 640;       // 8 softmax, 8 converter, tensor-issue, 2 copy, a spare warp
 constexpr uint32_t kScaleRing = 4;           // tiles whose scales are kept
 constexpr uint32_t kRawRing = 4;             // half tiles of codes on their way or in conversion
 constexpr uint32_t kPlanThreads = 1024;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
 
     // The block's 640 x 96 registers go where they are needed: 256 x 152 + 384 x 56.  (The spare
-    // warps make up the fifth warpgroup, so that every scheduler's share adds up, too.)
+    // warp makes up the fifth warpgroup, so that every scheduler's share adds up, too.)
     if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
 
@@ -744,10 +744,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 }
             }
         }
-    } else if (busy && warp == 17) {
+    } else if (busy && (warp == 17 || warp == 18)) {
         // =============================== copies ===============================
-        // Lane g takes group g of 16 keys.  A tile's pages are looked up two tiles before its
-        // codes are copied, and its scales read one tile before, so that neither is waited for.
+        // Warp 17 copies K, and gives the scales; warp 18 copies V.  Lane g looks after group g of
+        // 16 keys.  A tile's pages are looked up two tiles before its codes are copied, and its
+        // scales read one tile before, so that neither is waited for.
+        const bool values_too = warp == 18;
+        const int8_t *const pool = values_too ? p.c.V : p.c.K;
         struct Group {
             int32_t page;       // -1: not there
             uint32_t h, slot;   // head; slot of its first key in the page
@@ -780,6 +783,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 return;
             }
             const uint64_t at = static_cast<uint64_t>(g.page) * p.c.heads + g.h;
+            if (values_too) return;
             g.ks = __ldg(p.c.K_scale + at);
             g.vs = __ldg(p.c.V_scale + at);
         };
@@ -791,7 +795,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         look_up(next);
         look_up(later);
         read_scales(next);
-        uint32_t begun = 0;     // half tiles whose copies were begun
+        uint32_t begun = 0;     // tiles whose copies were begun
         bool ok = true;
         for (uint32_t it = 0; it < tiles; ++it) {
             now = next;
@@ -807,21 +811,27 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const uint64_t src = ((at << p.c.page_shift) + now.slot) * D;
             const uint32_t zeros = __ballot_sync(0xffffffffu, lane < kGroups && !(now.vs > 0.0f));
 #pragma unroll 1
-            for (uint32_t part = 0; part < 4; ++part) {      // K in two halves, V in two
-                constexpr uint32_t kPart = kGroups / 2;      // groups of a half
-                const uint32_t x = 4 * it + part, slot = x % kRawRing, first = (part & 1u) * kPart;
-                // A half tile is copied when its place's last one is converted.  K's first half:
+            for (uint32_t part = 0; part < 2; ++part) {
+                constexpr uint32_t kPart = kGroups / 2;      // groups of half a tile
+                const uint32_t slot = 2 * values_too + part, first = part * kPart;
+                // Half a tile is copied when its place's last one is converted.  K's first half:
                 // K of tile it - 1 is then, so the scores of tile it - 3 are there (two tiles of K
                 // are kept), and so the weights of tile it - 4: its scales' place is free, too.
-                if (x >= kRawRing && !(ok = wait_warp(&bar_r_free[slot], x / kRawRing - 1))) break;
-                if (lane == first)
+                if (it && !(ok = wait_warp(&bar_r_free[slot], it - 1))) break;
+                if (lane == 0)
                     mbar_arrive_expect_tx(&bar_r[slot], 16u * D * __popc(there >> first & ((1u << kPart) - 1u)));
-                // one copy for the groups of a page: by the lane of its first one in this half
-                if (now.page >= 0 && lane >= first && lane < first + kPart && (lane - first) % per_copy == 0)
-                    bulk_load_1d(raw + slot * Shape::kRawBytes + (lane - first) * 16u * D,
-                                 (part < 2 ? p.c.K : p.c.V) + src,
-                                 16u * D * __popc(there >> lane & ((1u << per_copy) - 1u)), &bar_r[slot]);
-                if (part == 0) {
+                begun = it + 1;
+                // one copy for the groups of a page, issued warp-uniformly (a branch of the lanes
+                // that own them took 300 clocks)
+#pragma unroll 1
+                for (uint32_t g = first; g < first + kPart; g += per_copy) {
+                    const uint32_t n = __popc(there >> g & ((1u << per_copy) - 1u));
+                    const uint64_t from = __shfl_sync(0xffffffffu, src, g);
+                    if (n && lane == 0)
+                        bulk_load_1d(raw + slot * Shape::kRawBytes + (g - first) * 16u * D, pool + from, 16u * D * n,
+                                     &bar_r[slot]);
+                }
+                if (part == 0 && !values_too) {
                     if (lane < kGroups) {
                         const float lv = now.vs > 0.0f ? __log2f(now.vs) : 0.0f;   // a page of zeros has the scale 0
                         sh_k[ring][lane] = now.ks;
@@ -832,14 +842,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bar_sc[ring]);
                 }
-                begun = x + 1;
             }
             if (!ok) break;
         }
         // a run that was given up may leave copies in flight: they end before the block does
-        if (!ok)
-            for (uint32_t x = begun > kRawRing ? begun - kRawRing : 0; x < begun; ++x)
-                mbar_wait(&bar_r[x % kRawRing], (x / kRawRing) & 1u, p.limit_ns, nullptr, nullptr);
+        if (!ok && begun)
+            for (uint32_t part = 0; part < 2; ++part) {
+                const uint32_t slot = 2 * values_too + part;
+                if (begun > 1) mbar_wait(&bar_r[slot], begun & 1u, p.limit_ns, nullptr, nullptr);
+                mbar_wait(&bar_r[slot], (begun - 1) & 1u, p.limit_ns, nullptr, nullptr);
+            }
     }
     __syncthreads();
     if (warp == 16) {
