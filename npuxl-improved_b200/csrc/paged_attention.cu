@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     __shared__ float sh_scale[kWarps][S][4];       // K_scale and V_scale of a unit's 16-key groups
     __shared__ float2 sh_ml[kWarps][16];
     __shared__ unsigned long long sh_sum[kWarps];
-    __shared__ uint32_t sh_b;
+    __shared__ Cursor sh_cursor;
     __shared__ unsigned long long sh_off;
     pdl_enter();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, n = lane >> 2, kq = lane & 3u;
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
             seq_units<MR>(p, b, cur, &bad);
             const unsigned long long w = static_cast<unsigned long long>(cur.rts) * p.c.heads * cur.nt;
             if (t0 < before + w) {
-                sh_b = b;
+                sh_cursor = cur;
                 sh_off = t0 - before;
                 break;
             }
@@ -189,8 +189,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     }
     __syncthreads();
     {
-        bool bad;
-        seq_units<MR>(p, sh_b, cur, &bad);
+        cur = sh_cursor;
         const unsigned long long off = sh_off;
         const unsigned long long nt = static_cast<uint32_t>(cur.nt), row_tile = off / nt;
         cur.h = static_cast<uint32_t>(row_tile / cur.rts);
@@ -307,37 +306,50 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     float m[NT][2], l[NT][2], qf[NT][2], q_bias[NT][2];
     int32_t kmin[NT][2], kmax[NT][2], kmin_last = 0, kmax_first = 0, kmin_first = 0, kmax_last = 0;
     int32_t first_tile = 0;
+    // The queries of the next row tile, read while the one before is written.
+    alignas(16) E next_q[NT][NG][16];
+    const auto read_rows = [&](const Cursor &k) {
+        const uint32_t rows = static_cast<uint32_t>(k.s.n) * p.group;
+#pragma unroll
+        for (uint32_t t = 0; t < NT; ++t) {
+            const uint32_t r = k.rt * MR + 8 * t + n;       // the row of this lane's fragment
+            const uint32_t token = r / p.group;
+            const E *q = static_cast<const E *>(p.Q) +
+                         static_cast<uint64_t>(k.s.row0 + static_cast<int32_t>(token)) * p.ldq +
+                         (k.h * p.group + (r - token * p.group)) * D;
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g) {
+                const uint32_t d = 16u * (kq + 4u * g);
+                uint4 *v = reinterpret_cast<uint4 *>(next_q[t][g]);
+                constexpr uint32_t NW = sizeof(E);          // 16-byte pieces of 16 elements
+#pragma unroll
+                for (uint32_t i = 0; i < NW; ++i) v[i] = make_uint4(0, 0, 0, 0);
+                if (r >= rows || d >= D) continue;
+                if (p.vec & 1u) {
+#pragma unroll
+                    for (uint32_t i = 0; i < NW; ++i) v[i] = __ldg(reinterpret_cast<const uint4 *>(q + d) + i);
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 16; ++e) next_q[t][g][e] = q[d + e];
+                }
+            }
+        }
+    };
     const auto begin_rows = [&]() {
         first_tile = cur.tile;
-        const uint32_t rows = static_cast<uint32_t>(cur.s.n) * p.group;
         row_limits(p, cur.s, cur.rt * MR, kmin_first, kmax_first);
         row_limits(p, cur.s, cur.rt * MR + MR - 1, kmin_last, kmax_last);
 #pragma unroll
         for (uint32_t t = 0; t < NT; ++t) {
-            const uint32_t r = cur.rt * MR + 8 * t + n;     // the row of this lane's fragment
             float v[NG][16];
             float most = 0.0f;
-            const uint32_t token = r / p.group;
-            const E *q = static_cast<const E *>(p.Q) +
-                         static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldq +
-                         (cur.h * p.group + (r - token * p.group)) * D;
 #pragma unroll
-            for (uint32_t g = 0; g < NG; ++g) {
-                const uint32_t d = 16u * (kq + 4u * g);
+            for (uint32_t g = 0; g < NG; ++g)
 #pragma unroll
-                for (uint32_t e = 0; e < 16; ++e) v[g][e] = 0.0f;
-                if (r < rows && d < D) {
-                    float x[8];
-                    load8(q + d, p.vec & 1u, x);
-#pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) v[g][e] = x[e];
-                    load8(q + d + 8, p.vec & 1u, x);
-#pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) v[g][8 + e] = x[e];
+                for (uint32_t e = 0; e < 16; ++e) {
+                    v[g][e] = to_f32(next_q[t][g][e]);
+                    most = fmaxf(most, fabsf(v[g][e]));
                 }
-#pragma unroll
-                for (uint32_t e = 0; e < 16; ++e) most = fmaxf(most, fabsf(v[g][e]));
-            }
             most = quad_max(most);
             const int ex = row_exponent(most);
             const float up = pow2(ex);
@@ -530,7 +542,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
 
     // The warps' sums of a row tile joined through their consumed slots, and
     // written: as the output when this CTA saw all its keys, else as a part.
-    const auto end_rows = [&](uint32_t slot, bool more) {
+    const auto end_rows = [&](uint32_t slot, bool more, const Cursor *after) {
         const uint32_t rows = min(MR, static_cast<uint32_t>(cur.s.n) * p.group - cur.rt * MR);
         float *const mine_o = reinterpret_cast<float *>(ring + slot * Shape::kSlot);
 #pragma unroll
@@ -558,6 +570,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
                         make_float4(acc[t][j][r], acc[t][j][2 + r], acc[t][j + 1][r], acc[t][j + 1][2 + r]);
                 }
             }
+        if (after) read_rows(*after);
         __syncthreads();
         const bool started = first_tile == cur.lo;
         const uint32_t part = 2 * cta + (started ? 1 : 0);
@@ -610,26 +623,29 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
         __syncthreads();  // the slots may be filled again
     };
 
+    read_rows(cur);
     uint32_t slot = 0;
     bool fresh = true;
     uint32_t parts = 0;
-    for (; left; --left) {
+    for (;; --left) {
         cp_async_wait_group<S - 2>();
         __syncwarp();
         issue();  // into the slot that the last step consumed
         fetch_pages();
         if (fresh) begin_rows();
         compute(slot);
-        const bool row_end = cur.tile + 1 == cur.lo + cur.nt;
-        fresh = row_end;
-        if (row_end || left == 1) {
+        Cursor after = cur;
+        fresh = left > 1 && next_unit<MR>(p, after);
+        if (fresh || left == 1) {
+            const bool row_end = cur.tile + 1 == cur.lo + cur.nt;
             if (!row_end && first_tile == cur.lo)   // the tile's first CTA joins its parts
                 parts = 1 + static_cast<uint32_t>((cur.lo + cur.nt - cur.tile - 1 + run - 1) / run);
-            end_rows(slot, !row_end);
+            end_rows(slot, !row_end, fresh ? &after : nullptr);
         } else {
             __syncwarp();
         }
-        if (left > 1) next_unit<MR>(p, cur);
+        if (left == 1) break;
+        cur = after;
         slot = slot + 1 == S ? 0 : slot + 1;
     }
     cp_async_wait_group<0>();
