@@ -288,7 +288,8 @@ typedef struct vnpu_b200_matmul_i8_swiglu_args_t {
  * counterpart: the reference has no KV cache).  K and V hold int8 codes,
  * [num_pages][heads][page_size][head_dim]; K_scale and V_scale one f32 for
  * each page and head, [num_pages][heads]; a cached value is code * scale.
- * All four are device memory, owned by the caller, the codes 16-byte aligned;
+ * Scales are not negative; a page of zeros may have the scale 0.  All four are
+ * device memory, owned by the caller, the codes 16-byte aligned;
  * nothing needs to be cleared before a page's first use.  page_size is a power
  * of two from 16 to 256, head_dim a multiple of 16 up to 256.
  */
@@ -405,8 +406,10 @@ typedef struct vnpu_b200_paged_kv_read_args_t {
  * that attends to nothing has the output 0.  Scores, softmax sums and
  * accumulators are 32 bits wide; the softmax weights enter the value product
  * as 16-bit floats for 16-bit outputs, and as two of them (22 bits) for f32.
- * max_length, when not 0, is the longest seq_lens[b] to expect; it only
- * chooses how the work is split.
+ * max_length, when not 0, is the longest seq_lens[b] to expect, for the
+ * device's byte and flop counters; the kernels read the lengths themselves.
+ * Scratch (partial sums of rows that are split over the GPU) is stream-ordered,
+ * about 4 MB for few rows and 38 MB for many.
  */
 #define VNPU_B200_OP_PAGED_ATTENTION  0x10bu
 

@@ -287,7 +287,6 @@ struct PagedAttention {
     RowType type = RowType::kF32;
     bool causal = true;
     uint32_t window = 0;             // 0 = none
-    uint32_t max_length = 0;         // expected longest sequence; 0 = the table's reach
     float scale = 1.0f;
 };
 cudaError_t paged_attention(const LaunchCtx &ctx, const PagedAttention &p);

@@ -13,7 +13,8 @@
 // the cache's side.  A query row is scaled by a power of two to a largest
 // element in [2^13, 2^14): f16 and bf16 queries are then exact too (down to
 // 2^-27 of the row's largest), and f32 ones become hi + lo, 22 bits, two
-// products on one accumulator; their weights p are split the same way.  Sums, maxima and accumulators are f32.
+// products on one accumulator; their weights p are split the same way.  Sums,
+// maxima and accumulators are f32.
 //
 // m follows the running maximum only when that has grown by more than 2^6, so
 // the accumulators are rescaled a few times a row instead of at every step.
@@ -786,7 +787,11 @@ cudaError_t launch_few(const LaunchCtx &ctx, const PagedAttention &a) {
 }  // namespace
 
 cudaError_t paged_attention(const LaunchCtx &ctx, const PagedAttention &a) {
-    if (1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > 32) {
+    // Rows of a key/value head in one sequence (tokens x group): up to 48 the few-row kernel's 16-row
+    // tiles read the codes again for each tile and still win.  16 sequences of 2048 keys, 8 heads of
+    // 128, bf16, in us, few against many: 32 rows 46 and 60, 48 rows 64 and 61, 64 rows 78 and 62;
+    // 64 sequences of 512 keys: 48 rows 78 and 85, 64 rows 94 and 86; f32 there: 118 and 114, 147 and 118.
+    if (1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > 48) {
         const cudaError_t e = paged_attention_many_rows(ctx, a);
         if (e != cudaErrorNotSupported) return e;
     }

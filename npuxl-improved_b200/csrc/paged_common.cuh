@@ -84,6 +84,7 @@ __device__ __forceinline__ bool load_seq(const PagedBatch &pb, uint32_t page_shi
     // c1 >= c0 >= 0 comes first: the differences above are then exact
     return c0 >= 0 && c1 >= c0 && static_cast<uint32_t>(c1) <= pb.tokens &&
            static_cast<uint32_t>(s.n) <= pb.max_tokens && s.len >= s.n &&
+           s.len <= 0x7fffff00 &&   // key tiles' ends stay in 32 bits
            static_cast<uint64_t>(s.len) <= (static_cast<uint64_t>(pb.table_stride) << page_shift);
 }
 

@@ -207,32 +207,6 @@ __device__ __forceinline__ void tmem_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// mbar_wait that lets the warp sleep for up to 50 us at a time: the waiting
-// roles' polls would take issue slots from the working ones.
-__device__ __forceinline__ bool wait_asleep(uint64_t *bar, uint32_t parity, uint64_t limit_ns,
-                                            uint32_t *err, volatile int *abort) {
-    const uint32_t a = smem_addr(bar);
-    uint64_t start = 0;
-    for (;;) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if (*abort) return false;
-        const uint64_t now = global_timer_ns();
-        if (!start) start = now;
-        if (now - start > limit_ns) {
-            record_error(err, kErrWaitTimeout);
-            *abort = 1;
-            return false;
-        }
-    }
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -336,7 +310,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const uint32_t tmem = sh_tmem;
     pdl_enter();
     const auto wait = [&](uint64_t *bar, uint32_t parity) {
-        return wait_asleep(bar, parity & 1u, p.limit_ns, p.err, &sh_abort);
+        return mbar_wait(bar, parity & 1u, p.limit_ns, p.err, &sh_abort);
     };
     // the same for a whole warp, which goes on together (tensor memory loads need that)
     const auto wait_warp = [&](uint64_t *bar, uint32_t parity) {

@@ -1196,7 +1196,6 @@ void exec_paged_attention(vnpu_stream_t *s, const vnpu_command_t &cmd, const Lau
     p.type = paged_row_type(a.dtype);
     p.causal = a.causal != 0;
     p.window = a.window;
-    p.max_length = a.max_length;
     p.scale = a.scale != 0.0f ? a.scale : 1.0f / std::sqrt(static_cast<float>(d));
     cuda_check(paged_attention(ctx, p), "paged_attention launch");
     st.finish();

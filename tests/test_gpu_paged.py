@@ -539,6 +539,76 @@ def test_step_in_a_graph_follows_the_device_arrays(gpu, torch):
     gpu.lib.b200_graph_destroy(graph)
 
 
+@pytest.mark.parametrize("dtype,spans", [("bf16", [(1, 3000), (1, 200)]), ("f32", [(70, 900), (3, 500)])])
+def test_graphs_keep_their_own_workspaces(gpu, torch, dtype, spans):
+    """Two captured attentions whose parts are joined, replayed in turns: each gives what the plain
+    call gives."""
+    s = Setup(torch, spans, 2, 128, 64)
+    qs = [rows(torch, np.random.default_rng(i), s.tokens, 4 * 128, dtype)[0].view(-1, 4, 128) for i in range(2)]
+    want, got = [torch.empty_like(q) for q in qs], [torch.empty_like(q) for q in qs]
+    torch.cuda.synchronize()
+    for q, o in zip(qs, want):
+        gpu.paged_attention(s.cache, s.batch, q, o)
+    graphs = [gpu.capture([vnpu.paged_attention_cmd(s.cache, s.batch, q, o)]) for q, o in zip(qs, got)]
+    for _ in range(3):
+        for o in got:
+            o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for g in graphs + graphs:
+            gpu.replay(g)
+        assert gpu.sync() == vnpu.OK
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for g in graphs:
+        gpu.lib.b200_graph_destroy(g)
+
+
+def test_two_streams_read_one_cache(gpu, torch):
+    """Attention on two streams at once, nothing between them: workspaces are not shared."""
+    s = Setup(torch, [(1, 6000), (1, 900), (80, 1500)], 2, 128, 64)
+    one = vnpu.paged_batch(s.dtable[:2], s.dcu[:3], s.dlens[:2], 2, 1)
+    q, q64 = rows(torch, np.random.default_rng(4), s.tokens, 4 * 128, "bf16")
+    q = q.view(-1, 4, 128)
+    want, size, most = attention64(s, q64, 4, True, 0)
+    other = C.c_void_p()
+    gpu.lib.check(gpu.lib.stream_create(gpu.dev, 0, C.byref(other)), "stream_create")
+    outs = [torch.empty((2 if i % 2 else s.tokens, 4, 128), dtype=torch.bfloat16, device="cuda") for i in range(8)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        cmd = (vnpu.Command * 1)(vnpu.paged_attention_cmd(s.cache, one if i % 2 else s.batch,
+                                                          q[:2] if i % 2 else q, o))
+        assert gpu.lib.stream_submit(other if i % 4 < 2 else gpu.stream, cmd, 1, None) == vnpu.OK
+    assert gpu.sync() == vnpu.OK and gpu.lib.stream_sync(other) == vnpu.OK
+    gpu.lib.stream_destroy(other)
+    for i, o in enumerate(outs):
+        n = len(o)
+        check_attention(o, want[:n], size[:n], most[:n], "bf16")
+
+
+def test_pools_of_more_than_four_gigabytes(gpu, torch):
+    """Pages whose offsets pass 32 bits: append, read and attention at the end of a 4.6 GB pool."""
+    hk, d, ps, n = 4, 256, 256, 300
+    pages = 4_600_000_000 // (hk * d * ps)
+    k, v = (torch.empty((pages, hk, ps, d), dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.full((pages, hk), float("nan"), device="cuda") for _ in range(2))
+    table = torch.tensor([[pages - 1, pages // 2 + 7]], dtype=torch.int32, device="cuda")
+    cu, lens = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, n], [n]))
+    cache, batch = vnpu.paged_cache(k, v, ks, vs), vnpu.paged_batch(table, cu, lens, n)
+    x = torch.randn((3, n, hk, d), generator=torch.Generator().manual_seed(1)).cuda()
+    back = torch.empty((2, n, hk, d), device="cuda")
+    q, o = torch.empty_like(x[0]), torch.empty_like(x[0])
+    torch.cuda.synchronize()
+    gpu.paged_kv_append(cache, batch, x[0].flatten(1), x[1].flatten(1), x[2].flatten(1), q.flatten(1),
+                        q_heads=hk, rope=False)
+    gpu.paged_kv_read(cache, batch, back[0], back[1])
+    step = x[1:].abs().amax() / 127
+    assert (back - x[1:]).abs().max() <= 0.5001 * step
+    gpu.paged_attention(cache, batch, q, o)
+    w = torch.einsum("qhd,khd->hqk", x[0].double(), back[0].double()) / 16
+    w = w.masked_fill(torch.ones((n, n), device="cuda").triu(1).bool(), -float("inf")).softmax(-1)
+    want = torch.einsum("hqk,khd->qhd", w, back[1].double())
+    assert (o.double() - want).abs().max() <= back[1].abs().max() * 2.0 ** -20 * (1 + 16 * 4 * 4)
+
+
 def test_host_rows_are_staged(gpu, torch):
     hq, hk, d = 2, 2, 64
     s = Setup(torch, SPANS["mixed"], hk, d, 16)

@@ -35,10 +35,11 @@ def test_sequences_of_any_lengths_step_together(b200_lib, torch, page_size):
             blk = B200Block(cfg, b200_lib, dev, torch)
             x = rows[s].cuda()
             torch.cuda.synchronize()
-            out = [blk.forward(x[:n], 0).clone()] if n > 1 else []
-            for i in range(n if n > 1 else 0, n + 6):
-                out.append(blk.forward(x[i:i + 1], i).clone())
-                dev.sync()
+            out = []
+            for i, j in [(0, n)] * (n > 1) + [(i, i + 1) for i in range(n if n > 1 else 0, n + 6)]:
+                y = blk.forward(x[i:j], i)
+                assert dev.sync() == vnpu.OK
+                out.append(y.clone())
             torch.cuda.synchronize()
             want[s] = torch.cat(out).cpu()
             blk.close()
