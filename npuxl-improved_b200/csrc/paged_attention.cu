@@ -28,6 +28,10 @@ namespace {
 constexpr uint32_t kWarps = 4, kThreadsA = kWarps * 32;
 constexpr uint32_t kTile = 128;      // keys of a work unit, 32 for each warp
 constexpr uint32_t kWarpKeys = kTile / kWarps;
+// Reach of a table up to which row tiles are not split.  One token, 16 sequences of 32/8 heads of 128,
+// us without and with splitting and joining: 256 keys 9.2 and 9.6, 384 keys 11.5 and 9.9; 64 sequences
+// of 8 heads of 64: 12.4 and 13.3, 15.6 and 14.8.
+constexpr uint32_t kWholeKeys = 256;
 
 // As many CTAs an SM as the registers allow (the kernel is bound by the latency
 // of its own instructions before it is by memory), rings as deep as that allows.
@@ -109,7 +113,8 @@ __device__ __forceinline__ bool next_unit(const AttnParams &p, Cursor &k) {
     return true;
 }
 
-// Persistent CTAs, each with an equal run of units: sequences of any lengths
+// Persistent CTAs, each with an equal run of units (or, with `whole`, of row
+// tiles, which are then not split and need no joining): sequences of any lengths
 // give every CTA the same work, and a (sequence, head, row tile) is split over
 // CTAs only where runs meet.  A warp keeps kStages - 1 units in flight through
 // its own ring of cp.async copies (no CTA-wide waits within a run), across
@@ -124,7 +129,7 @@ __device__ __forceinline__ bool next_unit(const AttnParams &p, Cursor &k) {
 // more.
 template <RowType T, uint32_t DP, uint32_t MR>
 __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
-    paged_attention_kernel(const __grid_constant__ AttnParams p, const uint32_t min_units) {
+    paged_attention_kernel(const __grid_constant__ AttnParams p, const bool whole) {
     using E = typename RowOf<T>::type;
     using Shape = AttnShape<DP, MR>;
     constexpr bool kSplit = T == RowType::kF32;
@@ -150,7 +155,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
         bool bad;
         seq_units<MR>(p, b, cur, &bad);
         if (bad) record_error(p.err, kErrBadIndex);
-        mine += static_cast<unsigned long long>(cur.rts) * p.c.heads * cur.nt;
+        mine += static_cast<unsigned long long>(cur.rts) * p.c.heads * (whole ? 1 : cur.nt);
     }
     unsigned long long upto = mine;
 #pragma unroll
@@ -166,20 +171,19 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
         if (w < warp) upto += sh_sum[w];
         total += sh_sum[w];
     }
-    unsigned long long run = (total + gridDim.x - 1) / gridDim.x;
-    if (run < min_units) run = min_units;
+    const unsigned long long run = max(1ull, (total + gridDim.x - 1) / gridDim.x);
     const unsigned long long t0 = run * cta;
     if (t0 >= total) {
         if (tid == 0 && p.ws_meta) p.ws_meta[2 * cta].x = 0;
         return;
     }
-    uint32_t left = static_cast<uint32_t>(min(run, total - t0));  // units of this CTA
+    uint32_t left = static_cast<uint32_t>(min(run, total - t0));  // units (row tiles) of this CTA
     unsigned long long before = upto - mine;
     if (before <= t0 && t0 < upto) {
         for (uint32_t b = b_lo; b < b_hi; ++b) {
             bool bad;
             seq_units<MR>(p, b, cur, &bad);
-            const unsigned long long w = static_cast<unsigned long long>(cur.rts) * p.c.heads * cur.nt;
+            const unsigned long long w = static_cast<unsigned long long>(cur.rts) * p.c.heads * (whole ? 1 : cur.nt);
             if (t0 < before + w) {
                 sh_cursor = cur;
                 sh_off = t0 - before;
@@ -192,7 +196,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     {
         cur = sh_cursor;
         const unsigned long long off = sh_off;
-        const unsigned long long nt = static_cast<uint32_t>(cur.nt), row_tile = off / nt;
+        const unsigned long long nt = whole ? 1u : static_cast<uint32_t>(cur.nt), row_tile = off / nt;
         cur.h = static_cast<uint32_t>(row_tile / cur.rts);
         cur.rt = static_cast<uint32_t>(row_tile - static_cast<unsigned long long>(cur.h) * cur.rts);
         cur.tile = cur.lo + static_cast<int32_t>(off - row_tile * nt);
@@ -284,7 +288,8 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
                     }
                 }
             }
-            if (--ahead_left && next_unit<MR>(p, ahead)) ahead_limits();
+            if (!whole || ahead.tile + 1 == ahead.lo + ahead.nt) --ahead_left;
+            if (ahead_left && next_unit<MR>(p, ahead)) ahead_limits();
         }
         cp_async_commit();
         slot_in = slot_in + 1 == S ? 0 : slot_in + 1;
@@ -628,24 +633,25 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     uint32_t slot = 0;
     bool fresh = true;
     uint32_t parts = 0;
-    for (;; --left) {
+    for (;;) {
         cp_async_wait_group<S - 2>();
         __syncwarp();
         issue();  // into the slot that the last step consumed
         fetch_pages();
         if (fresh) begin_rows();
         compute(slot);
+        const bool row_end = cur.tile + 1 == cur.lo + cur.nt;
+        if (!whole || row_end) --left;
         Cursor after = cur;
-        fresh = left > 1 && next_unit<MR>(p, after);
-        if (fresh || left == 1) {
-            const bool row_end = cur.tile + 1 == cur.lo + cur.nt;
+        fresh = left && next_unit<MR>(p, after);
+        if (fresh || !left) {
             if (!row_end && first_tile == cur.lo)   // the tile's first CTA joins its parts
                 parts = 1 + static_cast<uint32_t>((cur.lo + cur.nt - cur.tile - 1 + run - 1) / run);
             end_rows(slot, !row_end, fresh ? &after : nullptr);
         } else {
             __syncwarp();
         }
-        if (left == 1) break;
+        if (!left) break;
         cur = after;
         slot = slot + 1 == S ? 0 : slot + 1;
     }
@@ -746,8 +752,8 @@ cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
         ready_device = device;
     }
     const uint32_t grid = static_cast<uint32_t>(ctx.num_sms) * Shape::kCtasPerSm;
-    // One key tile holds all that the table reaches: nothing is split, nothing to join.
-    const bool split = (static_cast<uint64_t>(a.batch.table_stride) << a.cache.page_shift) > kTile;
+    // A table that reaches a few key tiles only: row tiles are not split, and nothing is joined.
+    const bool split = (static_cast<uint64_t>(a.batch.table_stride) << a.cache.page_shift) > kWholeKeys;
     void *ws = nullptr;
     const size_t o_bytes = 2ull * grid * MR * DP * sizeof(float);
     const size_t ml_bytes = 2ull * grid * MR * sizeof(float2);
@@ -759,7 +765,7 @@ cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
     }
     if (ctx.launch_counter) *ctx.launch_counter += split ? 2 : 1;
     cudaError_t e = launch_pdl(ctx.stream, &paged_attention_kernel<T, DP, MR>, dim3(grid), dim3(kThreadsA),
-                               Shape::kSmem, p, 1u);
+                               Shape::kSmem, p, !split);
     if (split) {
         const uint64_t rows = std::min<uint64_t>(MR, 1ull * a.batch.max_tokens * p.group);
         const uint32_t y = static_cast<uint32_t>((rows * (DP / 4) + 31) / 32);

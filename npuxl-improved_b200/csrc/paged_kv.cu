@@ -62,7 +62,7 @@ __device__ __forceinline__ bool find_numbers(const PagedCache &c, const PagedBat
         if (b >= pb.batch) return false;
         good = load_seq(pb, c.page_shift, b, s);
     }
-    if (!good && threadIdx.x == 0) record_error(err, kErrBadIndex);
+    if (!good && (threadIdx.x & 31u) == 0) record_error(err, kErrBadIndex);
     return good;
 }
 
@@ -76,7 +76,7 @@ __device__ __forceinline__ bool find_segment(const PagedCache &c, const PagedBat
     if (pb.max_tokens == 1) {
         b = item;  // one segment a sequence: item b is sequence b's
         if (!load_seq(pb, c.page_shift, b, s)) {
-            if (threadIdx.x == 0) record_error(err, kErrBadIndex);
+            if ((threadIdx.x & 31u) == 0) record_error(err, kErrBadIndex);
             return false;
         }
     } else {
@@ -104,7 +104,7 @@ __device__ __forceinline__ bool find_segment(const PagedCache &c, const PagedBat
 }
 __device__ __forceinline__ bool page_there(const PagedCache &c, const Segment &g, uint32_t *err) {
     const bool there = g.page >= 0 && g.page < c.num_pages;
-    if (!there && threadIdx.x == 0) record_error(err, kErrBadIndex);
+    if (!there && (threadIdx.x & 31u) == 0) record_error(err, kErrBadIndex);
     return there;
 }
 

@@ -756,6 +756,30 @@ def test_device_arrays_are_checked(b200_lib, gpu, torch, what):
     assert (gpu.sync()) == vnpu.OK
 
 
+@pytest.mark.parametrize("bad", range(5))
+def test_every_single_token_sequence_is_checked(b200_lib, gpu, torch, bad):
+    """One token a sequence, one bad page among five: reported wherever it is, the others appended."""
+    s = Setup(torch, [(1, 10 + i) for i in range(5)], 1, 64, 16)
+    table = s.dtable.clone()
+    table[bad] = s.pages + 5
+    batch = vnpu.paged_batch(table, s.dcu, s.dlens, 5, 1)
+    x = torch.full((5, 64), 50.0, device="cuda")
+    q = torch.zeros((5, 1, 64), device="cuda")
+    torch.cuda.synchronize()
+    cmds = [vnpu.paged_kv_append_cmd(s.cache, batch, None, x, x, None, rope=False),
+            vnpu.paged_kv_read_cmd(s.cache, batch, q.clone(), None),
+            vnpu.paged_attention_cmd(s.cache, batch, q, q.clone())]
+    for cmd in cmds:
+        _, sync = _status(b200_lib, cmd)
+        assert sync == vnpu.ERR_DEVICE_ERROR
+    for b in range(5):
+        new = s.dv[int(s.table[b, 0]), 0, 9 + b].cpu()
+        if b != bad:
+            assert (new == 127).all()
+        else:
+            assert np.array_equal(new, s.v[int(s.table[b, 0]), 0, 9 + b])
+
+
 def test_python_helpers_refuse(torch):
     k = torch.zeros((2, 1, 16, 64), dtype=torch.int8)
     sc = torch.zeros((2, 1))
