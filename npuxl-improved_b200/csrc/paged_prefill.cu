@@ -38,8 +38,11 @@ constexpr uint32_t kHalf = 128;              // rows of one accumulator (UMMA M)
 constexpr uint32_t kRows = 2 * kHalf;        // query rows of a block
 constexpr uint32_t kManyThreads = 640;       // 8 softmax, 8 converter, tensor-issue, 2 copy, a spare warp
 constexpr uint32_t kScaleRing = 4;           // tiles whose scales are kept
-constexpr uint32_t kRawRing = 4;             // half tiles of codes on their way or in conversion
+constexpr uint32_t kRawRing = 4;             // half tiles of codes: two of K, two of V
 constexpr uint32_t kPlanThreads = 1024;
+// What the start and the end of a block cost beside its key tiles, in tiles: runs are of equal cost.
+// (With 0, the CTAs of 8 ragged prompts took from 365 to 485 thousand clocks.)
+constexpr int32_t kBlockCost = 3;
 
 // A block of rows and the key tiles that any of its rows sees.
 struct RowBlock {
@@ -48,10 +51,10 @@ struct RowBlock {
 };
 
 struct Plan {
-    uint32_t *head;        // [0]: blocks, [1]: tiles of one head
+    uint32_t *head;        // [0]: blocks, [1]: cost of one head's
     uint32_t *seq_base;    // [batch + 1]: blocks before sequence b
     RowBlock *blocks;
-    uint32_t *before;      // tiles before block e (one head)
+    uint32_t *before;      // cost of the blocks before block e (one head)
 };
 
 template <uint32_t KT>
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const AttnPara
             x = block_tiles<KT>(p, s, lo, e - plan.seq_base[lo]);
             plan.blocks[e] = x;
         }
-        const uint32_t at = tiles + block_scan(static_cast<uint32_t>(x.nt), sh, &total);
+        const uint32_t at = tiles + block_scan(e < blocks ? static_cast<uint32_t>(x.nt + kBlockCost) : 0u, sh, &total);
         if (e < blocks) plan.before[e] = at;
         tiles += total;
     }
@@ -225,32 +228,41 @@ struct ManyShape {
     static constexpr uint32_t kPCol = kSplit ? 64 : 0, kOCol = 128, kHalfCols = 256;
 };
 
-// Where a CTA stands in the units: head, block, tile; the roles walk alike.
+// Where a CTA stands in its run: head, block, tiles; the roles walk alike.  A
+// block is kBlockCost units, then one for each key tile; a CTA has the tiles
+// whose units are in its run.
 struct Walk {
-    uint32_t left, h, e, blocks;    // tiles left; current head and block
-    int32_t tile, count;            // first tile and tiles of this segment
+    uint32_t left, h, e, blocks;    // units left; current head and block
+    int32_t used;                   // units of this segment
+    int32_t tile, count;            // its first tile and its tiles
     RowBlock x;
     PagedSeq s;
 
-    // Takes the segment that begins `off` tiles into block e.
+    // Takes the segment that begins `off` units into block e; it may have no tile.
     __device__ __forceinline__ void take(const AttnParams &p, const Plan &plan, uint32_t off) {
         const int4 v = __ldcg(reinterpret_cast<const int4 *>(plan.blocks) + e);
         x.b = static_cast<uint32_t>(v.x);
         x.rb = static_cast<uint32_t>(v.y);
         x.lo = v.z;
         x.nt = v.w;
-        tile = x.lo + static_cast<int32_t>(off);
-        count = min(x.nt - static_cast<int32_t>(off), static_cast<int32_t>(left));
+        const int32_t from = static_cast<int32_t>(off);
+        used = min(x.nt + kBlockCost - from, static_cast<int32_t>(min(left, 0x7fffffffu)));
+        const int32_t first = max(0, from - kBlockCost);
+        tile = x.lo + first;
+        count = max(0, from + used - kBlockCost) - first;
         load_seq(p.pb, p.c.page_shift, x.b, s);
     }
+    // The next segment that has tiles.
     __device__ __forceinline__ bool next(const AttnParams &p, const Plan &plan) {
-        left -= static_cast<uint32_t>(count);
-        if (!left) return false;
-        if (++e == blocks) {
-            e = 0;
-            ++h;
-        }
-        take(p, plan, 0);
+        do {
+            left -= static_cast<uint32_t>(used);
+            if (!left) return false;
+            if (++e == blocks) {
+                e = 0;
+                ++h;
+            }
+            take(p, plan, 0);
+        } while (!count);
         return true;
     }
 };
@@ -330,7 +342,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const uint64_t total = static_cast<uint64_t>(per_head) * p.c.heads;
     const uint64_t run = (total + gridDim.x - 1) / gridDim.x, t0 = run * cta;
     w.left = t0 < total ? static_cast<uint32_t>(min(run, total - t0)) : 0;
-    const bool busy = w.left != 0;
+    bool busy = w.left != 0;
     if (busy) {
         w.h = static_cast<uint32_t>(t0 / per_head);
         const uint32_t off = static_cast<uint32_t>(t0 - static_cast<uint64_t>(w.h) * per_head);
@@ -345,6 +357,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         w.e = lo;
         w.take(p, plan, off - __ldcg(plan.before + lo));
+        if (!w.count) busy = w.next(p, plan);
     }
 
     // The block's 640 x 96 registers go where they are needed: 256 x 152 + 384 x 56.  (The spare
@@ -495,9 +508,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             more = w.next(p, plan);
             if (tid == 0 && !more) {
                 // joined with the CTAs that go on with the block, when it begins here
-                const uint32_t parts = cur.tile == cur.x.lo && cur.count != cur.x.nt
-                                           ? 1 + static_cast<uint32_t>((cur.x.nt - cur.count + run - 1) / run)
-                                           : 0;
+                uint32_t parts = 0;
+                if (cur.tile == cur.x.lo && cur.count != cur.x.nt) {
+                    const uint64_t end = static_cast<uint64_t>(cur.h) * per_head + __ldcg(plan.before + cur.e) +
+                                         static_cast<uint32_t>(cur.x.nt + kBlockCost);
+                    parts = static_cast<uint32_t>((end - 1) / run) - cta + 1;
+                }
                 p.ws_meta[2 * cta] = make_uint4(parts, static_cast<uint32_t>(cur.s.row0), cur.x.rb * kRows, cur.h);
                 p.ws_meta[2 * cta + 1] = make_uint4(
                     min(kRows, static_cast<uint32_t>(cur.s.n) * p.group - cur.x.rb * kRows), 0, 0, 0);
@@ -642,15 +658,21 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             fence_proxy_async_smem();
         };
         // this warp's half of a tile's K, then of its V, and on to the next tile
+        uint32_t it = 0;
+        bool ok = true, more = true;
+        while (more && ok) {
+            const int32_t count = w.count;
+            more = w.next(p, plan);
 #pragma unroll 1
-        for (uint32_t x = second; x < 4 * w.left; x += 2) {
-            const uint32_t it = x >> 2, st = it & 1u, slot = x % kRawRing;
-            const bool v = x & 2u;
-            if (!wait_warp(&bar_r[slot], x / kRawRing)) break;
-            if (it >= 2 && !wait_warp(v ? &bar_v_free[st] : &bar_k_free[st], (it >> 1) - 1)) break;
-            convert(raw + slot * Shape::kRawBytes, (v ? sv : sk) + st * Shape::kKvBytes + second * (KT / 2 * 128u));
-            arrive_warp(v ? &bar_v[st] : &bar_k[st]);
-            arrive_warp(&bar_r_free[slot]);
+            for (int32_t x = 0; x < 2 * count; ++x) {
+                const uint32_t st = it & 1u, v = x & 1u, slot = 2 * v + second;
+                if (!(ok = wait_warp(&bar_r[slot], it))) break;
+                if (it >= 2 && !(ok = wait_warp(v ? &bar_v_free[st] : &bar_k_free[st], (it >> 1) - 1))) break;
+                convert(raw + slot * Shape::kRawBytes, (v ? sv : sk) + st * Shape::kKvBytes + second * (KT / 2 * 128u));
+                arrive_warp(v ? &bar_v[st] : &bar_k[st]);
+                arrive_warp(&bar_r_free[slot]);
+                it += v;
+            }
         }
     } else if (busy && warp == 16) {
         // =============================== tensor products ===============================
@@ -726,6 +748,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const bool values_too = warp == 18;
         const int8_t *const pool = values_too ? p.c.V : p.c.K;
         struct Group {
+            bool real;          // there is such a tile
             int32_t page;       // -1: not there
             uint32_t h, slot;   // head; slot of its first key in the page
             float ks, vs;
@@ -735,6 +758,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const auto look_up = [&](Group &g) {
             g.page = -1;
             g.ks = g.vs = 0.0f;
+            g.real = more;
             if (!more) return;
             const int32_t key = (w.tile + j) * static_cast<int32_t>(KT) + static_cast<int32_t>(lane * 16u);
             g.h = w.h;
@@ -761,7 +785,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             g.ks = __ldg(p.c.K_scale + at);
             g.vs = __ldg(p.c.V_scale + at);
         };
-        const uint32_t tiles = w.left;
         const uint32_t per_copy = min(1u << (p.c.page_shift - 4u), kGroups / 2);   // groups of a page in half a tile
         Group now, next, later;
         now.slot = next.slot = later.slot = 0xffffffffu;
@@ -771,12 +794,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         read_scales(next);
         uint32_t begun = 0;     // tiles whose copies were begun
         bool ok = true;
-        for (uint32_t it = 0; it < tiles; ++it) {
+        for (uint32_t it = 0; next.real; ++it) {
             now = next;
             next = later;
             later.slot = 0xffffffffu;
             look_up(later);
-            if (it + 1 < tiles) read_scales(next);
+            if (next.real) read_scales(next);
             const uint32_t ring = it % kScaleRing;
             // A group that is not there stays as it is in shared memory (whole numbers all the
             // same); its keys are masked or count as zeros.
