@@ -18,6 +18,11 @@
 //
 // m follows the running maximum only when that has grown by more than 2^6, so
 // the accumulators are rescaled a few times a row instead of at every step.
+//
+// Measured, bf16, 32/8 heads of 128: one token each for 2 sequences of 131072
+// keys 93 us (537 MB, 5.75 TB/s, 87 % of the copy bandwidth) and 7 us of
+// joining; for 64 sequences of up to 4096 keys 67 us with joining (304 MB, 4.5
+// TB/s: the starts and ends of rows beside the stream).
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -319,7 +324,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
 #pragma unroll
         for (uint32_t t = 0; t < NT; ++t) {
             const uint32_t r = k.rt * MR + 8 * t + n;       // the row of this lane's fragment
-            const uint32_t token = r / p.group;
+            const uint32_t token = token_of(p, r);
             const E *q = static_cast<const E *>(p.Q) +
                          static_cast<uint64_t>(k.s.row0 + static_cast<int32_t>(token)) * p.ldq +
                          (k.h * p.group + (r - token * p.group)) * D;
@@ -605,7 +610,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
                 o.w = fmaf(x.w, f, o.w);
             }
             if (started && !more) {
-                const uint32_t r = cur.rt * MR + row, token = r / p.group;
+                const uint32_t r = cur.rt * MR + row, token = token_of(p, r);
                 const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
                 E *out = static_cast<E *>(p.O) +
                          static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldo +
@@ -716,7 +721,7 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const AttnPar
         o.w += v.w * f;
     }
     const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
-    const uint32_t r = meta.z + row, token = r / p.group;
+    const uint32_t r = meta.z + row, token = token_of(p, r);
     E *out = static_cast<E *>(p.O) + static_cast<uint64_t>(meta.y + token) * p.ldo +
              (meta.w * p.group + (r - token * p.group)) * p.c.head_dim + 4u * d4;
     from_f32(o.x * inv, out[0]);
@@ -737,6 +742,7 @@ cudaError_t launch_attention(const LaunchCtx &ctx, const PagedAttention &a) {
     p.ldq = a.ldq;
     p.ldo = a.ldo;
     p.group = a.q_heads / a.cache.heads;
+    p.group_inverse = inverse_of(p.group);
     p.causal = a.causal;
     p.window = a.window;
     p.scale_log2 = a.scale * 1.4426950408889634f;

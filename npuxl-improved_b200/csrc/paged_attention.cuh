@@ -23,6 +23,7 @@ struct AttnParams {
     const void *Q;
     void *O;
     uint32_t ldq, ldo, group;
+    uint32_t group_inverse;   // floor(2^32 / group); 0 for a group of one
     uint32_t causal, window;
     float scale_log2;
     uint32_t vec;          // bit 0: Q 16-byte accesses, bit 1: O 4-element, bit 2: O 16-byte accesses
@@ -53,11 +54,22 @@ __device__ __forceinline__ int row_exponent(float most) {
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 
+// Row of a sequence's (token, head of the group) rows to its token: the product
+// with the rounded-down inverse is the quotient or one less.
+__device__ __forceinline__ uint32_t token_of(const AttnParams &p, uint32_t r) {
+    if (p.group == 1) return r;
+    const uint32_t q = __umulhi(r, p.group_inverse);
+    return r - q * p.group >= p.group ? q + 1 : q;
+}
+inline uint32_t inverse_of(uint32_t group) {
+    return group == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / group);
+}
+
 // Positions that row r (clamped to the sequence's last) of a sequence sees.
 __device__ __forceinline__ void row_limits(const AttnParams &p, const PagedSeq &s, uint32_t r,
                                            int32_t &kmin, int32_t &kmax) {
     const uint32_t rows = static_cast<uint32_t>(s.n) * p.group;
-    const int32_t pos = s.start + static_cast<int32_t>(min(r, rows - 1) / p.group);
+    const int32_t pos = s.start + static_cast<int32_t>(token_of(p, min(r, rows - 1)));
     kmax = p.causal ? pos : s.len - 1;
     kmin = p.window && static_cast<uint32_t>(pos) + 1u > p.window ? pos + 1 - static_cast<int32_t>(p.window) : 0;
 }

@@ -9,6 +9,12 @@
 // a run of n rows touches at most floor(n / page_size) + 2 pages, so sequence
 // b's segments can start at floor(cu[b] / page_size) + 2 b, which any CTA can
 // search for; the numbers left over are CTAs that leave at once.
+//
+// Measured, bf16, 32/8 heads of 128 where not said: append of 8800 tokens in 16
+// prompts 45 us (135 MB, 3.0 TB/s; issue slots and latency, not memory), of 64
+// single tokens 5.2 us (three dependent loads); read-back of 26 000 tokens of 8
+// heads of 64 in f16 16.5 us (58 MB, 3.5 TB/s), of 512 tokens of 32 heads in f32
+// 11 us (21 MB; one wave of CTAs and its latency).
 #include <algorithm>
 
 #include "paged_common.cuh"
@@ -126,8 +132,8 @@ __device__ __forceinline__ void turn_sincos(int32_t pos, uint64_t t, float *sn, 
     sincospif(half_turns(pos, t), sn, cs);
 }
 // Keys' angles, one for each pair and head: the fast sine and cosine, 2^-21 off
-// at most in (-pi, pi], a ten-thousandth of a code (with the exact ones the
-// prompts' append took 80 us instead of 40).
+// at most in (-pi, pi], a ten-thousandth of a code (16 prompts, 8800 tokens of
+// 32/8 heads of 128: 80.5 us with the exact ones, 50.5 with these).
 __device__ __forceinline__ void turn_sincos_fast(int32_t pos, uint64_t t, float *sn, float *cs) {
     __sincosf(half_turns(pos, t) * 3.14159265358979f, sn, cs);
 }
@@ -529,8 +535,8 @@ cudaError_t paged_kv_append(const LaunchCtx &ctx, const PagedAppend &p) {
     PagedTurns turns{};
     for (uint32_t j = 0; j < p.rotary / 2; ++j) turns.t[j] = p.turns[j];
     const uint64_t items = segment_items(p.cache, p.batch) * 2 * p.cache.heads;
-    // One token a sequence: a segment is one row, a warp's work (as a CTA's, 64 sequences of 8
-    // heads took 13 us instead of 6).
+    // One token a sequence: a segment is one row, a warp's work (64 sequences of 32/8 heads of 128:
+    // 13.1 us as a CTA's, 6.4 as a warp's).
     const bool single = p.batch.max_tokens == 1;
     const uint32_t nt = single ? 128 : 256, rows = kQueryRows(nt);
     const uint64_t kv = single ? (items + 3) / 4 : items;
