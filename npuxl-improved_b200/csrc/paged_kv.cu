@@ -12,9 +12,9 @@
 //
 // Measured, bf16, 32/8 heads of 128 where not said: append of 8800 tokens in 16
 // prompts 45 us (135 MB, 3.0 TB/s; issue slots and latency, not memory), of 64
-// single tokens 5.2 us (three dependent loads); read-back of 26 000 tokens of 8
-// heads of 64 in f16 16.5 us (58 MB, 3.5 TB/s), of 512 tokens of 32 heads in f32
-// 11 us (21 MB; one wave of CTAs and its latency).
+// single tokens 5.2 us (three dependent loads); read-back, pass after pass, of
+// 26 000 tokens of 8 heads of 64 in f16 11.7 us (58 MB, 5.0 TB/s), of 512 tokens
+// of 32 heads in f32 8.4 us (21 MB; one wave of CTAs and its latency).
 #include <algorithm>
 
 #include "paged_common.cuh"
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(NT, kWarp ? 6 : U == 2 ? 3 : 2) paged_append_k
 template <RowType T, uint32_t NT>
 __global__ void __launch_bounds__(NT, 10) paged_read_kernel(
     const PagedCache c, const PagedBatch pb, void *first, void *second, uint64_t ld_row,
-    uint64_t ld_head, uint32_t span, uint32_t spans, bool vec, bool swap, uint32_t *err) {
+    uint64_t ld_head, uint32_t span, uint32_t spans, uint32_t align, bool swap, uint32_t *err) {
     using E = typename RowOf<T>::type;
     pdl_enter();
     const uint32_t item = blockIdx.x / spans, h0 = (blockIdx.x - item * spans) * span;
@@ -472,22 +472,19 @@ __global__ void __launch_bounds__(NT, 10) paged_read_kernel(
     const uint64_t at0 = static_cast<uint64_t>(g.page) * c.heads + h0;
     const auto put = [&](const uint4 &w, float s, E *out) {
         const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+        float v[16];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t x, y;          // by way of exact 16-bit floats
-                codes_to_half4(word[2 * half + i], x, y);
-                const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&x));
-                const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&y));
-                v[4 * i] = lo.x * s;
-                v[4 * i + 1] = lo.y * s;
-                v[4 * i + 2] = hi.x * s;
-                v[4 * i + 3] = hi.y * s;
-            }
-            store8(out + 8 * half, vec, v);
+        for (int i = 0; i < 4; ++i) {
+            uint32_t x, y;          // by way of exact 16-bit floats
+            codes_to_half4(word[i], x, y);
+            const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+            const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&y));
+            v[4 * i] = lo.x * s;
+            v[4 * i + 1] = lo.y * s;
+            v[4 * i + 2] = hi.x * s;
+            v[4 * i + 3] = hi.y * s;
         }
+        store16(out, align, v);
     };
     constexpr uint32_t B = 4;
     for (uint32_t k0 = threadIdx.x; k0 < units; k0 += B * NT) {
@@ -559,7 +556,8 @@ cudaError_t paged_kv_append(const LaunchCtx &ctx, const PagedAppend &p) {
 
 cudaError_t paged_kv_read(const LaunchCtx &ctx, const PagedRead &p) {
     const uint32_t elem = p.type == RowType::kF32 ? 4 : 2;
-    const bool vec = aligned16(p.K_out, p.ld_row * elem) && aligned16(p.V_out, p.ld_head * elem);
+    const uint32_t align = common_align(reinterpret_cast<uintptr_t>(p.K_out) | reinterpret_cast<uintptr_t>(p.V_out) |
+                                        p.ld_row * elem | p.ld_head * elem);
     // Heads of a CTA: enough for 4 units a thread, where pages are small.
     const uint32_t in_head = (p.cache.head_dim << p.cache.page_shift) / 16u;
     const uint32_t span = std::max(1u, std::min(p.cache.heads, 512u / in_head));
@@ -573,7 +571,7 @@ cudaError_t paged_kv_read(const LaunchCtx &ctx, const PagedRead &p) {
         void *const first = p.K_out ? p.K_out : p.V_out;
         return launch_pdl(ctx.stream, &paged_read_kernel<T, 128>,
                           dim3(static_cast<uint32_t>(grid), p.K_out && p.V_out ? 2 : 1), dim3(128), 0, p.cache,
-                          p.batch, first, p.V_out, p.ld_row, p.ld_head, span, spans, vec, p.K_out == nullptr,
+                          p.batch, first, p.V_out, p.ld_row, p.ld_head, span, spans, align, p.K_out == nullptr,
                           ctx.err);
     });
 }

@@ -488,6 +488,29 @@ def test_read(gpu, torch, dtype, spans, hk, d, ps, layout):
         assert torch.equal(o.cpu(), torch.from_numpy(want).to(o.dtype))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shift", [16, 8, 4, 1], ids=lambda e: f"from{e}")
+@pytest.mark.parametrize("gap", [0, 16, 8, 1], ids=lambda e: f"gap{e}")
+@pytest.mark.parametrize("spans", [[(300, 300), (5, 40)], [(5, 40), (1, 300)]], ids=["many", "few"])
+def test_places_of_outputs(gpu, torch, dtype, shift, gap, spans):
+    """Read-back and attention to bases and rows of every alignment: the same values, nothing beside them."""
+    hk, d, ps = 2, 64, 16
+    s = Setup(torch, spans, hk, d, ps)
+    q, _ = rows(torch, np.random.default_rng(5), s.tokens, hk * d, dtype)
+    q = q.view(s.tokens, hk, d)
+    width = hk * d + gap
+    flat = [torch.full((shift + s.tokens * width,), 5.0, dtype=dt(torch, dtype), device="cuda") for _ in range(3)]
+    outs = [x[shift:].view(s.tokens, width)[:, :hk * d] for x in flat]
+    dense = [torch.empty((s.tokens, hk * d), dtype=dt(torch, dtype), device="cuda") for _ in range(3)]
+    torch.cuda.synchronize()
+    for k, v, o in (outs, dense):
+        gpu.paged_kv_read(s.cache, s.batch, k.unflatten(1, (hk, d)), v.unflatten(1, (hk, d)))
+        gpu.paged_attention(s.cache, s.batch, q, o.unflatten(1, (hk, d)))
+    for x, o, want in zip(flat, outs, dense):
+        assert torch.equal(o, want)
+        assert bool((x[:shift] == 5).all()) and bool((x[shift:].view(s.tokens, width)[:, hk * d:] == 5).all())
+
+
 def test_read_one_output_feeds_attention_f32(gpu, torch):
     """The cache taken out head-major for ATTENTION_F32 gives what PAGED_ATTENTION gives."""
     hk, d, n = 4, 128, 96
