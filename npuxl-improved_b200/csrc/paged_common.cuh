@@ -51,47 +51,33 @@ __device__ __forceinline__ void load8(const E *p, bool vec, float (&v)[8]) {
         for (uint32_t i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
     }
 }
-template <typename E>
-__device__ __forceinline__ void store8(E *p, bool vec, const float (&v)[8]) {
-    alignas(16) E e[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) from_f32(v[i], e[i]);
-    if (vec) {
-#pragma unroll
-        for (uint32_t i = 0; i < sizeof(e) / 16; ++i)
-            reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(e)[i];
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) p[i] = e[i];
-    }
-}
-
 // 8 words to a 32-byte place, a whole sector in one store: sectors that are
 // written in halves by two stores cost their way to L2 twice (read-back of 512
 // tokens of 32 heads of 128 in f32: 14.0 us in 16-byte stores, 8.4 in these; of
-// 26 000 tokens of 8 heads of 64 in f16: 14.9 and 11.7).
+// 19 000 tokens of 8 heads of 64 in f16: 14.9 and 11.7; append of f32 rows 4 to
+// 6 % less).
 __device__ __forceinline__ void store_sector(void *p, const uint32_t *r) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-// 16 consecutive elements to a place that `align` bytes divide: 32, 16, or less.
-template <typename E>
-__device__ __forceinline__ void store16(E *p, uint32_t align, const float (&v)[16]) {
-    alignas(32) E e[16];
+// N consecutive elements to a place that `align` bytes divide: 32, 16, or less.
+template <uint32_t N, typename E>
+__device__ __forceinline__ void store_n(E *p, uint32_t align, const float (&v)[N]) {
+    alignas(32) E e[N];
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) from_f32(v[i], e[i]);
-    if (align == 32) {
+    for (uint32_t i = 0; i < N; ++i) from_f32(v[i], e[i]);
+    if (sizeof(e) % 32 == 0 && align == 32) {
 #pragma unroll
         for (uint32_t i = 0; i < sizeof(e) / 32; ++i)
             store_sector(reinterpret_cast<char *>(p) + 32 * i, reinterpret_cast<const uint32_t *>(e) + 8 * i);
-    } else if (align == 16) {
+    } else if (align >= 16) {
 #pragma unroll
         for (uint32_t i = 0; i < sizeof(e) / 16; ++i)
             reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(e)[i];
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) p[i] = e[i];
+        for (uint32_t i = 0; i < N; ++i) p[i] = e[i];
     }
 }
 // The largest power of two up to 32 that divides all of these.

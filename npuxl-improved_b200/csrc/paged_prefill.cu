@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                 float x[8];
 #pragma unroll
                                 for (uint32_t k = 0; k < 8; ++k) x[k] = __uint_as_float(v[i + k]) * inv;
-                                store8(out + 32 * c + i, p.vec & 4u, x);
+                                store_n(out + 32 * c + i, p.vec & 4u ? 16u : 1u, x);
                             }
                     } else {
 #pragma unroll

@@ -465,6 +465,28 @@ def test_append_in_place_and_odd_strides(gpu, torch):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shift", [16, 8, 4, 1], ids=lambda e: f"from{e}")
+@pytest.mark.parametrize("gap", [0, 16, 8, 1], ids=lambda e: f"gap{e}")
+@pytest.mark.parametrize("spans", ["decode", "mixed"])
+def test_places_of_rotated_queries(gpu, torch, dtype, shift, gap, spans):
+    """Rotated queries to bases and rows of every alignment: the same values, nothing beside them."""
+    hq, hk, d, ps = 4, 2, 64, 16
+    s = Setup(torch, SPANS[spans], hk, d, ps)
+    rng = np.random.default_rng(6)
+    q = rows(torch, rng, s.tokens, hq * d, dtype)[0]
+    k, v = (rows(torch, rng, s.tokens, hk * d, dtype)[0] for _ in range(2))
+    width = hq * d + gap
+    flat = torch.full((shift + s.tokens * width,), 5.0, dtype=dt(torch, dtype), device="cuda")
+    out = flat[shift:].view(s.tokens, width)[:, :hq * d]
+    want = torch.empty((s.tokens, hq * d), dtype=dt(torch, dtype), device="cuda")
+    torch.cuda.synchronize()
+    for o in (out, want):
+        gpu.paged_kv_append(s.cache, s.batch, q, k, v, o, q_heads=hq)
+    assert torch.equal(out, want)
+    assert bool((flat[:shift] == 5).all()) and bool((flat[shift:].view(s.tokens, width)[:, hq * d:] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("spans", ["one", "decode", "mixed", "prefill"])
 @pytest.mark.parametrize("hk,d,ps", [(2, 128, 64), (3, 48, 16), (1, 256, 256)])
 @pytest.mark.parametrize("layout", ["rows", "heads", "gaps"])
