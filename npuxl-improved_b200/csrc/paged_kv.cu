@@ -13,8 +13,9 @@
 // Measured, bf16, 32/8 heads of 128 where not said: append of 6300 tokens in 16
 // prompts 45 us (142 MB, 3.2 TB/s; issue slots and latency, not memory), of 64
 // single tokens 5.2 us (three dependent loads); read-back, pass after pass, of
-// 19 000 tokens of 8 heads of 64 in f16 11.7 us (58 MB, 5.0 TB/s), of 512 tokens
-// of 32 heads in f32 8.4 us (21 MB; one wave of CTAs and its latency).
+// 19 000 tokens of 8 heads of 64 in f16 11.7 us of one cache and 14.3 of three in
+// turn (58 MB, 5.0 and 4.1 TB/s), of 512 tokens of 32 heads in f32 8.4 and 9.6 us
+// (21 MB; one wave of CTAs and its latency).
 #include <algorithm>
 
 #include "paged_common.cuh"
