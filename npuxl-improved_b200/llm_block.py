@@ -24,6 +24,7 @@ Two backends share the code:
 from __future__ import annotations
 
 import ctypes as C
+from contextlib import contextmanager
 from dataclasses import dataclass
 
 import numpy as np
@@ -190,8 +191,27 @@ def _cmd(op, field, args):
     return c
 
 
+@contextmanager
+def ordered_on(torch, stream):
+    """Makes the library's `stream` torch's current one, its work ordered with the caller's current
+    stream as a torch operator's is: after what that was given before, and before what it is given
+    next, so the caller may use the results, and overwrite or free the inputs, at once.  Where the
+    caller is on `stream` already (a capture) there is nothing to order."""
+    caller = torch.cuda.current_stream()
+    apart = caller.cuda_stream != stream.cuda_stream
+    if apart:
+        stream.wait_stream(caller)
+    try:
+        with torch.cuda.stream(stream):
+            yield
+    finally:
+        if apart:
+            caller.wait_stream(stream)
+
+
 class B200Block:
-    """The block with every tensor resident in HBM."""
+    """The block with every tensor resident in HBM.  forward() and replay_decode() run on the
+    library's stream, ordered with the stream that is current where they are called."""
 
     def __init__(self, cfg: BlockConfig, lib, dev, torch, fused: bool = True,
                  swiglu_epilogue: bool = True):
@@ -318,7 +338,7 @@ class B200Block:
         token; `positions` (device int32[1]) replaces pos0 for graph replay."""
         t, cfg = self.t, self.cfg
         T, d, H, hd = x.shape[0], cfg.d, cfg.heads, cfg.head_dim
-        with t.cuda.stream(self.stream):
+        with ordered_on(t, self.stream):
             if self.fused:
                 # RMSNorm -> QUANTIZE_I8, then the QKV projection with RoPE and
                 # the cache append in its epilogue (VNPU_B200_OP_QKV_ROPE_APPEND).
@@ -434,6 +454,7 @@ class B200Block:
 
     def replay_decode(self):
         """One decode step: the graph replays on the library stream, ordered
-        with everything else this block submits there."""
-        with self.t.cuda.stream(self.stream):
+        with everything else this block submits there and with the caller's
+        stream."""
+        with ordered_on(self.t, self.stream):
             self.graph.replay()
