@@ -15,7 +15,7 @@ from __future__ import annotations
 import numpy as np
 
 import vnpu
-from llm_block import BlockConfig, _cmd, make_weights
+from llm_block import BlockConfig, _cmd, make_weights, ordered_on
 
 
 class PagedBlock:
@@ -68,8 +68,8 @@ class PagedBlock:
 
     def step(self, x, counts: dict):
         """x: [tokens][d] f32 on the device, the rows of `counts`' sequences in its order;
-        counts: sequence -> its number of new tokens.  Returns [tokens][d], enqueued on the
-        library's stream."""
+        counts: sequence -> its number of new tokens.  Returns [tokens][d].  The step runs on the
+        library's stream, ordered with the stream that is current where it is called."""
         t, cfg = self.t, self.cfg
         T, d, H, hd = x.shape[0], cfg.d, cfg.heads, cfg.head_dim
         if T != sum(counts.values()) or not counts or len(counts) > self.max_batch:
@@ -81,8 +81,8 @@ class PagedBlock:
             row[:len(self.pages[s])] = self.pages[s]
         cu = np.concatenate([[0], np.cumsum(list(counts.values()))]).astype(np.int32)
         lens = np.array([self.length[s] for s in counts], np.int32)
-        with t.cuda.stream(self.stream):
-            self.stream.wait_stream(t.cuda.default_stream())     # x, and new tensors' memory
+        y = t.empty((T, d), device="cuda")        # the caller's stream's memory, as x is
+        with ordered_on(t, self.stream):
             dev = lambda a: t.from_numpy(a).cuda(non_blocking=False)  # noqa: E731
             table, cu, lens = dev(table), dev(cu), dev(lens)
             new = lambda *shape, dtype=t.float32: t.empty(shape, dtype=dtype, device="cuda")  # noqa: E731
@@ -94,10 +94,10 @@ class PagedBlock:
                 return a8, sa, vnpu.b200_command(vnpu.OP_B200_RMSNORM_QUANTIZE_I8, vnpu.RmsnormQuantizeArgs(
                     vnpu.ptr(src), vnpu.ptr(weight), None, vnpu.ptr(a8), vnpu.ptr(sa), T, K, cfg.eps, 0))
 
-            def projection(src, residual, name):
+            def projection(src, residual, name, out):
                 w, K, N = self.w[name]
-                a8, sa, out = new(T, K, dtype=t.int8), new(T), new(T, N)
-                return out, [
+                a8, sa = new(T, K, dtype=t.int8), new(T)
+                return [
                     _cmd(vnpu.OP_QUANTIZE_I8, "quantize_i8", vnpu.QuantizeI8Args(
                         vnpu.ptr(src), vnpu.ptr(a8), vnpu.ptr(sa), T, K, 0, 0)),
                     vnpu.b200_command(vnpu.OP_B200_MATMUL_I8_RESIDUAL, vnpu.MatmulI8ResidualArgs(
@@ -114,15 +114,16 @@ class PagedBlock:
                     vnpu.paged_kv_append_cmd(self.cache, batch, q, k, v, q, q_heads=H, theta=cfg.theta),
                     vnpu.paged_attention_cmd(self.cache, batch, q.unflatten(1, (H, hd)), att,
                                              max_length=int(max(self.length[s] for s in counts)))]
-            x1, more = projection(att, x, "o")
+            x1 = new(T, d)
+            more = projection(att, x, "o", x1)
             w, K, N = self.w["gate_up"]
             b8, sb, pre = norm(x1, self.n2, "gate_up")
             ff = new(T, cfg.inter)
-            y, last = projection(ff, x1, "down")
+            last = projection(ff, x1, "down", y)
             cmds += more + [pre, vnpu.b200_command(vnpu.OP_B200_MATMUL_I8_SWIGLU, vnpu.MatmulI8SwigluArgs(
                 vnpu.ptr(b8), w, vnpu.ptr(sb), None, vnpu.ptr(ff), T, K, N, 0, 0, 0, 1.0, 0))] + last
             self.lib.check(self.dev.submit(cmds), "submit")
-            # the stream's tensors are the caching allocator's on this stream: they may go now
+            # all but x and y is the caching allocator's memory of this stream: it may go now
         return y
 
 

@@ -115,3 +115,48 @@ def test_block_replay_is_ordered_with_the_callers_stream(b200_lib, torch, held, 
     want = run_replay(b200_lib, torch, None, caller)
     for a, b in zip(run_replay(b200_lib, torch, held, caller), want):
         assert torch.equal(a, b)
+
+
+def run_paged(b200_lib, torch, held, caller):
+    from llm_block import BlockConfig
+    from llm_paged import PagedBlock
+    cfg = BlockConfig(d=256, heads=4, inter=704, cap=64)
+    gen = torch.Generator().manual_seed(3)
+    prompts = {"a": 20, "b": 1, "c": 33}
+    late, outs = Late(torch, held), []
+    with vnpu.Device(b200_lib) as dev:
+        blk = PagedBlock(cfg, b200_lib, dev, torch, pages=24, page_size=16)
+        stream, submit = caller_stream(torch, caller), dev.submit
+
+        def submit_late(cmds, event=None):
+            late.here("library", blk.stream)
+            return submit(cmds, event)
+
+        dev.submit = submit_late
+        sources = [torch.randn((n, cfg.d), generator=gen).cuda() for n in [54] + [3] * 6]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for i, source in enumerate(sources):
+                late.here("caller", stream)
+                x = source * 1
+                late.done()
+                y = blk.step(x, dict(prompts) if i == 0 else dict.fromkeys(prompts, 1))
+                late.done()
+                outs.append(y * 1)
+                y.fill_(float("nan"))
+                del x, y
+                for _ in range(3):            # of the sizes of x and y, in their places
+                    torch.full((source.shape[0], cfg.d), float("nan"), device="cuda")
+        torch.cuda.synchronize()
+        assert dev.sync() == vnpu.OK
+        blk.close()
+    return outs
+
+
+@pytest.mark.parametrize("held", ["caller", "library"])
+@pytest.mark.parametrize("caller", ["default", "own"])
+def test_paged_steps_of_temporaries(b200_lib, torch, held, caller):
+    """Inputs and outputs that go as soon as they are used, no sync between steps."""
+    want = run_paged(b200_lib, torch, None, caller)
+    for a, b in zip(run_paged(b200_lib, torch, held, caller), want):
+        assert torch.equal(a, b)
