@@ -72,8 +72,13 @@ class PagedBlock:
         library's stream, ordered with the stream that is current where it is called."""
         t, cfg = self.t, self.cfg
         T, d, H, hd = x.shape[0], cfg.d, cfg.heads, cfg.head_dim
-        if T != sum(counts.values()) or not counts or len(counts) > self.max_batch:
+        if T != sum(counts.values()) or not counts or len(counts) > self.max_batch or min(counts.values()) < 0:
             raise ValueError("rows of x and counts differ, or the batch is too large")
+        if x.dtype != t.float32 or tuple(x.shape) != (T, d) or not x.is_contiguous() or not x.is_cuda:
+            raise ValueError(f"x: contiguous float32 of shape {(T, d)} on the device, got {x.dtype} "
+                             f"{tuple(x.shape)} with strides {x.stride()} on {x.device}")
+        if T == 0:
+            return t.empty((0, d), device="cuda")
         self._grow(counts)
         width = max(len(self.pages[s]) for s in counts)
         table = np.full((len(counts), width), -1, np.int32)
