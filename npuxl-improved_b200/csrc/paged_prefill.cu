@@ -58,6 +58,7 @@ struct Plan {
     uint32_t *seq_base;    // [batch + 1]: blocks before sequence b
     RowBlock *blocks;
     uint32_t *before;      // cost of the blocks before block e (one head)
+    uint32_t capacity;     // entries of `blocks` and `before`
 };
 
 template <uint32_t KT>
@@ -73,38 +74,42 @@ __device__ __forceinline__ RowBlock block_tiles(const AttnParams &p, const Paged
 }
 
 // Exclusive prefix of x over the block, and the sum.
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *sh, uint32_t *total) {
+__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t *sh, uint64_t *total) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    uint32_t v = x;
+    uint64_t v = x;
 #pragma unroll
     for (uint32_t o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, v, o);
+        const uint64_t y = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += y;
     }
     if (lane == 31) sh[warp] = v;
     __syncthreads();
     if (warp == 0) {
-        uint32_t w = sh[lane];
+        uint64_t w = sh[lane];
 #pragma unroll
         for (uint32_t o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, w, o);
+            const uint64_t y = __shfl_up_sync(0xffffffffu, w, o);
             if (lane >= o) w += y;
         }
         sh[lane] = w;
     }
     __syncthreads();
-    const uint32_t base = warp ? sh[warp - 1] : 0;
+    const uint64_t base = warp ? sh[warp - 1] : 0;
     *total = sh[31];
     __syncthreads();
     return base + v - x;
 }
 
+// Sequences are looked at one by one, and rows that do not fall share no rows:
+// their blocks are within the capacity.  Where the numbers do fall, the same rows
+// can count many times over; no entry of the plan is written before the sum is
+// known to fit.
 template <uint32_t KT>
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const AttnParams p, const Plan plan) {
-    __shared__ uint32_t sh[32];
+    __shared__ uint64_t sh[32];
     pdl_enter();
     const uint32_t tid = threadIdx.x, batch = p.pb.batch;
-    uint32_t blocks = 0, total;
+    uint64_t blocks = 0, total;
     for (uint32_t b0 = 0; b0 < batch; b0 += kPlanThreads) {
         const uint32_t b = b0 + tid;
         uint32_t mine = 0;
@@ -113,13 +118,21 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const AttnPara
             if (!load_seq(p.pb, p.c.page_shift, b, s)) record_error(p.err, kErrBadIndex);
             else mine = (static_cast<uint32_t>(s.n) * p.group + kRows - 1) / kRows;
         }
-        const uint32_t at = blocks + block_scan(mine, sh, &total);
-        if (b < batch) plan.seq_base[b] = at;
+        const uint64_t at = blocks + block_scan(mine, sh, &total);
+        if (b < batch) plan.seq_base[b] = static_cast<uint32_t>(at);
         blocks += total;
     }
-    if (tid == 0) plan.seq_base[batch] = blocks;
+    if (blocks > plan.capacity) {       // nothing is done
+        if (tid == 0) {
+            record_error(p.err, kErrBadIndex);
+            plan.head[0] = 0;
+            plan.head[1] = 0;
+        }
+        return;
+    }
+    if (tid == 0) plan.seq_base[batch] = static_cast<uint32_t>(blocks);
     __syncthreads();
-    uint32_t tiles = 0;
+    uint64_t tiles = 0;
     for (uint32_t e0 = 0; e0 < blocks; e0 += kPlanThreads) {
         const uint32_t e = e0 + tid;
         RowBlock x{0, 0, 0, 0};
@@ -135,13 +148,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const AttnPara
             x = block_tiles<KT>(p, s, lo, e - plan.seq_base[lo]);
             plan.blocks[e] = x;
         }
-        const uint32_t at = tiles + block_scan(e < blocks ? static_cast<uint32_t>(x.nt + kBlockCost) : 0u, sh, &total);
-        if (e < blocks) plan.before[e] = at;
+        const uint64_t at = tiles + block_scan(e < blocks ? static_cast<uint32_t>(x.nt + kBlockCost) : 0u, sh, &total);
+        if (e < blocks) plan.before[e] = static_cast<uint32_t>(at);
         tiles += total;
     }
     if (tid == 0) {
-        plan.head[0] = blocks;
-        plan.head[1] = tiles;
+        plan.head[0] = static_cast<uint32_t>(blocks);
+        plan.head[1] = static_cast<uint32_t>(tiles);
     }
 }
 
@@ -951,6 +964,7 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     p.ws_ml = reinterpret_cast<float2 *>(carve(ml_bytes));
     p.ws_meta = reinterpret_cast<uint4 *>(carve(meta_bytes));
     Plan plan;
+    plan.capacity = static_cast<uint32_t>(blocks);   // below 2^23 + 2^24
     plan.blocks = reinterpret_cast<RowBlock *>(carve(block_bytes));
     plan.before = reinterpret_cast<uint32_t *>(carve(before_bytes));
     plan.seq_base = reinterpret_cast<uint32_t *>(carve(seq_bytes));
