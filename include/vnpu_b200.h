@@ -318,8 +318,9 @@ typedef struct vnpu_b200_paged_cache_t {
  * What the arrays say is checked on the device: a sequence whose rows exceed
  * max_tokens, `tokens` or its length, or a page outside the cache or the
  * table, is not touched (its cached tokens and outputs that would depend on
- * them are left out or zero) and sets the stream's device error.  tokens = 0
- * or batch = 0 is no work.
+ * them are left out or zero) and sets the stream's device error.  Where
+ * cu_tokens falls, so that rows count for several sequences, a command may be
+ * left out whole.  tokens = 0 or batch = 0 is no work.
  */
 typedef struct vnpu_b200_paged_batch_t {
     const int32_t *block_table;   /* [batch][table_stride] */
@@ -406,6 +407,8 @@ typedef struct vnpu_b200_paged_kv_read_args_t {
  * that attends to nothing has the output 0.  Scores, softmax sums and
  * accumulators are 32 bits wide; the softmax weights enter the value product
  * as 16-bit floats for 16-bit outputs, and as two of them (22 bits) for f32.
+ * A command that takes 2^32 steps of 256 query rows by 64 or 128 keys or more,
+ * a minute's work at least, is left out and sets the stream's device error.
  * max_length, when not 0, is the longest seq_lens[b] to expect, for the
  * device's byte and flop counters; the kernels read the lengths themselves.
  * Scratch (partial sums of rows that are split over the GPU) is stream-ordered,

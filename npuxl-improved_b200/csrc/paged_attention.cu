@@ -178,7 +178,9 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     }
     const unsigned long long run = max(1ull, (total + gridDim.x - 1) / gridDim.x);
     const unsigned long long t0 = run * cta;
-    if (t0 >= total) {
+    const bool countable = run <= 0xffffffffu;   // a run's units are counted in 32 bits; more are an hour's work
+    if (t0 >= total || !countable) {
+        if (tid == 0 && !countable) record_error(p.err, kErrBadIndex);
         if (tid == 0 && p.ws_meta) p.ws_meta[2 * cta].x = 0;
         return;
     }

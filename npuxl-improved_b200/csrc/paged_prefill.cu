@@ -152,9 +152,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const AttnPara
         if (e < blocks) plan.before[e] = static_cast<uint32_t>(at);
         tiles += total;
     }
+    // A run's units, and so all of them, are counted in 32 bits: more than 2^32 tiles of 256 rows,
+    // a minute's work, are refused.
+    const bool fits = tiles <= 0xffffffffu / p.c.heads;
     if (tid == 0) {
-        plan.head[0] = static_cast<uint32_t>(blocks);
-        plan.head[1] = static_cast<uint32_t>(tiles);
+        if (!fits) record_error(p.err, kErrBadIndex);
+        plan.head[0] = fits ? static_cast<uint32_t>(blocks) : 0;
+        plan.head[1] = fits ? static_cast<uint32_t>(tiles) : 0;
     }
 }
 

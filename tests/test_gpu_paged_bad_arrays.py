@@ -84,3 +84,24 @@ def test_bad_numbers_of_many_rows(b200_lib, gpu, torch, dtype, what):
         check_attention(o[:70], want[:70], size[:70], top[:70], dtype)
         assert bool((o[70:] == 7).all())
     assert bool(torch.isfinite(o).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_steps_than_can_be_counted(b200_lib, torch, dtype):
+    """Every page the same one, 2^31 keys, 256 and 512 blocks of rows: nearly 2^33 steps of 256
+    rows by a tile of keys.  Left out and reported, nothing is written."""
+    n = 1024 if dtype == "f32" else 2048                   # tiles of 64 and of 128 keys
+    heads, d, ps, length = 64, 16, 256, 0x7fffff00
+    codes = torch.zeros((1, 1, ps, d), dtype=torch.int8, device="cuda")
+    scale = torch.ones((1, 1), device="cuda")
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.zeros((1, length // ps + 1), dtype=torch.int32, device="cuda")
+    q = torch.zeros((n, heads, d), device="cuda").to(torch.bfloat16 if dtype == "bf16" else torch.float32)
+    flat, o = guarded(torch, n, heads, d, q.dtype)
+    assert (n * heads // 256) * ((length - n) // (64 if dtype == "f32" else 128)) >= 2 ** 32
+    torch.cuda.synchronize()
+    _, sync = _status(b200_lib, vnpu.paged_attention_cmd(
+        vnpu.paged_cache(codes, codes, scale, scale),
+        vnpu.paged_batch(table, ints(0, n), ints(length), n), q, o))
+    assert sync == vnpu.ERR_DEVICE_ERROR
+    assert bool((flat == 7).all())
