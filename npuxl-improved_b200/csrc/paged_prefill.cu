@@ -57,8 +57,9 @@ struct Plan {
     uint32_t *head;        // [0]: blocks, [1]: cost of one head's
     uint32_t *seq_base;    // [batch + 1]: blocks before sequence b
     RowBlock *blocks;
+    PagedSeq *seqs;        // block e's sequence
     uint32_t *before;      // cost of the blocks before block e (one head)
-    uint32_t capacity;     // entries of `blocks` and `before`
+    uint32_t capacity;     // entries of `blocks`, `seqs` and `before`
 };
 
 template <uint32_t KT>
@@ -147,6 +148,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const AttnPara
             load_seq(p.pb, p.c.page_shift, lo, s);
             x = block_tiles<KT>(p, s, lo, e - plan.seq_base[lo]);
             plan.blocks[e] = x;
+            plan.seqs[e] = s;
         }
         const uint64_t at = tiles + block_scan(e < blocks ? static_cast<uint32_t>(x.nt + kBlockCost) : 0u, sh, &total);
         if (e < blocks) plan.before[e] = static_cast<uint32_t>(at);
@@ -251,6 +253,7 @@ struct ManyShape {
 // Where a CTA stands in its run: head, block, tiles; the roles walk alike.  A
 // block is kBlockCost units, then one for each key tile; a CTA has the tiles
 // whose units are in its run.
+static_assert(sizeof(RowBlock) == 16 && sizeof(PagedSeq) == 16, "read as one word each");
 struct Walk {
     uint32_t left, h, e, blocks;    // units left; current head and block
     int32_t used;                   // units of this segment
@@ -270,7 +273,12 @@ struct Walk {
         const int32_t first = max(0, from - kBlockCost);
         tile = x.lo + first;
         count = max(0, from + used - kBlockCost) - first;
-        load_seq(p.pb, p.c.page_shift, x.b, s);
+        // the numbers that the plan looked at, whatever the arrays hold by now
+        const int4 u = __ldcg(reinterpret_cast<const int4 *>(plan.seqs) + e);
+        s.row0 = u.x;
+        s.n = u.y;
+        s.start = u.z;
+        s.len = u.w;
     }
     // The next segment that has tiles.
     __device__ __forceinline__ bool next(const AttnParams &p, const Plan &plan) {
@@ -953,10 +961,12 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     const size_t ml_bytes = pad(2ull * grid * kRows * sizeof(float2));
     const size_t meta_bytes = pad(2ull * grid * sizeof(uint4));
     const size_t block_bytes = pad(blocks * sizeof(RowBlock)), before_bytes = pad(blocks * sizeof(uint32_t));
+    const size_t seqs_bytes = pad(blocks * sizeof(PagedSeq));
     const size_t seq_bytes = pad((a.batch.batch + 1ull) * sizeof(uint32_t));
     char *ws = nullptr;
     VNPU_LAUNCH(cudaMallocAsync(reinterpret_cast<void **>(&ws),
-                                o_bytes + ml_bytes + meta_bytes + block_bytes + before_bytes + seq_bytes + 256,
+                                o_bytes + ml_bytes + meta_bytes + block_bytes + seqs_bytes + before_bytes + seq_bytes +
+                                    256,
                                 ctx.stream));
     char *at = ws;
     const auto carve = [&](size_t n) {
@@ -970,6 +980,7 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     Plan plan;
     plan.capacity = static_cast<uint32_t>(blocks);   // below 2^23 + 2^24
     plan.blocks = reinterpret_cast<RowBlock *>(carve(block_bytes));
+    plan.seqs = reinterpret_cast<PagedSeq *>(carve(seqs_bytes));
     plan.before = reinterpret_cast<uint32_t *>(carve(before_bytes));
     plan.seq_base = reinterpret_cast<uint32_t *>(carve(seq_bytes));
     plan.head = reinterpret_cast<uint32_t *>(at);
