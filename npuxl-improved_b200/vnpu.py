@@ -328,13 +328,16 @@ def _paged_dtype(*tensors) -> int:
 
 
 def _int32(name, t):
-    if not str(t.dtype).endswith("int32"):
+    if str(t.dtype) != "torch.int32":
         raise TypeError(f"{name}: int32, got {t.dtype}")
     return t
 
 
-def _row_stride(name, t, width: int) -> int:
-    """Row stride in elements of a [rows][width] or [rows][heads][dim] tensor, rows dense inside."""
+def _row_stride(name, t, width: int, rows: int) -> int:
+    """Row stride in elements of a [rows][width] or [rows][heads][dim] tensor of at least `rows`
+    rows, dense inside."""
+    if t.shape[0] < rows:
+        raise ValueError(f"{name}: {rows} rows, got {t.shape[0]}")
     inner = 1
     for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
         if n > 1 and st != inner:
@@ -343,6 +346,8 @@ def _row_stride(name, t, width: int) -> int:
         inner *= n
     if inner != width:
         raise ValueError(f"{name}: rows of {width} elements, got {inner}")
+    if t.shape[0] > 1 and t.stride(0) < width:   # one row for all (0) would read as dense rows
+        raise ValueError(f"{name}: rows that do not overlap, got strides {tuple(t.stride())}")
     return t.stride(0) if t.shape[0] > 1 else width
 
 
@@ -353,7 +358,7 @@ def paged_cache(k, v, k_scale, v_scale) -> PagedCache:
     for name, t, shape, kind in (("k", k, tuple(k.shape), "int8"), ("v", v, tuple(k.shape), "int8"),
                                  ("k_scale", k_scale, (pages, heads), "float32"),
                                  ("v_scale", v_scale, (pages, heads), "float32")):
-        if tuple(t.shape) != shape or not str(t.dtype).endswith(kind) or not t.is_contiguous():
+        if tuple(t.shape) != shape or str(t.dtype) != "torch." + kind or not t.is_contiguous():
             raise ValueError(f"{name}: contiguous {kind} of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     return PagedCache(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), pages, heads, page_size, head_dim)
 
@@ -368,6 +373,9 @@ def paged_batch(block_table, cu_tokens, seq_lens, tokens: int, max_tokens: int =
         _int32(name, t)
         if t.shape and t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"{name}: entries lie one after the other")
+    if n > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError(f"block_table: rows of its own for each sequence, got strides "
+                         f"{tuple(block_table.stride())}")
     stride = block_table.stride(0) if n > 1 else block_table.shape[1]
     return PagedBatch(ptr(block_table), ptr(cu_tokens), ptr(seq_lens), n, stride, tokens, max_tokens)
 
@@ -377,12 +385,13 @@ def paged_kv_append_cmd(cache: PagedCache, batch: PagedBatch, q, k, v, q_out, *,
                         theta: float = 10000.0, scaling: float = 1.0) -> "Command":
     """VNPU_B200_OP_PAGED_KV_APPEND: rotates q into q_out (or q None: no queries) and k, and
     appends k and v ([tokens][heads * head_dim], row-strided views allowed) to the cache."""
-    d, h = cache.head_dim, cache.heads
+    d, h, n = cache.head_dim, cache.heads, batch.tokens
     flags = (PAGED_INTERLEAVED if interleaved else 0) | (0 if rope else PAGED_NO_ROPE)
     return b200_command(OP_B200_PAGED_KV_APPEND, PagedKvAppendArgs(
         cache, batch, ptr(q), ptr(k), ptr(v), ptr(q_out),
-        _row_stride("q", q, q_heads * d) if q is not None else 0, _row_stride("k", k, h * d),
-        _row_stride("v", v, h * d), _row_stride("q_out", q_out, q_heads * d) if q_out is not None else 0,
+        _row_stride("q", q, q_heads * d, n) if q is not None else 0, _row_stride("k", k, h * d, n),
+        _row_stride("v", v, h * d, n),
+        _row_stride("q_out", q_out, q_heads * d, n) if q_out is not None else 0,
         q_heads, _paged_dtype(q, k, v, q_out), flags, rotary_dim, theta, scaling))
 
 
@@ -391,20 +400,23 @@ def paged_kv_read_cmd(cache: PagedCache, batch: PagedBatch, k_out, v_out) -> "Co
     layout with dense head_dim (token-major, or head-major through a transposed view)."""
     outs = [t for t in (k_out, v_out) if t is not None]
     if not outs or any(tuple(t.shape[1:]) != (cache.heads, cache.head_dim) or t.stride(2) != 1 or
-                       t.stride() != outs[0].stride() for t in outs):
+                       t.shape[0] < batch.tokens or t.stride() != outs[0].stride() for t in outs):
         raise ValueError("k_out, v_out: [tokens][heads][head_dim] of one layout, dense head_dim")
+    # a stride of a single row or head says nothing; 0 of several would read as dense
+    strides = [t.stride(i) if t.shape[i] > 1 else 0 for t in outs[:1] for i in (0, 1)]
+    if any(st == 0 and outs[0].shape[i] > 1 for i, st in enumerate(strides)):
+        raise ValueError(f"k_out, v_out: rows and heads of their own, got strides {outs[0].stride()}")
     return b200_command(OP_B200_PAGED_KV_READ, PagedKvReadArgs(
-        cache, batch, ptr(k_out), ptr(v_out), outs[0].stride(0), outs[0].stride(1),
-        _paged_dtype(*outs), 0))
+        cache, batch, ptr(k_out), ptr(v_out), *strides, _paged_dtype(*outs), 0))
 
 
 def paged_attention_cmd(cache: PagedCache, batch: PagedBatch, q, o, *, causal: bool = True,
                         window: int = 0, scale: float = 0.0, max_length: int = 0) -> "Command":
     """VNPU_B200_OP_PAGED_ATTENTION: q, o [tokens][q_heads][head_dim] (rows may be strided)."""
-    heads = q.shape[1]
+    heads, n = q.shape[1], batch.tokens
     width = heads * cache.head_dim
     return b200_command(OP_B200_PAGED_ATTENTION, PagedAttentionArgs(
-        cache, batch, ptr(q), ptr(o), _row_stride("q", q, width), _row_stride("o", o, width), heads,
+        cache, batch, ptr(q), ptr(o), _row_stride("q", q, width, n), _row_stride("o", o, width, n), heads,
         _paged_dtype(q, o), int(causal), window, max_length, scale))
 
 
