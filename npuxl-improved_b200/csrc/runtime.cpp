@@ -1153,8 +1153,17 @@ void exec_paged_kv_read(vnpu_stream_t *s, const vnpu_command_t &cmd, const Launc
         p.ld_row < d || (T > 1 && h > 1 && p.ld_row < row_extent && p.ld_head < head_extent))
         throw CommandError("paged_kv_read strides", VNPU_ERR_INVALID_ARGUMENT);
     const uint64_t span = ((T - 1) * p.ld_row + (h - 1) * p.ld_head + d) * elem;
-    p.K_out = st.out(static_cast<char *>(a.K_out), span, true);  // gaps survive staging
-    p.V_out = st.out(static_cast<char *>(a.V_out), span, true);
+    // Gaps survive staging.  Outputs in each other's gaps are staged as one: apart, the copy back of
+    // the second would bring back what the first one's places held before.
+    char *const K = static_cast<char *>(a.K_out), *const V = static_cast<char *>(a.V_out);
+    if (K && V && K < V + span && V < K + span) {
+        char *const low = std::min(K, V), *const both = st.out(low, std::max(K, V) - low + span, true);
+        p.K_out = both + (K - low);
+        p.V_out = both + (V - low);
+    } else {
+        p.K_out = st.out(K, span, true);
+        p.V_out = st.out(V, span, true);
+    }
     p.type = paged_row_type(a.dtype);
     cuda_check(paged_kv_read(ctx, p), "paged_kv_read launch");
     st.finish();
