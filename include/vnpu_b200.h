@@ -288,7 +288,8 @@ typedef struct vnpu_b200_matmul_i8_swiglu_args_t {
  * counterpart: the reference has no KV cache).  K and V hold int8 codes,
  * [num_pages][heads][page_size][head_dim]; K_scale and V_scale one f32 for
  * each page and head, [num_pages][heads]; a cached value is code * scale.
- * Scales are not negative; a page of zeros may have the scale 0.  All four are
+ * Scales are not negative; a page of zeros may have the scale 0, which
+ * PAGED_ATTENTION takes V scales below 2^-96 for.  All four are
  * device memory, owned by the caller, the codes 16-byte aligned;
  * nothing needs to be cleared before a page's first use.  page_size is a power
  * of two from 16 to 256, head_dim a multiple of 16 up to 256.

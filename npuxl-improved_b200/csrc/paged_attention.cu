@@ -443,8 +443,8 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const float vs = sc[2 + i];
-            on[i] = vs > 0.0f;                 // a page of zeros has the scale 0
-            lv[i] = on[i] ? __log2f(vs) : 0.0f;
+            on[i] = vs >= kLeastScale;         // else a page of zeros, or nothing that is seen
+            lv[i] = on[i] ? __log2f(vs) : kZeroLog;
             iv[i] = on[i] ? ex2(-lv[i]) : 1.0f;
         }
         const bool edge = k0 + static_cast<int32_t>(kWarpKeys) - 1 > kmax_first || k0 < kmin_last;
@@ -491,6 +491,14 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) acc[t][j][e] *= f[e & 1];
             }
+        }
+        if (!(on[0] && on[1])) {               // warp-uniform: those count as they are
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) s[i][t][e] -= on[i] ? 0.0f : kZeroLog;
         }
         uint32_t pb[2][NT][2], pl[2][kSplit ? NT : 1][2];
 #pragma unroll
@@ -613,7 +621,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
             }
             if (started && !more) {
                 const uint32_t r = cur.rt * MR + row, token = token_of(p, r);
-                const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+                const float inv = inverse_sum(ll);
                 E *out = static_cast<E *>(p.O) +
                          static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldo +
                          (cur.h * p.group + (r - token * p.group)) * D + 4u * d4;
@@ -722,7 +730,7 @@ __global__ void __launch_bounds__(256) paged_attention_join_kernel(const AttnPar
         o.z += v.z * f;
         o.w += v.w * f;
     }
-    const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+    const float inv = inverse_sum(ll);
     const uint32_t r = meta.z + row, token = token_of(p, r);
     E *out = static_cast<E *>(p.O) + static_cast<uint64_t>(meta.y + token) * p.ldo +
              (meta.w * p.group + (r - token * p.group)) * p.c.head_dim + 4u * d4;

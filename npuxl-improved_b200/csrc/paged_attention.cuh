@@ -16,6 +16,15 @@ namespace {
 // mathematics) and the parameters.
 constexpr float kSlack = 6.0f;       // growth of the maximum before a rescale (log2)
 constexpr float kLift = 8.0f;        // weights are scaled by 2^8: small ones stay normal numbers
+// A page of zeros (V scale 0, or below kLeastScale: values below 2^-89) counts in the sum l alone,
+// with the weight 2^(s - m + 8) of its score.  For the maximum m it stands in with a scale of
+// 2^kZeroLog: m is then the others' wherever they are seen in the output (2^-8 below, a weight still
+// has its 22 bits), and l stays below 2^102 a key.
+constexpr float kLeastScale = 0x1p-96f;
+constexpr float kZeroLog = -88.0f;
+
+// 1 / l of a row: 0 where it saw nothing, NaN where it is NaN.
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
 struct AttnParams {
     PagedCache c;

@@ -310,8 +310,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     __shared__ uint64_t bar_k[2], bar_k_free[2], bar_v[2], bar_v_free[2];   // f16 tiles
     __shared__ uint64_t bar_r[kRawRing], bar_r_free[kRawRing];              // codes
     __shared__ uint64_t bar_sc[kScaleRing];
-    // a tile's 16-key groups: K scale, log2 of the V scale, 1 / V scale; pages of zeros as bits
-    __shared__ __align__(16) float sh_k[kScaleRing][8], sh_lv[kScaleRing][8], sh_iv[kScaleRing][8];
+    // a tile's 16-key groups: K scale, log2 of the V scale (for the maximum, and for the weights),
+    // 1 / V scale; pages of zeros as bits
+    __shared__ __align__(16) float sh_k[kScaleRing][8], sh_top[kScaleRing][8], sh_lv[kScaleRing][8], sh_iv[kScaleRing][8];
     __shared__ uint32_t sh_zeros[kScaleRing];
     __shared__ uint32_t sh_tmem;
     __shared__ int sh_abort;
@@ -501,7 +502,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const uint32_t r = cur.x.rb * kRows + row, token = token_of(p, r);
                 const bool live = r < static_cast<uint32_t>(cur.s.n) * p.group;
                 const uint32_t part = 2 * cta + (started ? 1 : 0);
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const float inv = inverse_sum(l);
                 E *out = static_cast<E *>(p.O) +
                          static_cast<uint64_t>(cur.s.row0 + static_cast<int32_t>(token)) * p.ldo +
                          (cur.h * p.group + (r - token * p.group)) * D;
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         const float y4 = max3(score(12), score(13), score(14));
                         // scales are not negative: the largest product is the largest score
                         top = fmaxf(top, fmaf(fmaxf(max3(y0, y1, y2), max3(y3, y4, score(15))),
-                                              factor(4 * c + g), sh_lv[ring][4 * c + g]));
+                                              factor(4 * c + g), sh_top[ring][4 * c + g]));
                     }
                 }
                 if (__any_sync(0xffffffffu, top > m + kSlack)) {
@@ -834,7 +835,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const uint64_t at = now.page >= 0 ? static_cast<uint64_t>(now.page) * p.c.heads + now.h : 0;
             const uint32_t there = __ballot_sync(0xffffffffu, now.page >= 0);
             const uint64_t src = ((at << p.c.page_shift) + now.slot) * D;
-            const uint32_t zeros = __ballot_sync(0xffffffffu, lane < kGroups && !(now.vs > 0.0f));
+            const uint32_t zeros = __ballot_sync(0xffffffffu, lane < kGroups && !(now.vs >= kLeastScale));
 #pragma unroll 1
             for (uint32_t part = 0; part < 2; ++part) {
                 constexpr uint32_t kPart = kGroups / 2;      // groups of half a tile
@@ -858,10 +859,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 }
                 if (part == 0 && !values_too) {
                     if (lane < kGroups) {
-                        const float lv = now.vs > 0.0f ? __log2f(now.vs) : 0.0f;   // a page of zeros has the scale 0
+                        const bool on = now.vs >= kLeastScale;   // else a page of zeros
+                        const float lv = on ? __log2f(now.vs) : 0.0f;
                         sh_k[ring][lane] = now.ks;
+                        sh_top[ring][lane] = on ? lv : kZeroLog;
                         sh_lv[ring][lane] = lv;
-                        sh_iv[ring][lane] = now.vs > 0.0f ? ex2(-lv) : 1.0f;
+                        sh_iv[ring][lane] = ex2(-lv);
                     }
                     if (lane == 0) sh_zeros[ring] = zeros;
                     __syncwarp();
@@ -915,7 +918,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const AttnParam
             o.z = o.z * f + v.z * g;
             o.w = o.w * f + v.w * g;
         }
-        const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+        const float inv = inverse_sum(ll);
         const uint32_t r = meta.z + row, token = token_of(p, r);
         E *out = static_cast<E *>(p.O) + static_cast<uint64_t>(meta.y + token) * p.ldo +
                  (meta.w * p.group + (r - token * p.group)) * p.c.head_dim + 4u * d4;
