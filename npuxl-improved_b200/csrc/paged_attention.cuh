@@ -39,6 +39,7 @@ struct AttnParams {
     float *ws_o;           // [2 * grid][tile rows][DP] partial sums
     float2 *ws_ml;         // [2 * grid][tile rows] their m and l
     uint4 *ws_meta;        // [2 * grid]: who joins what
+    float *ws_run;         // many f32 rows: [grid][DP][tile rows] sums of a run's earlier key tiles
     uint32_t *err;
     uint64_t limit_ns;
 };
@@ -48,6 +49,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// A part's factor where the maximum of all is `all`: one that saw no key holds zeros (or the NaN of its
+// query), taken as they are.
+__device__ __forceinline__ float row_factor(float m, float all) { return m == -INFINITY ? 1.0f : ex2(m - all); }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);

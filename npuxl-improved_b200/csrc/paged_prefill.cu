@@ -17,7 +17,10 @@
 //
 // f32 rows: Q = hi + lo in f16 (22 bits), P likewise; each product is two
 // tensor instructions on the same accumulator, with tiles of 64 keys so that S
-// and both halves of P fit beside each other.
+// and both halves of P fit beside each other.  The tensor core's sums are not
+// rounded to nearest, which over the steps of a long run is a drift (at 131072
+// keys 3e-4 of the output): every kRunTiles tiles O moves to a sum in memory,
+// added in f32, a thread a row.
 //
 // What bounds it: at head_dim 128 a 256 x 128 tile costs 32768 exponentials at
 // 16 a clock (2048 clocks) against 2048 clocks of the tensor core, with about
@@ -43,6 +46,9 @@ constexpr uint32_t kManyThreads = 640;       // 8 softmax, 8 converter, tensor-i
 constexpr uint32_t kScaleRing = 4;           // tiles whose scales are kept
 constexpr uint32_t kRawRing = 4;             // half tiles of codes: two of K, two of V
 constexpr uint32_t kPlanThreads = 1024;
+// f32 rows: tiles whose O the tensor core adds up.  2048 tokens over 32768 keys, 32/8 heads of 128, in us, and
+// the drift: all 2400 and 8e-5, 32 tiles 2440 and 5e-6, 16 tiles 2520 and 2.7e-6, 8 tiles 2700 and 1.3e-6.
+constexpr int32_t kRunTiles = 16;
 // What the start and the end of a block cost beside its key tiles, in tiles: runs are of equal cost.
 // (8 ragged prompts, 32/8 heads: 308 us with 0, 263 with 2, 255 with 3, 258 with 5, 270 with 8.)
 constexpr int32_t kBlockCost = 3;
@@ -295,7 +301,8 @@ struct Walk {
     }
 };
 
-template <RowType T, uint32_t DP>
+// kRuns: f32 rows whose runs may pass kRunTiles tiles (the code for that costs the others a tenth).
+template <RowType T, uint32_t DP, bool kRuns>
 __global__ void __launch_bounds__(kManyThreads, 1)
     paged_prefill_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ Plan plan) {
     using E = typename RowOf<T>::type;
@@ -487,7 +494,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             return half == 0 || static_cast<uint32_t>(k.s.n) * p.group > k.x.rb * kRows + kHalf;
         };
         uint32_t tile_no = 0, done = 0, seg = 0;  // tiles of the run; tiles and segments of this half
-        float m = 0.0f, l = 0.0f;
+        float m = 0.0f, l = 0.0f, m_run = 0.0f;   // m_run: the maximum that the sums in memory go by
+        float *const run_sums = p.ws_run + (static_cast<uint64_t>(cta) * DP * kRows + row);
+        const auto read_sums = [&](uint32_t c, float (&had)[32]) {
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) had[i] = run_sums[(32 * c + i) * kRows];
+        };
         bool more = true, ok = true, write = false;
         Walk cur = w;                             // the segment in work, whose output comes last
         for (;;) {
@@ -514,6 +526,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     tmem_ld_32cols(lanes + Shape::kOCol + 32 * c, v);
                     tmem_wait_ld();
                     if (!live) continue;
+                    if (kRuns && cur.count > kRunTiles) {
+                        float had[32];
+                        read_sums(c, had);
+                        const float k = row_factor(m_run, m);
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i)
+                            v[i] = __float_as_uint(fmaf(had[i], k, __uint_as_float(v[i])));
+                    }
                     if (whole) {
 #pragma unroll
                         for (uint32_t i = 0; i < 32; i += 8)
@@ -558,103 +578,124 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             row_limits(p, cur.s, cur.x.rb * kRows + half * kHalf + kHalf - 1, kmin_last, unused);
             m = -INFINITY;
             l = 0.0f;
-            for (int32_t j = 0; j < cur.count; ++j, ++tile_no, ++done) {
-                const int32_t k0 = (cur.tile + j) * static_cast<int32_t>(KT);
-                const uint32_t ring = tile_no % kScaleRing;
-                const bool edge = k0 + static_cast<int32_t>(KT) - 1 > kmax_first || k0 < kmin_last;
-                if (!(ok = wait_warp(&bar_sc[ring], tile_no / kScaleRing) && wait_warp(full_s, done))) break;
-                tc_fence_after();
-                const uint32_t zeros = sh_zeros[ring];
-                // Loops over 64 keys are not unrolled: the code of all roles has to stay in the
-                // instruction caches (unrolled, a fifth of the stalls were for instructions).
-                const auto read = [&](uint32_t c, uint32_t (&x)[64]) {
-                    tmem_ld_32cols(lanes + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(x));
-                    tmem_ld_32cols(lanes + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
-                    tmem_wait_ld();
-                    if (edge) {   // bits of the keys that the row sees
-                        const int64_t lo = max(0, min(64, kmin - k0 - static_cast<int32_t>(64 * c)));
-                        const int64_t hi = max(0, min(64, kmax + 1 - k0 - static_cast<int32_t>(64 * c)));
-                        const uint64_t seen = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
-#pragma unroll
-                        for (uint32_t i = 0; i < 64; ++i)
-                            if (!(seen >> i & 1u)) x[i] = 0xff800000u;  // -infinity
-                    }
-                };
-                // a factor of zero would make masked scores NaN
-                const auto factor = [&](uint32_t g) { return fmaxf(f * sh_k[ring][g], 1e-38f); };
-                float top = -INFINITY;
+            for (int32_t j0 = 0; ok && j0 < cur.count; j0 += kRuns ? kRunTiles : cur.count) {
+                if (kRuns && j0) {                    // a run's sums to memory
+                    if (!(ok = wait_warp(full_s, done))) break;   // S of the next tile is done, so the products are
+                    tc_fence_after();
+                    const float k = row_factor(m_run, m);
 #pragma unroll 1
-                for (uint32_t c = 0; c < KT / 64; ++c) {
-                    uint32_t x[64];
-                    read(c, x);
-#pragma unroll
-                    for (uint32_t g = 0; g < 4; ++g) {
-                        const auto score = [&](uint32_t i) { return __uint_as_float(x[16 * g + i]); };
-                        const float y0 = max3(score(0), score(1), score(2)), y1 = max3(score(3), score(4), score(5));
-                        const float y2 = max3(score(6), score(7), score(8)), y3 = max3(score(9), score(10), score(11));
-                        const float y4 = max3(score(12), score(13), score(14));
-                        // scales are not negative: the largest product is the largest score
-                        top = fmaxf(top, fmaf(fmaxf(max3(y0, y1, y2), max3(y3, y4, score(15))),
-                                              factor(4 * c + g), sh_top[ring][4 * c + g]));
-                    }
-                }
-                if (__any_sync(0xffffffffu, top > m + kSlack)) {
-                    // some row's maximum grew by more than the slack
-                    const float to = fmaxf(m, top);
-                    const float a = to > m ? ex2(m - to) : 1.0f;
-                    l *= a;
-                    m = to;
-                    if (j) {   // S of this tile is done, so the products before it are
-#pragma unroll 1
-                        for (uint32_t c = 0; c < DP / 32; ++c) {
-                            uint32_t r[32];
-                            tmem_ld_32cols(lanes + Shape::kOCol + 32 * c, r);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (uint32_t i = 0; i < 32; ++i)
-                                r[i] = __float_as_uint(__uint_as_float(r[i]) * a);
-                            tmem_st_32cols(lanes + Shape::kOCol + 32 * c, r);
-                        }
-                    }
-                }
-                const float off = m == -INFINITY ? 0.0f : m - kLift;
-#pragma unroll 1
-                for (uint32_t c = 0; c < KT / 64; ++c) {
-                    uint32_t x[64], h[32], lo[kSplit ? 32 : 1];
-                    read(c, x);
-#pragma unroll
-                    for (uint32_t g = 0; g < 4; ++g) {
-                        const float fg = factor(4 * c + g), b = sh_lv[ring][4 * c + g] - off;
-                        float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i) {
-                            const float u = ex2(fmaf(__uint_as_float(x[16 * g + 2 * i]), fg, b));
-                            const float v = ex2(fmaf(__uint_as_float(x[16 * g + 2 * i + 1]), fg, b));
-                            s0 += u;
-                            s1 += v;
-                            h[8 * g + i] = pack_half2(u, v);
-                            if constexpr (kSplit) {
-                                const float2 y = unpack_half2(h[8 * g + i]);
-                                lo[8 * g + i] = pack_half2(u - y.x, v - y.y);
-                            }
-                        }
-                        l = fmaf(s0 + s1, sh_iv[ring][4 * c + g], l);
-                    }
-                    const uint32_t zero4 = zeros >> (4 * c) & 15u;
-                    if (zero4) {   // pages of zeros count in the sum alone
+                    for (uint32_t c = 0; c < DP / 32; ++c) {
+                        uint32_t v[32];
+                        float had[32];
+                        if (j0 > kRunTiles) read_sums(c, had);
+                        tmem_ld_32cols(lanes + Shape::kOCol + 32 * c, v);
+                        tmem_wait_ld();
 #pragma unroll
                         for (uint32_t i = 0; i < 32; ++i)
-                            if (zero4 >> (i / 8) & 1u) {
-                                h[i] = 0;
-                                if constexpr (kSplit) lo[i] = 0;
-                            }
+                            run_sums[(32 * c + i) * kRows] =
+                                j0 > kRunTiles ? fmaf(had[i], k, __uint_as_float(v[i])) : __uint_as_float(v[i]);
                     }
-                    tmem_st_32cols(lanes + Shape::kPCol + 32 * c, h);
-                    if constexpr (kSplit) tmem_st_32cols(lanes + Shape::kPCol + 32, lo);
+                    m_run = m;
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                arrive_warp(full_p);
+                const int32_t j1 = kRuns ? min(cur.count, j0 + kRunTiles) : cur.count;
+                for (int32_t j = j0; j < j1; ++j, ++tile_no, ++done) {
+                    const int32_t k0 = (cur.tile + j) * static_cast<int32_t>(KT);
+                    const uint32_t ring = tile_no % kScaleRing;
+                    const bool edge = k0 + static_cast<int32_t>(KT) - 1 > kmax_first || k0 < kmin_last;
+                    if (!(ok = wait_warp(&bar_sc[ring], tile_no / kScaleRing) && wait_warp(full_s, done))) break;
+                    tc_fence_after();
+                    const uint32_t zeros = sh_zeros[ring];
+                    // Loops over 64 keys are not unrolled: the code of all roles has to stay in the
+                    // instruction caches (unrolled, a fifth of the stalls were for instructions).
+                    const auto read = [&](uint32_t c, uint32_t (&x)[64]) {
+                        tmem_ld_32cols(lanes + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(x));
+                        tmem_ld_32cols(lanes + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+                        tmem_wait_ld();
+                        if (edge) {   // bits of the keys that the row sees
+                            const int64_t lo = max(0, min(64, kmin - k0 - static_cast<int32_t>(64 * c)));
+                            const int64_t hi = max(0, min(64, kmax + 1 - k0 - static_cast<int32_t>(64 * c)));
+                            const uint64_t seen = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
+#pragma unroll
+                            for (uint32_t i = 0; i < 64; ++i)
+                                if (!(seen >> i & 1u)) x[i] = 0xff800000u;  // -infinity
+                        }
+                    };
+                    // a factor of zero would make masked scores NaN
+                    const auto factor = [&](uint32_t g) { return fmaxf(f * sh_k[ring][g], 1e-38f); };
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (uint32_t c = 0; c < KT / 64; ++c) {
+                        uint32_t x[64];
+                        read(c, x);
+#pragma unroll
+                        for (uint32_t g = 0; g < 4; ++g) {
+                            const auto score = [&](uint32_t i) { return __uint_as_float(x[16 * g + i]); };
+                            const float y0 = max3(score(0), score(1), score(2)), y1 = max3(score(3), score(4), score(5));
+                            const float y2 = max3(score(6), score(7), score(8)), y3 = max3(score(9), score(10), score(11));
+                            const float y4 = max3(score(12), score(13), score(14));
+                            // scales are not negative: the largest product is the largest score
+                            top = fmaxf(top, fmaf(fmaxf(max3(y0, y1, y2), max3(y3, y4, score(15))),
+                                                  factor(4 * c + g), sh_top[ring][4 * c + g]));
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                        // some row's maximum grew by more than the slack
+                        const float to = fmaxf(m, top);
+                        const float a = to > m ? ex2(m - to) : 1.0f;
+                        l *= a;
+                        m = to;
+                        if (j != j0) {   // S of this tile is done, so the products before it are
+#pragma unroll 1
+                            for (uint32_t c = 0; c < DP / 32; ++c) {
+                                uint32_t r[32];
+                                tmem_ld_32cols(lanes + Shape::kOCol + 32 * c, r);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (uint32_t i = 0; i < 32; ++i)
+                                    r[i] = __float_as_uint(__uint_as_float(r[i]) * a);
+                                tmem_st_32cols(lanes + Shape::kOCol + 32 * c, r);
+                            }
+                        }
+                    }
+                    const float off = m == -INFINITY ? 0.0f : m - kLift;
+#pragma unroll 1
+                    for (uint32_t c = 0; c < KT / 64; ++c) {
+                        uint32_t x[64], h[32], lo[kSplit ? 32 : 1];
+                        read(c, x);
+#pragma unroll
+                        for (uint32_t g = 0; g < 4; ++g) {
+                            const float fg = factor(4 * c + g), b = sh_lv[ring][4 * c + g] - off;
+                            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i) {
+                                const float u = ex2(fmaf(__uint_as_float(x[16 * g + 2 * i]), fg, b));
+                                const float v = ex2(fmaf(__uint_as_float(x[16 * g + 2 * i + 1]), fg, b));
+                                s0 += u;
+                                s1 += v;
+                                h[8 * g + i] = pack_half2(u, v);
+                                if constexpr (kSplit) {
+                                    const float2 y = unpack_half2(h[8 * g + i]);
+                                    lo[8 * g + i] = pack_half2(u - y.x, v - y.y);
+                                }
+                            }
+                            l = fmaf(s0 + s1, sh_iv[ring][4 * c + g], l);
+                        }
+                        const uint32_t zero4 = zeros >> (4 * c) & 15u;
+                        if (zero4) {   // pages of zeros count in the sum alone
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; ++i)
+                                if (zero4 >> (i / 8) & 1u) {
+                                    h[i] = 0;
+                                    if constexpr (kSplit) lo[i] = 0;
+                                }
+                        }
+                        tmem_st_32cols(lanes + Shape::kPCol + 32 * c, h);
+                        if constexpr (kSplit) tmem_st_32cols(lanes + Shape::kPCol + 32, lo);
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    arrive_warp(full_p);
+                }
             }
             if (!ok) break;
         }
@@ -750,7 +791,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     if (j >= 0) {
                         if (!(ok = wait_warp(&bar_p[half], done[half]++))) break;
                         tc_fence_after();
-                        values(half, st, j != 0);
+                        values(half, st, kRuns ? j % kRunTiles != 0 : j != 0);
                     } else if (!(ok = wait_warp(&bar_q[half], seg[half]++))) {
                         break;
                     }
@@ -910,7 +951,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const AttnParam
             const float2 ml = p.ws_ml[at];
             const float4 v = reinterpret_cast<const float4 *>(p.ws_o)[at * (DP / 4) + d4];
             const float to = fmaxf(mm, ml.x);
-            const float f = mm == -INFINITY ? 1.0f : ex2(mm - to), g = ml.x == -INFINITY ? 1.0f : ex2(ml.x - to);
+            const float f = row_factor(mm, to), g = row_factor(ml.x, to);
             mm = to;
             ll = ll * f + ml.y * g;
             o.x = o.x * f + v.x * g;
@@ -929,7 +970,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const AttnParam
     }
 }
 
-template <RowType T, uint32_t DP>
+template <RowType T, uint32_t DP, bool kRuns>
 cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     using Shape = ManyShape<T, DP>;
     const uint32_t elem = T == RowType::kF32 ? 4 : 2;
@@ -953,7 +994,7 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     int device = 0;
     VNPU_LAUNCH(cudaGetDevice(&device));
     if (ready_device != device) {
-        VNPU_LAUNCH(cudaFuncSetAttribute(paged_prefill_kernel<T, DP>,
+        VNPU_LAUNCH(cudaFuncSetAttribute(paged_prefill_kernel<T, DP, kRuns>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem));
         ready_device = device;
     }
@@ -965,10 +1006,11 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     const size_t meta_bytes = pad(2ull * grid * sizeof(uint4));
     const size_t block_bytes = pad(blocks * sizeof(RowBlock)), before_bytes = pad(blocks * sizeof(uint32_t));
     const size_t seqs_bytes = pad(blocks * sizeof(PagedSeq));
+    const size_t run_bytes = kRuns ? pad(1ull * grid * kRows * DP * sizeof(float)) : 0;
     const size_t seq_bytes = pad((a.batch.batch + 1ull) * sizeof(uint32_t));
     char *ws = nullptr;
     VNPU_LAUNCH(cudaMallocAsync(reinterpret_cast<void **>(&ws),
-                                o_bytes + ml_bytes + meta_bytes + block_bytes + seqs_bytes + before_bytes + seq_bytes +
+                                o_bytes + ml_bytes + meta_bytes + block_bytes + seqs_bytes + before_bytes + seq_bytes + run_bytes +
                                     256,
                                 ctx.stream));
     char *at = ws;
@@ -980,6 +1022,7 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     p.ws_o = reinterpret_cast<float *>(carve(o_bytes));
     p.ws_ml = reinterpret_cast<float2 *>(carve(ml_bytes));
     p.ws_meta = reinterpret_cast<uint4 *>(carve(meta_bytes));
+    p.ws_run = reinterpret_cast<float *>(carve(run_bytes));
     Plan plan;
     plan.capacity = static_cast<uint32_t>(blocks);   // below 2^23 + 2^24
     plan.blocks = reinterpret_cast<RowBlock *>(carve(block_bytes));
@@ -990,17 +1033,26 @@ cudaError_t launch_many(const LaunchCtx &ctx, const PagedAttention &a) {
     if (ctx.launch_counter) *ctx.launch_counter += 3;
     cudaError_t e = launch_pdl(ctx.stream, &paged_plan_kernel<Shape::KT>, dim3(1), dim3(kPlanThreads), 0, p, plan);
     if (e == cudaSuccess)
-        e = launch_pdl(ctx.stream, &paged_prefill_kernel<T, DP>, dim3(grid), dim3(kManyThreads), Shape::kSmem, p, plan);
+        e = launch_pdl(ctx.stream, &paged_prefill_kernel<T, DP, kRuns>, dim3(grid), dim3(kManyThreads), Shape::kSmem, p,
+                       plan);
     if (e == cudaSuccess)
         e = launch_pdl(ctx.stream, &paged_prefill_join_kernel<T, DP>, dim3(grid, kRows * DP / 4 / 256), dim3(256), 0, p);
     const cudaError_t f = cudaFreeAsync(ws, ctx.stream);
     return e == cudaSuccess ? f : e;
 }
 
+template <RowType T, uint32_t DP>
+cudaError_t many_by_reach(const LaunchCtx &ctx, const PagedAttention &a) {
+    if constexpr (ManyShape<T, DP>::kSplit) {
+        const uint64_t reach = static_cast<uint64_t>(a.batch.table_stride) << a.cache.page_shift;
+        if (reach > static_cast<uint64_t>(kRunTiles) * ManyShape<T, DP>::KT) return launch_many<T, DP, true>(ctx, a);
+    }
+    return launch_many<T, DP, false>(ctx, a);
+}
 template <RowType T>
 cudaError_t many_by_dim(const LaunchCtx &ctx, const PagedAttention &a) {
-    if (a.cache.head_dim <= 64) return launch_many<T, 64>(ctx, a);
-    return launch_many<T, 128>(ctx, a);
+    if (a.cache.head_dim <= 64) return many_by_reach<T, 64>(ctx, a);
+    return many_by_reach<T, 128>(ctx, a);
 }
 
 }  // namespace

@@ -9,7 +9,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_gpu_paged import HALF_ULP, Setup, attention64, rows, torch  # noqa: F401
+import vnpu
+from test_gpu_paged import HALF_ULP, Setup, attention64, dt, rows, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +45,49 @@ def test_zero_pages_beside_small_values(gpu, torch, dtype, small, spans, zeros):
     tol = tol + np.abs(want) * HALF_ULP[dtype] + least
     off = np.abs(o.double().cpu().numpy() - want)
     assert (off <= tol).all(), (off / tol).max()
+
+
+# ------------------------------------------------------------------------------------------------
+# Long runs of keys
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("length", [1024, 8192, 32768, 131072])
+@pytest.mark.parametrize("rows_of", ["few", "many"])
+def test_error_does_not_grow_with_the_keys(gpu, torch, dtype, length, rows_of):
+    """Every CTA walks all keys of its rows (as many row tiles as CTAs, one shared prefix): the
+    error against the output's own size, which falls with the keys, stays what it is at 1024.
+
+    An output is a weighted mean of values of either sign; errors of the weights (2^-20 (1 + size),
+    each its own) come out as that part of the output's rms, 16-bit weights as 2^-11 / sqrt(12) of
+    it, and the output's rounding as at most its half unit in the last place.  What is common to all
+    weights (a sum that is not rounded to nearest) is a part of the output itself: 2^-19."""
+    hk, d, ps = 4, 128, 64
+    g, batch, n = (1, 112, 1) if rows_of == "few" else (4, 37, 64)      # x 4 heads: 448 and 148 row tiles
+    hq, pages = g * hk, length // ps
+    gen = torch.Generator(device="cuda").manual_seed(length)
+    k, v = (torch.randint(-127, 128, (pages, hk, ps, d), generator=gen, device="cuda", dtype=torch.int8)
+            for _ in range(2))
+    ks, vs = (torch.rand((pages, hk), generator=gen, device="cuda") * 0.01 + 0.01 for _ in range(2))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(batch, 1)
+    cu = torch.arange(0, (batch + 1) * n, n, dtype=torch.int32, device="cuda")
+    lens = torch.full((batch,), length, dtype=torch.int32, device="cuda")
+    q = torch.randn((batch * n, hq, d), generator=gen, device="cuda").to(dt(torch, dtype))
+    o = torch.empty_like(q)
+    torch.cuda.synchronize()
+    gpu.paged_attention(vnpu.paged_cache(k, v, ks, vs), vnpu.paged_batch(table, cu, lens, batch * n, n), q, o,
+                        causal=False)
+    sample = torch.arange(0, batch * n, 37 if rows_of == "many" else 1, device="cuda")[:112]
+    error = square = size = 0.0
+    for h in range(hq):
+        kk = (k[:, h // g].double() * ks[:, h // g, None, None].double()).reshape(length, d)
+        vv = (v[:, h // g].double() * vs[:, h // g, None, None].double()).reshape(length, d)
+        x = q[sample, h].double()
+        w = torch.softmax((x @ kk.T) / d ** 0.5, -1)
+        want = w @ vv
+        size = max(size, float((x.abs() @ kk.abs().T).max()) / d ** 0.5)
+        error += float((o[sample, h].double() - want).square().sum())
+        square += float(want.square().sum())
+    tol = 2.0 ** -20 * (1 + size) + 2.0 ** -19
+    if dtype == "f16":
+        tol += 2.0 ** -11 / 12 ** 0.5 + HALF_ULP[dtype]
+    assert error ** 0.5 <= tol * square ** 0.5, (error / square) ** 0.5 / tol
