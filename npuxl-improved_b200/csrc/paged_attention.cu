@@ -319,9 +319,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
     uint32_t bq[NT][NG][4][2];             // query fragments
     uint32_t bl[kSplit ? NT : 1][NG][4][2];  // f32: their low halves
     float acc[NT][NJ][4];
-    // of rows 8 t + 2 kq and + 1: running maximum, sum, score factor, and what the scores have too
-    // much (codes_to_half4_biased)
-    float m[NT][2], l[NT][2], qf[NT][2], q_bias[NT][2];
+    float m[NT][2], l[NT][2], qf[NT][2];   // of rows 8 t + 2 kq and + 1: running maximum, sum, score factor
     int32_t kmin[NT][2], kmax[NT][2], kmin_last = 0, kmax_first = 0, kmin_first = 0, kmax_last = 0;
     int32_t first_tile = 0;
     // The queries of the next row tile, read while the one before is written.
@@ -371,7 +369,6 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
             most = quad_max(most);
             const int ex = row_exponent(most);
             const float up = pow2(ex);
-            float total = 0.0f;
 #pragma unroll
             for (uint32_t g = 0; g < NG; ++g)
 #pragma unroll
@@ -380,17 +377,15 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
                     for (uint32_t k = 0; k < 2; ++k) {
                         const float x0 = v[g][4 * s + 2 * k] * up, x1 = v[g][4 * s + 2 * k + 1] * up;
                         bq[t][g][s][k] = pack_half2(x0, x1);
-                        const float2 y = unpack_half2(bq[t][g][s][k]);
-                        if constexpr (kSplit) bl[t][g][s][k] = pack_half2(x0 - y.x, x1 - y.y);
-                        else total += y.x + y.y;
+                        if constexpr (kSplit) {
+                            const float2 y = unpack_half2(bq[t][g][s][k]);
+                            bl[t][g][s][k] = pack_half2(x0 - y.x, x1 - y.y);
+                        }
                     }
-            total += __shfl_xor_sync(0xffffffffu, total, 1);
-            total += __shfl_xor_sync(0xffffffffu, total, 2);
             const float factor = p.scale_log2 * pow2(-ex);
 #pragma unroll
             for (uint32_t e = 0; e < 2; ++e) {
                 qf[t][e] = __shfl_sync(0xffffffffu, factor, 8 * kq + 4 * e);
-                q_bias[t][e] = kCodeBias * __shfl_sync(0xffffffffu, total, 8 * kq + 4 * e);
                 row_limits(p, cur.s, cur.rt * MR + 8 * t + 2 * kq + e, kmin[t][e], kmax[t][e]);
                 m[t][e] = -INFINITY;
                 l[t][e] = 0.0f;
@@ -429,13 +424,8 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i) {
                     uint32_t a0, a1, a2, a3;
-                    if constexpr (kSplit) {
-                        codes_to_half4(word(2 * i, e), a0, a2);
-                        codes_to_half4(word(2 * i + 1, e), a1, a3);
-                    } else {
-                        codes_to_half4_biased(word(2 * i, e), a0, a2);
-                        codes_to_half4_biased(word(2 * i + 1, e), a1, a3);
-                    }
+                    codes_to_half4(word(2 * i, e), a0, a2);
+                    codes_to_half4(word(2 * i + 1, e), a1, a3);
 #pragma unroll
                     for (uint32_t t = 0; t < NT; ++t) {
                         mma_f16(s[i][t], a0, a1, a2, a3, bq[t][g][e][0], bq[t][g][e][1]);
@@ -463,10 +453,9 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i) {
                     const float f = qf[t][r] * sc[i];
-                    const float b = kSplit ? lv[i] : fmaf(-q_bias[t][r], f, lv[i]);
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) {
-                        float x = fmaf(s[i][t][2 * e + r], f, b);
+                        float x = fmaf(s[i][t][2 * e + r], f, lv[i]);
                         if (edge) {
                             const int32_t key = k0 + static_cast<int32_t>(16 * i + 8 * e + n);
                             if (key > kmax[t][r] || key < kmin[t][r]) x = -INFINITY;

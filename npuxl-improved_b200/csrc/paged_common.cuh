@@ -133,16 +133,5 @@ __device__ __forceinline__ void codes_to_half4(uint32_t w, uint32_t &h01, uint32
     h23 = *reinterpret_cast<uint32_t *>(&y);
 }
 
-// The same without taking 1152 off: for products with 16-bit rows, whose sums
-// then are too large by 1152 times the row's sum, one number for all keys.  At
-// head_dim 128 that costs 5 of the f32 sum's 24 bits, which 16-bit rows do not
-// notice, and saves two of five instructions a word.
-constexpr float kCodeBias = 1152.0f;
-__device__ __forceinline__ void codes_to_half4_biased(uint32_t w, uint32_t &h01, uint32_t &h23) {
-    const uint32_t u = w ^ 0x80808080u;
-    h01 = __byte_perm(u, 0x64646464u, 0x4140);
-    h23 = __byte_perm(u, 0x64646464u, 0x4342);
-}
-
 }  // namespace
 }  // namespace vnpu_b200

@@ -91,3 +91,64 @@ def test_error_does_not_grow_with_the_keys(gpu, torch, dtype, length, rows_of):
     if dtype == "f16":
         tol += 2.0 ** -11 / 12 ** 0.5 + HALF_ULP[dtype]
     assert error ** 0.5 <= tol * square ** 0.5, (error / square) ** 0.5 / tol
+
+
+# ------------------------------------------------------------------------------------------------
+# Rows of one sign
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("spans", ["few", "many"])
+@pytest.mark.parametrize("size", [50, 1000, 16000])
+def test_scores_of_rows_of_one_sign(gpu, torch, dtype, spans, size):
+    """Two keys with scores of thousands, a few units apart, values +1 and -1: the output is
+    tanh((s0 - s1) / 2), which shows the scores' errors.  All query elements are positive.
+
+    Each score may be off by 2^-21 of its size (16-bit queries are exact), the output by half their
+    difference's error; weights of 16-bit rows by 2^-11, f32 queries have 22 bits: another 2^-22."""
+    d, ps, n = 128, 16, 600
+    rng = np.random.default_rng(size)
+    s = Setup(torch, [(1, 2)] * n if spans == "few" else [(200, 200)] * 3, 1, d, ps)
+    if spans == "few":
+        q = rng.uniform(0.5, 1.5, (n, d))
+        k0 = rng.integers(-127, 128, (n, d))
+        k1 = k0.copy()
+        for _ in range(6):             # moves of one code from one place to another: sums stay alike
+            i, j = rng.integers(0, d, (2, n))
+            r = np.arange(n)
+            step = np.minimum(rng.integers(1, 40, n), np.minimum(127 - k1[r, i], 127 + k1[r, j]))
+            k1[r, i] += step
+            k1[r, j] -= step
+        s.k[s.table[:, 0], 0, 0], s.k[s.table[:, 0], 0, 1] = k0, k1
+        s.v[s.table[:, 0], 0, 0], s.v[s.table[:, 0], 0, 1] = 127, -127
+    else:
+        # keys in pairs within a page, only the first two of each sequence are near the top
+        q = rng.uniform(0.5, 1.5, (600, d))
+        for b in range(3):
+            for page in s.table[b, :13]:
+                s.k[page] = -127
+                s.v[page] = 127
+            page = s.table[b, 0]
+            k0 = rng.integers(-60, 128, d)
+            k1 = k0.copy()
+            for _ in range(6):
+                i, j = rng.integers(0, d, 2)
+                step = min(int(rng.integers(1, 40)), 127 - k1[i], 127 + k1[j])
+                k1[i] += step
+                k1[j] -= step
+            s.k[page, 0, 0], s.k[page, 0, 1] = k0, k1
+            s.v[page, 0, 0], s.v[page, 0, 1] = 127, -127
+    s.ks[:], s.vs[:] = 1 / 64, 1 / 127
+    for x, y in ((s.dk, s.k), (s.dv, s.v), (s.dks, s.ks), (s.dvs, s.vs)):
+        x.copy_(torch.from_numpy(y))
+    q = torch.from_numpy(q.astype(np.float32)).to(dt(torch, dtype)).cuda()
+    scale = size / (d * 1.0)                               # |q| is 1 and |k| 1 on the average
+    scale = float(np.float32(scale))
+    o = torch.empty((s.tokens, 1, d), dtype=q.dtype, device="cuda")
+    torch.cuda.synchronize()
+    gpu.paged_attention(s.cache, s.batch, q.view(-1, 1, d), o, causal=False, scale=scale)
+    want, sizes, _ = attention64(s, q.double().cpu().numpy(), 1, False, 0, scale)
+    assert (np.abs(want) < 0.9).mean() > (0.02 if size > 1000 else 0.1)     # rows that show something
+    tol = sizes * 2.0 ** -21 * (1.5 if dtype == "f32" else 1) + 2.0 ** -20
+    tol = tol + (0 if dtype == "f32" else 2.0 ** -11) + np.abs(want) * HALF_ULP[dtype]
+    off = np.abs(o.double().cpu().numpy() - want)
+    assert (off <= tol).all(), ((off / tol).max(), (off > tol).sum())
