@@ -119,24 +119,33 @@ inline uint64_t segment_items(const PagedCache &c, const PagedBatch &b) {
     return b.max_tokens == 1 ? b.batch : (static_cast<uint64_t>(b.tokens) >> c.page_shift) + 2ull * b.batch;
 }
 
-// `pos` times t 2^-64 turns in half turns, in [-1, 1).  The product is taken
-// modulo one turn (the 64-bit wrap) and rounded to 32 bits: off by 2^-24 of the
-// angle at every position, where a 32-bit position * frequency is off by 2^-24
-// of the whole angle, 1e-2 at position 1e5.
-__device__ __forceinline__ float half_turns(int32_t pos, uint64_t t) {
+// `pos` times t 2^-64 turns, in 2^-32 turns.  The product is taken modulo one
+// turn (the 64-bit wrap): off by 2^-32 of a turn at every position, where a
+// 32-bit position * frequency is off by 2^-24 of the whole angle, 1e-2 at
+// position 1e5.
+__device__ __forceinline__ uint32_t turn_fraction(int32_t pos, uint64_t t) {
     const uint32_t p = static_cast<uint32_t>(pos);
-    const uint32_t top = p * static_cast<uint32_t>(t >> 32) + __umulhi(p, static_cast<uint32_t>(t));
-    return static_cast<float>(static_cast<int32_t>(top)) * 0x1p-31f;
+    return p * static_cast<uint32_t>(t >> 32) + __umulhi(p, static_cast<uint32_t>(t));
 }
-// Queries' angles, shared by their heads: sine and cosine to the last places.
+// Queries' angles, shared by their heads: the library's sine and cosine.
 __device__ __forceinline__ void turn_sincos(int32_t pos, uint64_t t, float *sn, float *cs) {
-    sincospif(half_turns(pos, t), sn, cs);
+    sincospif(static_cast<float>(static_cast<int32_t>(turn_fraction(pos, t))) * 0x1p-31f, sn, cs);
 }
-// Keys' angles, one for each pair and head: the fast sine and cosine, 2^-21 off
-// at most in (-pi, pi], a ten-thousandth of a code (16 prompts, 6300 tokens of
-// 32/8 heads of 128: 80.5 us with the exact ones, 50.5 with these).
-__device__ __forceinline__ void turn_sincos_fast(int32_t pos, uint64_t t, float *sn, float *cs) {
-    __sincosf(half_turns(pos, t) * 3.14159265358979f, sn, cs);
+// Keys' angles, one for each pair and head: the nearest quarter turn is taken off
+// in whole numbers, what is left is x in [-pi/4, pi/4], off by 2^-24 of itself,
+// and the Taylor series of sine and cosine to x^9 and x^10 are within 2e-9 there.
+// Sine and cosine are off by 2^-23.3 at most.  (The library's sincospif for each pair
+// and head cost 60 % more time; its fast sine and cosine, 2^-21 off, flipped codes and
+// took 58.0 us where these take 60.5: 16 prompts, 8600 tokens of 32/8 heads of 128.)
+__device__ __forceinline__ void turn_sincos_series(int32_t pos, uint64_t t, float *sn, float *cs) {
+    const uint32_t turn = turn_fraction(pos, t), quarter = (turn + (1u << 29)) >> 30;
+    const float x = static_cast<float>(static_cast<int32_t>(turn - (quarter << 30))) * 1.46291807926715968e-9f;  // 2 pi / 2^32
+    const float y = x * x;
+    const float s = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), x);
+    const float c = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const float u = quarter & 1u ? c : s, v = quarter & 1u ? s : c;
+    *sn = __uint_as_float(__float_as_uint(u) ^ (quarter & 2u) << 30);
+    *cs = __uint_as_float(__float_as_uint(v) ^ ((quarter + 1u) & 2u) << 30);
 }
 
 // A head's 16 elements of unit u as two groups of 8 and their pairs' first
@@ -350,7 +359,7 @@ __global__ void __launch_bounds__(NT, kWarp ? 6 : U == 2 ? 3 : 2) paged_append_k
         const Unit x = unit_of(at.u, rot, interleaved);
         if (x.pair >= 0)
             rotate_unit(a, b, interleaved, [&](int e, float *sn, float *cs) {
-                turn_sincos_fast(g.pos0 + static_cast<int32_t>(at.r), sh_rate[pad8(x.pair) + e], sn, cs);
+                turn_sincos_series(g.pos0 + static_cast<int32_t>(at.r), sh_rate[pad8(x.pair) + e], sn, cs);
             });
     };
     float most = 0.0f;

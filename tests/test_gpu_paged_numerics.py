@@ -152,3 +152,33 @@ def test_scores_of_rows_of_one_sign(gpu, torch, dtype, spans, size):
     tol = tol + (0 if dtype == "f32" else 2.0 ** -11) + np.abs(want) * HALF_ULP[dtype]
     off = np.abs(o.double().cpu().numpy() - want)
     assert (off <= tol).all(), ((off / tol).max(), (off > tol).sum())
+
+
+# ------------------------------------------------------------------------------------------------
+# Append: angles and codes
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("single", [True, False], ids=["single", "runs"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_angles_of_keys(gpu, torch, single, interleaved):
+    """One pair (1, 0) a head and page: the page's scale is the larger of |cos| and |sin| over 127,
+    in 32 bits.  The angle is off by 2^-24 of at most pi/4 off a quarter turn, sine and cosine by 2
+    units in the last place (2^-23 of values above 1/2), the scale's division by half a unit."""
+    d, ps, hk, n = 16, 16, 8, 512
+    rng = np.random.default_rng(7)
+    starts = rng.integers(0, 200_000, n) // ps * ps         # each token opens a page
+    table = np.full((n, 200_000 // ps + 1), -1, np.int32)
+    table[np.arange(n), starts // ps] = np.arange(n)
+    k = torch.zeros((n, hk, d), device="cuda")
+    for h in range(hk):
+        k[:, h, 2 * h if interleaved else h] = 1.0
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()  # noqa: E731
+    codes = [torch.zeros((n, hk, ps, d), dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros((n, hk), device="cuda") for _ in range(2)]
+    cache = vnpu.paged_cache(*codes, *scales)
+    batch = vnpu.paged_batch(dev(table), dev(np.arange(n + 1)), dev(starts + 1), n, 1 if single else 2)
+    torch.cuda.synchronize()
+    gpu.paged_kv_append(cache, batch, None, k.flatten(1), k.flatten(1), None, interleaved=interleaved)
+    angle = starts[:, None] * 10000.0 ** (-2.0 * np.arange(hk) / d)
+    want = np.maximum(np.abs(np.cos(angle)), np.abs(np.sin(angle))) / 127
+    off = np.abs(scales[0].double().cpu().numpy() / want - 1)
+    assert off.max() <= np.pi / 4 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -24 + 1e-10, off.max()
