@@ -194,34 +194,66 @@ __device__ __forceinline__ void rotate_unit(float (&a)[8], float (&b)[8], bool i
     }
 }
 
-// Code of x: nearest, ties to even; NaN 0 (the conversion's own), infinities
-// the largest code.
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-    const int q = __float2int_rn(__fmul_rn(x, inv));
-    return static_cast<uint32_t>(max(-127, min(127, q))) & 0xffu;
+// What codes are made with: 1 / scale, the scale, and half of it (infinite for a
+// page of zeros).
+struct Rounding {
+    float inv, scale, half;
+};
+// x * inv + 1.5 * 2^23: the nearest whole number (ties to even) of the product in
+// the low bits, two's complement.  *rest: what x has more than that many scales,
+// exactly.
+__device__ __forceinline__ uint32_t rounded(float x, const Rounding &by, float *rest) {
+    const float z = __fmaf_rn(x, by.inv, 12582912.0f);
+    *rest = __fmaf_rn(12582912.0f - z, by.scale, x);
+    return __float_as_uint(z);
 }
-// Codes of 4 finite values: adding 1.5 * 2^23 leaves the nearest whole number
-// (ties to even) in the low bits, two's complement, in one instruction a value.
-__device__ __forceinline__ uint32_t codes4_finite(const float *v, float inv) {
-    uint32_t q[4];
+// The product can miss the quotient's nearest number where that is close to a
+// tie: the rest then passes half a scale, or is half of it on an odd number.
+__device__ __forceinline__ uint32_t set_right(uint32_t z, float rest, const Rounding &by) {
+    return __float_as_uint(fabsf(rest)) + (z & 1u) > __float_as_uint(by.half) ? z + (rest > 0.0f ? 1u : ~0u) : z;
+}
+// Codes of 8 values: x / scale to nearest, ties to even.
+__device__ __forceinline__ uint2 codes8_finite(const float (&v)[8], const Rounding &by) {
+    uint32_t q[8];
+    float rest[8], most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fmaf_rn(v[i], inv, 12582912.0f));
-    return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    for (int i = 0; i < 8; ++i) {
+        q[i] = rounded(v[i], by, &rest[i]);
+        most = fmaxf(most, fabsf(rest[i]));
+    }
+    if (most >= by.half) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = set_right(q[i], rest[i], by);
+    }
+    const auto pack = [&](int i) {
+        return __byte_perm(__byte_perm(q[i], q[i + 1], 0x0040), __byte_perm(q[i + 2], q[i + 3], 0x0040), 0x5410);
+    };
+    return make_uint2(pack(0), pack(4));
+}
+// The same with NaN 0 and infinities the largest code.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], const Rounding &by) {
+    uint2 r = make_uint2(0, 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float rest;
+        uint32_t q = set_right(rounded(v[i], by, &rest), rest, by);
+        if (!(fabsf(v[i]) <= 3.402823466e38f)) q = v[i] > 0.0f ? 127u : v[i] < 0.0f ? 129u : 0u;
+        (i < 4 ? r.x : r.y) |= (q & 0xffu) << (8 * (i & 3));
+    }
+    return r;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where either is
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-__device__ __forceinline__ uint32_t codes4(const float *v, float inv) {
-    return code_of(v[0], inv) | (code_of(v[1], inv) << 8) | (code_of(v[2], inv) << 16) |
-           (code_of(v[3], inv) << 24);
-}
+// Older codes on a larger scale, whose part `ratio` theirs is.
 __device__ __forceinline__ uint32_t rescaled4(uint32_t w, float ratio) {
     uint32_t r = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        r |= code_of(static_cast<float>(static_cast<int8_t>(w >> (8 * i))), ratio) << (8 * i);
+        r |= (static_cast<uint32_t>(__float2int_rn(static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * ratio)) & 0xffu)
+             << (8 * i);
     return r;
 }
 
@@ -424,20 +456,15 @@ __global__ void __launch_bounds__(NT, kWarp ? 6 : U == 2 ? 3 : 2) paged_append_k
     }
 
     // A scale below the smallest normal number has no finite reciprocal: such a page is zero.
-    const float fresh = __fdiv_rn(__uint_as_float(bits), 127.0f);
-    const float now = fmaxf(held, fresh < 1.17549435e-38f ? 0.0f : fresh);
-    const float inv = now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f;
+    const float larger = fmaxf(held, __fdiv_rn(__uint_as_float(bits), 127.0f));
+    const float now = larger < 1.17549435e-38f ? 0.0f : larger;
+    const Rounding by = {now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f, now, now > 0.0f ? 0.5f * now : INFINITY};
     if (lane == 0) *scale = now;
     const auto put = [&](const Place &k, const float (&a)[8], const float (&b)[8]) {
         const Unit x = unit_of(k.u, rot, interleaved);
         int8_t *row = page + static_cast<uint32_t>(g.slot0 + k.r) * D;
-        if (finite) {
-            *reinterpret_cast<uint2 *>(row + x.o0) = make_uint2(codes4_finite(a, inv), codes4_finite(a + 4, inv));
-            *reinterpret_cast<uint2 *>(row + x.o1) = make_uint2(codes4_finite(b, inv), codes4_finite(b + 4, inv));
-        } else {
-            *reinterpret_cast<uint2 *>(row + x.o0) = make_uint2(codes4(a, inv), codes4(a + 4, inv));
-            *reinterpret_cast<uint2 *>(row + x.o1) = make_uint2(codes4(b, inv), codes4(b + 4, inv));
-        }
+        *reinterpret_cast<uint2 *>(row + x.o0) = finite ? codes8_finite(a, by) : codes8(a, by);
+        *reinterpret_cast<uint2 *>(row + x.o1) = finite ? codes8_finite(b, by) : codes8(b, by);
     };
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)

@@ -182,3 +182,36 @@ def test_angles_of_keys(gpu, torch, single, interleaved):
     want = np.maximum(np.abs(np.cos(angle)), np.abs(np.sin(angle))) / 127
     off = np.abs(scales[0].double().cpu().numpy() / want - 1)
     assert off.max() <= np.pi / 4 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -24 + 1e-10, off.max()
+
+
+@pytest.mark.parametrize("single", [True, False], ids=["single", "runs"])
+def test_codes_are_to_nearest(gpu, torch, single):
+    """A code is x / scale to nearest: off by half a code and the 32-bit quotient's rounding, 2^-24
+    of at most 127.  Whole and half multiples of a scale that is no power of two go to even."""
+    d, ps, hk = 256, 16, 4
+    n = 1024
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((n, hk, d)).astype(np.float32)
+    x[:16, 0] = rng.integers(-254, 255, (16, d)) * np.float32(1.5)     # scale 3, halves of it
+    x[:16, 0, 0] = 381.0
+    spans = [(1, 1)] * n if single else [(n, n)]
+    s = Setup(torch, spans, hk, d, ps)
+    if single:
+        x[::7, 0] = rng.integers(-254, 255, x[::7, 0].shape) * np.float32(1.5)
+        x[::7, 0, 0] = 381.0
+    dx = torch.from_numpy(x).cuda()
+    torch.cuda.synchronize()
+    gpu.paged_kv_append(s.cache, s.batch, None, dx.flatten(1), dx.flatten(1), None, rope=False)
+    for codes, scale in ((s.dk, s.dks), (s.dv, s.dvs)):
+        codes, scale = codes.cpu().numpy().astype(np.float64), scale.cpu().numpy().astype(np.float64)
+        if single:
+            got, per = codes[s.table[:, 0], :, 0], scale[s.table[:, 0]]
+        else:
+            pages = s.table[0, :n // ps]
+            got = codes[pages].transpose(0, 2, 1, 3).reshape(n, hk, d)
+            per = np.repeat(scale[pages], ps, 0)
+        y = x / per[:, :, None]
+        off = np.abs(got - y)
+        assert off.max() <= 0.5 + 127 * 2.0 ** -24, off.max() - 0.5
+        halves = np.abs(y - np.trunc(y)) == 0.5
+        assert halves.sum() > 100 and np.array_equal(got[halves], np.rint(y[halves]))
