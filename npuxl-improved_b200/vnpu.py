@@ -377,6 +377,9 @@ def paged_batch(block_table, cu_tokens, seq_lens, tokens: int, max_tokens: int =
         raise ValueError(f"block_table: rows of its own for each sequence, got strides "
                          f"{tuple(block_table.stride())}")
     stride = block_table.stride(0) if n > 1 else block_table.shape[1]
+    room = block_table.untyped_storage().nbytes() // 4 - block_table.storage_offset()
+    if n * stride > room:       # a command may read (from the host: copies) a whole stride of the last row
+        raise ValueError(f"block_table: {n} rows of {stride} entries, got {room} entries")
     return PagedBatch(ptr(block_table), ptr(cu_tokens), ptr(seq_lens), n, stride, tokens, max_tokens)
 
 

@@ -82,3 +82,14 @@ def test_types_and_tables(cache):
         vnpu.paged_batch(table.to(torch.uint32), ints(0, 3, 4), ints(3, 1), 4)
     with pytest.raises(ValueError):
         vnpu.paged_batch(table[:1].expand(2, -1), ints(0, 3, 4), ints(3, 1), 4)
+
+
+def test_table_rows_are_whole(cache):
+    """Some columns of a wider table: its rows are read by their stride, the last one too."""
+    wide = torch.zeros((3, 8), dtype=torch.int32)
+    cu, lens = ints(0, 1, 2, 3), ints(1, 1, 1)
+    assert vnpu.paged_batch(wide[:, :5], cu, lens, 3).table_stride == 8
+    assert vnpu.paged_batch(wide[:2, 4:], cu[:3], lens[:2], 2).table_stride == 8
+    with pytest.raises(ValueError):
+        vnpu.paged_batch(wide[:, 4:], cu, lens, 3)
+    assert vnpu.paged_batch(wide[2:, 4:], cu[:2], lens[:1], 1).table_stride == 4
