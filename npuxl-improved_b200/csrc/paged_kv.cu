@@ -194,25 +194,31 @@ __device__ __forceinline__ void rotate_unit(float (&a)[8], float (&b)[8], bool i
     }
 }
 
-// What codes are made with: 1 / scale, the scale, and half of it (infinite for a
-// page of zeros).
+// What codes are made with: 1 / scale, the scale, half of it (infinite for a page
+// of zeros), and 2^-24 of it.
 struct Rounding {
-    float inv, scale, half;
+    float inv, scale, half, unit;
 };
-// x * inv + 1.5 * 2^23: the nearest whole number (ties to even) of the product in
-// the low bits, two's complement.  *rest: what x has more than that many scales,
-// exactly.
+// The code of x is the nearest whole number, ties to even, of the 32-bit quotient
+// x / scale.  That is the nearest of x * inv, in the low bits of x * inv + 1.5 *
+// 2^23, unless *rest, what x has more than that many scales, exactly, is within
+// 2^-15 scales of half a scale: the product is off by 2^-24 of at most 127 and the
+// quotient by half as much.
 __device__ __forceinline__ uint32_t rounded(float x, const Rounding &by, float *rest) {
     const float z = __fmaf_rn(x, by.inv, 12582912.0f);
     *rest = __fmaf_rn(12582912.0f - z, by.scale, x);
     return __float_as_uint(z);
 }
-// The product can miss the quotient's nearest number where that is close to a
-// tie: the rest then passes half a scale, or is half of it on an odd number.
-__device__ __forceinline__ uint32_t set_right(uint32_t z, float rest, const Rounding &by) {
-    return __float_as_uint(fabsf(rest)) + (z & 1u) > __float_as_uint(by.half) ? z + (rest > 0.0f ? 1u : ~0u) : z;
+// There the quotient is a tie where it is half a unit in the last place from one
+// at most (2^-24 of its power of two), and else on the side that the rest says.
+// Ties are common: 16-bit x are one in a thousand times.
+__device__ __forceinline__ uint32_t settled(float x, uint32_t z, float rest, const Rounding &by) {
+    const float over = fabsf(rest) - by.half;
+    const uint32_t power = max(__float_as_uint(fabsf(x * by.inv)) & 0x7f800000u, 0x3f000000u);   // of quotients from 1/2
+    const bool tie = fabsf(over) <= __uint_as_float(power) * by.unit;
+    return (tie ? (z & 1u) != 0 : over > 0.0f) ? z + (rest > 0.0f ? 1u : ~0u) : z;
 }
-// Codes of 8 values: x / scale to nearest, ties to even.
+// Codes of 8 values.
 __device__ __forceinline__ uint2 codes8_finite(const float (&v)[8], const Rounding &by) {
     uint32_t q[8];
     float rest[8], most = 0.0f;
@@ -221,9 +227,9 @@ __device__ __forceinline__ uint2 codes8_finite(const float (&v)[8], const Roundi
         q[i] = rounded(v[i], by, &rest[i]);
         most = fmaxf(most, fabsf(rest[i]));
     }
-    if (most >= by.half) {
+    if (most >= by.half * (1.0f - 0x1p-14f)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = set_right(q[i], rest[i], by);
+        for (int i = 0; i < 8; ++i) q[i] = settled(v[i], q[i], rest[i], by);
     }
     const auto pack = [&](int i) {
         return __byte_perm(__byte_perm(q[i], q[i + 1], 0x0040), __byte_perm(q[i + 2], q[i + 3], 0x0040), 0x5410);
@@ -236,7 +242,8 @@ __device__ __forceinline__ uint2 codes8(const float (&v)[8], const Rounding &by)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float rest;
-        uint32_t q = set_right(rounded(v[i], by, &rest), rest, by);
+        const uint32_t z = rounded(v[i], by, &rest);
+        uint32_t q = settled(v[i], z, rest, by);
         if (!(fabsf(v[i]) <= 3.402823466e38f)) q = v[i] > 0.0f ? 127u : v[i] < 0.0f ? 129u : 0u;
         (i < 4 ? r.x : r.y) |= (q & 0xffu) << (8 * (i & 3));
     }
@@ -458,7 +465,8 @@ __global__ void __launch_bounds__(NT, kWarp ? 6 : U == 2 ? 3 : 2) paged_append_k
     // A scale below the smallest normal number has no finite reciprocal: such a page is zero.
     const float larger = fmaxf(held, __fdiv_rn(__uint_as_float(bits), 127.0f));
     const float now = larger < 1.17549435e-38f ? 0.0f : larger;
-    const Rounding by = {now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f, now, now > 0.0f ? 0.5f * now : INFINITY};
+    const Rounding by = {now > 0.0f ? __fdiv_rn(1.0f, now) : 0.0f, now, now > 0.0f ? 0.5f * now : INFINITY,
+                         now * 0x1p-24f};
     if (lane == 0) *scale = now;
     const auto put = [&](const Place &k, const float (&a)[8], const float (&b)[8]) {
         const Unit x = unit_of(k.u, rot, interleaved);

@@ -215,3 +215,22 @@ def test_codes_are_to_nearest(gpu, torch, single):
         assert off.max() <= 0.5 + 127 * 2.0 ** -24, off.max() - 0.5
         halves = np.abs(y - np.trunc(y)) == 0.5
         assert halves.sum() > 100 and np.array_equal(got[halves], np.rint(y[halves]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_codes_of_16_bit_values(gpu, torch, dtype):
+    """16-bit values are often exactly between two codes of their largest over 127, though not of that
+    scale's 32-bit rounding: the code is the 32-bit quotient's nearest, ties to even, to the bit."""
+    d, ps, hk, n = 128, 64, 8, 1024
+    s = Setup(torch, [(n, n)], hk, d, ps)
+    x = torch.randn((n, hk * d), generator=torch.Generator().manual_seed(4)).to(
+        torch.bfloat16 if dtype == "f32" else dt(torch, dtype)).to(dt(torch, dtype)).cuda()
+    torch.cuda.synchronize()
+    gpu.paged_kv_append(s.cache, s.batch, None, x, x, None, rope=False)
+    x = x.float().cpu().numpy().reshape(n, hk, d)
+    for codes, scale in ((s.dk, s.dks), (s.dv, s.dvs)):
+        pages = s.table[0, :n // ps]
+        got = codes.cpu().numpy()[pages].transpose(0, 2, 1, 3).reshape(n, hk, d)
+        per = np.repeat(scale.cpu().numpy()[pages], ps, 0)[:, :, None]
+        assert np.array_equal(per, np.repeat(np.abs(x).reshape(-1, ps, hk, d).max((1, 3)) / np.float32(127), ps, 0)[:, :, None])
+        assert np.array_equal(got, np.rint(x / per).astype(np.int8))
