@@ -40,7 +40,8 @@ constexpr uint32_t kTile = 128;      // keys of a work unit, 32 for each warp
 constexpr uint32_t kWarpKeys = kTile / kWarps;
 // Reach of a table up to which row tiles are not split.  One token, 16 sequences of 32/8 heads of 128,
 // us without and with splitting and joining: 256 keys 9.2 and 9.6, 384 keys 11.5 and 9.9; 64 sequences
-// of 8 heads of 64: 12.4 and 13.3, 15.6 and 14.8.
+// of 8 heads of 64: 12.4 and 13.3, 15.6 and 14.8.  (The lengths are the device's: the reach is what
+// the host knows of them.)
 constexpr uint32_t kWholeKeys = 256;
 
 // As many CTAs an SM as the registers allow (the kernel is bound by the latency
@@ -809,11 +810,15 @@ cudaError_t launch_few(const LaunchCtx &ctx, const PagedAttention &a) {
 }  // namespace
 
 cudaError_t paged_attention(const LaunchCtx &ctx, const PagedAttention &a) {
-    // Rows of a key/value head in one sequence (tokens x group): up to 48 the few-row kernel's 16-row
-    // tiles read the codes again for each tile and still win.  16 sequences of 2048 keys, 8 heads of
-    // 128, bf16, in us, few against many: 32 rows 46 and 60, 48 rows 64 and 61, 64 rows 78 and 62;
-    // 64 sequences of 512 keys: 48 rows 78 and 85, 64 rows 94 and 86; f32 there: 118 and 114, 147 and 118.
-    if (1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > 48) {
+    // Rows of a key/value head in one sequence (tokens x group): the few-row kernel's 16-row tiles read
+    // and convert the codes again for each tile, the many-row kernel has a block's start and end.  In
+    // us, few and many, 16 sequences of 2048 keys, 64 of 512, 4 of 8192, 8 key/value heads:
+    //   16-bit, 64:  48 rows 49 and 51, 55 and 66, 46 and 48; 56 rows 60 and 51, 67 and 66, 58 and 48
+    //   16-bit, 128: 48 rows 65 and 61, 78 and 85, 60 and 57; 56 rows 79 and 62, 92 and 86, 76 and 57
+    //   f32, 64:     64 rows 69 and 75, 78 and 89, 66 and 71; a fifth tile is 14 more
+    //   f32, 128:    32 rows 77 and 97, 90 and 121, 73 and 88; 40 rows 107 and 98, 131 and 121, 99 and 89
+    const uint64_t few = a.type != RowType::kF32 ? 48 : a.cache.head_dim <= 64 ? 64 : 32;
+    if (1ull * a.batch.max_tokens * (a.q_heads / a.cache.heads) > few) {
         const cudaError_t e = paged_attention_many_rows(ctx, a);
         if (e != cudaErrorNotSupported) return e;
     }
