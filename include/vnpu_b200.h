@@ -407,7 +407,8 @@ typedef struct vnpu_b200_paged_kv_read_args_t {
  * O = sum_j softmax_j(scale * q.k_j) v_j (scale 0 = 1/sqrt(head_dim)).  A query
  * that attends to nothing has the output 0.  Scores, softmax sums and
  * accumulators are 32 bits wide; the softmax weights enter the value product
- * as 16-bit floats for 16-bit outputs, and as two of them (22 bits) for f32.
+ * as 16-bit floats for 16-bit outputs, and as two of them (22 bits) for f32, as
+ * f32 queries enter the scores.
  * A command that takes 2^32 steps of 256 query rows by 64 or 128 keys or more,
  * a minute's work at least, is left out and sets the stream's device error.
  * max_length, when not 0, is the longest seq_lens[b] to expect, for the

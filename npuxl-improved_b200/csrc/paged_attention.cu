@@ -25,8 +25,8 @@
 // the accumulators are rescaled a few times a row instead of at every step.
 //
 // Measured, bf16, 32/8 heads of 128: one token each for 2 sequences of 131072
-// keys 93 us (537 MB, 5.75 TB/s, 87 % of the copy bandwidth) and 7 us of
-// joining; for 64 sequences of up to 4096 keys 67 us with joining (304 MB, 4.5
+// keys 95 us (537 MB, 5.65 TB/s, 86 % of the copy bandwidth) and 6 us of
+// joining; for 64 sequences of up to 4096 keys 68 us with joining (304 MB, 4.5
 // TB/s: the starts and ends of rows beside the stream).
 #include <algorithm>
 

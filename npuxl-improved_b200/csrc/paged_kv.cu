@@ -11,8 +11,8 @@
 // search for; the numbers left over are CTAs that leave at once.
 //
 // Measured, bf16, 32/8 heads of 128 where not said: append of 6300 tokens in 16
-// prompts 45 us (142 MB, 3.2 TB/s; issue slots and latency, not memory), of 64
-// single tokens 5.2 us (three dependent loads); read-back, pass after pass, of
+// prompts 50 us (142 MB, 2.8 TB/s; issue slots and latency, not memory), of 64
+// single tokens 5.5 us (three dependent loads); read-back, pass after pass, of
 // 19 000 tokens of 8 heads of 64 in f16 11.7 us of one cache and 14.3 of three in
 // turn (58 MB, 5.0 and 4.1 TB/s), of 512 tokens of 32 heads in f32 8.4 and 9.6 us
 // (21 MB; one wave of CTAs and its latency).

@@ -25,7 +25,7 @@
 // What bounds it: at head_dim 128 a 256 x 128 tile costs 32768 exponentials at
 // 16 a clock (2048 clocks) against 2048 clocks of the tensor core, with about
 // 1400 issue slots a scheduler beside them.  Measured, bf16, 32/8 heads of 128:
-// 2048 tokens over 32768 keys 1250 us (850 TFLOP/s, 52 % of the measured product
+// 2048 tokens over 32768 keys 1257 us (847 TFLOP/s, 52 % of the measured product
 // rate); 880 us with the softmax's arithmetic left out, of which the products
 // are 463: the rest is a tile's way through the roles.
 //
