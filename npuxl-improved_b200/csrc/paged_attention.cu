@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kThreadsA, AttnShape<DP, MR>::kCtasPerSm)
             const float vs = sc[2 + i];
             on[i] = vs >= kLeastScale;         // else a page of zeros, or nothing that is seen
             lv[i] = on[i] ? __log2f(vs) : kZeroLog;
-            iv[i] = on[i] ? ex2(-lv[i]) : 1.0f;
+            iv[i] = on[i] ? reciprocal(vs) : 1.0f;   // not 2^-lv: what lv is off by then cancels in o / l
         }
         const bool edge = k0 + static_cast<int32_t>(kWarpKeys) - 1 > kmax_first || k0 < kmin_last;
         float top[NT][2];

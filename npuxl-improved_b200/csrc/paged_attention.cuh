@@ -49,6 +49,12 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 1 / x within a unit in the last place.
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // A part's factor where the maximum of all is `all`: one that saw no key holds zeros (or the NaN of its
 // query), taken as they are.
 __device__ __forceinline__ float row_factor(float m, float all) { return m == -INFINITY ? 1.0f : ex2(m - all); }

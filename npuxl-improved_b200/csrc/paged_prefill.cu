@@ -905,7 +905,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         sh_k[ring][lane] = now.ks;
                         sh_top[ring][lane] = on ? lv : kZeroLog;
                         sh_lv[ring][lane] = lv;
-                        sh_iv[ring][lane] = ex2(-lv);
+                        sh_iv[ring][lane] = on ? reciprocal(now.vs) : 1.0f;   // what lv is off by cancels in o / l
                     }
                     if (lane == 0) sh_zeros[ring] = zeros;
                     __syncwarp();

@@ -94,6 +94,37 @@ def test_error_does_not_grow_with_the_keys(gpu, torch, dtype, length, rows_of):
 
 
 # ------------------------------------------------------------------------------------------------
+# One key
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [1e-25, 1e-9, 1e-4, 1.0, 1e3, 1e20])
+@pytest.mark.parametrize("spans", [[(1, 200), (5, 70)], [(130, 300)]], ids=["few", "many"])
+def test_one_key_gives_its_value(gpu, torch, dtype, size, spans):
+    """A window of one: the output is the cached value, whatever its page's scale.  A weight is rounded
+    to 22 bits (11 for 16-bit rows), the scale's reciprocal by 2^-23, the sum, its reciprocal and the
+    output's product by 2^-24 each."""
+    if dtype == "f16" and size not in (1e-4, 1.0):
+        pytest.skip("past what f16 holds")
+    hk, d, ps = 2, 64, 16
+    s = Setup(torch, spans, hk, d, ps)
+    s.vs *= np.float32(size)
+    s.dvs.copy_(torch.from_numpy(s.vs))
+    q, _ = rows(torch, np.random.default_rng(3), s.tokens, hk * d, dtype)
+    o = torch.empty((s.tokens, hk, d), dtype=q.dtype, device="cuda")
+    torch.cuda.synchronize()
+    gpu.paged_attention(s.cache, s.batch, q.view(s.tokens, hk, d), o, window=1)
+    want = []
+    for b, (n, length) in enumerate(spans):
+        v, vs = s.seq_codes("v", b)
+        want.append((v * vs[:, :, None])[length - n:])
+    want = np.concatenate(want)
+    part = (2.0 ** -22 if dtype == "f32" else 2.0 ** -11) + 2.0 ** -23 + 4 * 2.0 ** -24
+    off = np.abs(o.double().cpu().numpy() - want)
+    tol = np.abs(want) * (part + HALF_ULP[dtype]) + (2.0 ** -25 if dtype == "f16" else 0)
+    assert (off <= tol).all(), (off / (tol + 1e-300)).max()
+
+
+# ------------------------------------------------------------------------------------------------
 # Rows of one sign
 # ------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
